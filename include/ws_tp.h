@@ -237,6 +237,37 @@ ws_status_t ws_fp8_gemm_static_scratch(const ws_fp8_gemm_args_t *args, int32_t d
                                        char *err, size_t err_len);
 ws_status_t ws_fp8_gemm_static_scratch_check(int32_t device, void *stream, char *err, size_t err_len);
 
+/* ---- operators between the steps --------------------------------------------------------------
+ * What an engine does between two reduction points, on the tensors that the steps above take and
+ * return.  They need no endpoint and run on the calling thread's current device.  Types are
+ * WS_ACT_BF16 or WS_ACT_F32, sums and statistics are held in 32 bits.  `err` (optional, err_len bytes)
+ * gets the text of an error.  m = 0 launches nothing. */
+
+/* Norms before and after a block with its gate, residual scale and the residual stream:
+ *   u = y, or with post_weight  y * rsqrt(mean(y^2) + eps) * (weight_offset + post_weight)
+ *   hidden = residual_scale * residual + block_scale * act(gate) * u
+ *   normed = hidden * rsqrt(mean(hidden^2) + eps) * (weight_offset + next_weight), from the unrounded hidden
+ * (takes the place of the reference's `rmsnorm` launches between its blocks). */
+enum { WS_GATE_LINEAR = 0, WS_GATE_SIGMOID = 1 };
+typedef struct {
+    const void *y;            /* [m, n] the block's output, row stride ldy (elements, as all strides)   */
+    int64_t ldy;
+    const void *residual;     /* [m, n] or NULL (no residual)                                           */
+    int64_t ldr;
+    const void *gate;         /* NULL: 1.  gate[row * ldg + i * gate_inc]: ldg 0 shares one row of gates, */
+    int64_t ldg;              /*   gate_inc 0 is one gate a row, 1 one a value                          */
+    const void *post_weight;  /* [n] or NULL: no norm of the block's output                             */
+    const void *next_weight;  /* [n]; needed with normed                                                */
+    void *hidden;             /* [m, n] or NULL; may be `residual` itself                               */
+    int64_t ldh;
+    void *normed;             /* [m, n] or NULL                                                         */
+    int64_t ldn;
+    int32_t m, n, gate_inc, gate_act;
+    int32_t y_dtype, residual_dtype, gate_dtype, weight_dtype, hidden_dtype, normed_dtype;
+    float weight_offset, eps, residual_scale, block_scale;
+} ws_block_norm_args_t;
+ws_status_t ws_block_norm(const ws_block_norm_args_t *args, void *stream, char *err, size_t err_len);
+
 const char *ws_version(void);
 
 #ifdef __cplusplus

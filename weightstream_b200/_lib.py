@@ -16,6 +16,7 @@ WS_OK = 0
 WS_ERR_INVALID, WS_ERR_CUDA, WS_ERR_TIMEOUT, WS_ERR_SEQUENCE, WS_ERR_CAPACITY, WS_ERR_UNSUPPORTED = -1, -2, -3, -4, -5, -6
 WS_SCALE_UE8M0, WS_SCALE_F32 = 0, 1
 WS_ACT_BF16, WS_ACT_F32 = 0, 1
+WS_GATE_LINEAR, WS_GATE_SIGMOID = 0, 1
 
 STATUS_NAMES = {0: "WS_OK", -1: "WS_ERR_INVALID", -2: "WS_ERR_CUDA", -3: "WS_ERR_TIMEOUT",
                 -4: "WS_ERR_SEQUENCE", -5: "WS_ERR_CAPACITY", -6: "WS_ERR_UNSUPPORTED"}
@@ -30,7 +31,8 @@ EXPORTS = [
     "ws_lm_head_allgather_argmax", "ws_lm_head_allgather_argmax_group",
     "ws_allreduce_f32", "ws_allgather_f32", "ws_allreduce_f32_group", "ws_allgather_f32_group",
     "ws_allreduce_f32_host", "ws_allgather_f32_host", "ws_fp8_rowpar_gemm_allreduce_host",
-    "ws_act_quant_fp8", "ws_tp_set_split", "ws_tp_set_kernel", "ws_fp8_gemm_static_scratch", "ws_fp8_gemm_static_scratch_check", "ws_version",
+    "ws_act_quant_fp8", "ws_tp_set_split", "ws_tp_set_kernel", "ws_fp8_gemm_static_scratch", "ws_fp8_gemm_static_scratch_check",
+    "ws_block_norm", "ws_version",
 ]
 
 
@@ -69,6 +71,16 @@ class MoeDownArgs(C.Structure):
 class LmHeadArgs(C.Structure):
     _fields_ = [("g", Fp8GemmArgs), ("vocab_row0", C.c_int64), ("vocab", C.c_int32),
                 ("reserved", C.c_int32), ("logits", C.c_void_p), ("argmax", C.c_void_p)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [("y", C.c_void_p), ("ldy", C.c_int64), ("residual", C.c_void_p), ("ldr", C.c_int64),
+                ("gate", C.c_void_p), ("ldg", C.c_int64), ("post_weight", C.c_void_p), ("next_weight", C.c_void_p),
+                ("hidden", C.c_void_p), ("ldh", C.c_int64), ("normed", C.c_void_p), ("ldn", C.c_int64),
+                ("m", C.c_int32), ("n", C.c_int32), ("gate_inc", C.c_int32), ("gate_act", C.c_int32),
+                ("y_dtype", C.c_int32), ("residual_dtype", C.c_int32), ("gate_dtype", C.c_int32),
+                ("weight_dtype", C.c_int32), ("hidden_dtype", C.c_int32), ("normed_dtype", C.c_int32),
+                ("weight_offset", C.c_float), ("eps", C.c_float), ("residual_scale", C.c_float), ("block_scale", C.c_float)]
 
 
 _lib = None
@@ -162,5 +174,8 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     L.ws_fp8_gemm_static_scratch.argtypes = [C.POINTER(Fp8GemmArgs), C.c_int32, P, C.c_char_p, C.c_size_t]
     L.ws_fp8_gemm_static_scratch_check.restype = st
     L.ws_fp8_gemm_static_scratch_check.argtypes = [C.c_int32, P, C.c_char_p, C.c_size_t]
+    for name, args in (("ws_block_norm", BlockNormArgs),):
+        getattr(L, name).restype = st
+        getattr(L, name).argtypes = [C.POINTER(args), P, C.c_char_p, C.c_size_t]
     _lib = L
     return L

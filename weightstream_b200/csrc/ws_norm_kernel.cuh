@@ -1,0 +1,93 @@
+// Norms before and after a block, with its gate, residual scale and the residual stream, one launch.
+//
+//   u = y                                       or  y * rsqrt(mean(y^2) + eps) * (o + w_post)
+//   h = residual_scale * residual + block_scale * act(gate) * u
+//   z = h * rsqrt(mean(h^2) + eps) * (o + w_next)
+//
+// All of it is held in 32 bits between the loads and the one rounding of h and of z to their types; z is taken from the
+// unrounded h.
+#pragma once
+
+#include "ws_device.cuh"
+
+namespace ws {
+
+struct NormParams {
+    const void *y, *residual, *gate, *post_weight, *next_weight;
+    void *hidden, *normed;
+    int64_t ldy, ldr, ldg, ldh, ldn;   // elements a row; ldg 0: one gate for all rows
+    int32_t m, n;
+    int32_t gate_inc;                  // 1: a gate a value, 0: a gate a row
+    int32_t y_dtype, r_dtype, g_dtype, w_dtype, h_dtype, n_dtype, gate_act;
+    float weight_offset, eps, residual_scale, block_scale;
+};
+
+__device__ __forceinline__ float load1(const void *p, int dtype, int64_t i) {
+    if (dtype == WS_ACT_F32) return static_cast<const float *>(p)[i];
+    return __uint_as_float((uint32_t)static_cast<const uint16_t *>(p)[i] << 16);
+}
+__device__ __forceinline__ uint32_t bf16_bits(float v) {  // to nearest even
+    uint16_t b;
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(b) : "f"(v));
+    return b;
+}
+__device__ __forceinline__ void store1(void *p, int dtype, int64_t i, float v) {
+    if (dtype == WS_ACT_F32) static_cast<float *>(p)[i] = v;
+    else static_cast<uint16_t *>(p)[i] = (uint16_t)bf16_bits(v);
+}
+__device__ __forceinline__ float gate_value(float g, int act) { return act == WS_GATE_SIGMOID ? __fdividef(1.0f, 1.0f + __expf(-g)) : g; }
+
+// The block's sum of v, the same on all threads.  `slot`: 32 floats of shared memory that the previous sum did not use.
+__device__ __forceinline__ float block_sum(float v, float *slot) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) slot[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < warps ? slot[lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Any width, any alignment: a block a row, three passes over it (L2 serves the second and third).  The last pass reads
+// each value and writes its results on one thread, so that the stream may be updated in place.
+__global__ void __launch_bounds__(512) block_norm_any_kernel(const __grid_constant__ NormParams p) {
+    __shared__ float slots[64];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_predecessor();
+    const int64_t row = blockIdx.x;
+    const float inv_n = 1.0f / (float)p.n;
+    float post = 1.0f;
+    if (p.post_weight) {
+        float s = 0.0f;
+        for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
+            const float v = load1(p.y, p.y_dtype, row * p.ldy + i);
+            s = fmaf(v, v, s);
+        }
+        post = rsqrtf(fmaf(block_sum(s, slots), inv_n, p.eps));
+    }
+    auto value = [&](int i) {
+        float u = load1(p.y, p.y_dtype, row * p.ldy + i);
+        if (p.post_weight) u *= post * (p.weight_offset + load1(p.post_weight, p.w_dtype, i));
+        u *= p.block_scale;
+        if (p.gate) u *= gate_value(load1(p.gate, p.g_dtype, row * p.ldg + (int64_t)i * p.gate_inc), p.gate_act);
+        return p.residual ? fmaf(p.residual_scale, load1(p.residual, p.r_dtype, row * p.ldr + i), u) : u;
+    };
+    float next = 0.0f;
+    if (p.normed) {
+        float s = 0.0f;
+        for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
+            const float h = value(i);
+            s = fmaf(h, h, s);
+        }
+        next = rsqrtf(fmaf(block_sum(s, slots + 32), inv_n, p.eps));
+    }
+    for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
+        const float h = value(i);
+        if (p.hidden) store1(p.hidden, p.h_dtype, row * p.ldh + i, h);
+        if (p.normed) store1(p.normed, p.n_dtype, row * p.ldn + i, h * next * (p.weight_offset + load1(p.next_weight, p.w_dtype, i)));
+    }
+}
+
+}  // namespace ws

@@ -10,8 +10,12 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <optional>
 
 #include <vector>
 
@@ -263,8 +267,121 @@ PyObject *py_fp8_group(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- operators between the steps.  An error's text is the Python layer's to give: it gets None and makes the same call.
+//
+// Device and stream of a call.  What is allocated meanwhile belongs to the stream that writes it.
+struct CallOn {
+    c10::cuda::CUDAGuard device;
+    std::optional<c10::cuda::CUDAStreamGuard> guard;
+    void *stream;
+    CallOn(const at::Tensor &t, PyObject *o) : device(t.device()) {
+        if (o != Py_None) {
+            stream = PyLong_AsVoidPtr(o);
+            guard.emplace(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(stream), t.device().index()));
+        } else {
+            stream = c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+        }
+    }
+};
+
+// A [m, n] tensor of rows that are stored one value after the other, on the device of `like`.
+bool rows(const at::Tensor *t, const at::Tensor &like, int64_t m, int64_t n, int64_t *ld) {
+    if (!t || t->dim() != 2 || t->size(0) != m || t->size(1) != n || t->device() != like.device()) return false;
+    if ((n > 1 && t->stride(1) != 1) || (m > 1 && t->stride(0) < n)) return false;
+    *ld = m > 1 ? t->stride(0) : n;
+    return true;
+}
+bool vec(const at::Tensor *t, const at::Tensor &like, int64_t n) {
+    return t && t->dim() == 1 && t->size(0) == n && t->is_contiguous() && t->device() == like.device();
+}
+// A result type as Python names it; None stands for `otherwise`.
+bool result_dtype(PyObject *o, at::ScalarType otherwise, at::ScalarType *out, int32_t *code) {
+    if (o != Py_None && !THPDtype_Check(o)) return false;
+    *out = o == Py_None ? otherwise : reinterpret_cast<THPDtype *>(o)->scalar_type;
+    *code = *out == at::kFloat ? WS_ACT_F32 : WS_ACT_BF16;
+    return *out == at::kFloat || *out == at::kBFloat16;
+}
+at::Tensor new_like(const at::Tensor &like, at::IntArrayRef sizes, at::ScalarType t) {
+    return at::empty(sizes, like.options().dtype(t).requires_grad(false));
+}
+
+// block_norm(y, residual, post_weight, next_weight, gate, gate_act, eps, weight_offset, residual_scale, block_scale, out,
+//            out_dtype, normed_dtype, stream) -> (hidden, normed | None)
+PyObject *py_block_norm(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 14) { PyErr_SetString(PyExc_TypeError, "block_norm takes 14 arguments"); return nullptr; }
+    const at::Tensor *y = tensor(v[0]);
+    if (!y || y->dim() != 2) Py_RETURN_NONE;
+    ws_block_norm_args_t a{};
+    const int64_t m = y->size(0), n = y->size(1);
+    if (m > INT32_MAX || n > INT32_MAX || !rows(y, *y, m, n, &a.ldy) || !act_dtype(*y, &a.y_dtype)) Py_RETURN_NONE;
+    a.m = (int32_t)m; a.n = (int32_t)n; a.y = y->data_ptr();
+    at::ScalarType hidden_type = at::kBFloat16, normed_type;
+    if (v[1] != Py_None) {
+        const at::Tensor *r = tensor(v[1]);
+        if (!rows(r, *y, m, n, &a.ldr) || !act_dtype(*r, &a.residual_dtype)) Py_RETURN_NONE;
+        a.residual = r->data_ptr();
+        hidden_type = r->scalar_type();
+    }
+    const void **weights[2] = {&a.post_weight, &a.next_weight};
+    int32_t seen = -1;
+    for (int i = 0; i < 2; ++i) {
+        if (v[2 + i] == Py_None) continue;
+        const at::Tensor *w = tensor(v[2 + i]);
+        if (!vec(w, *y, n) || !act_dtype(*w, &a.weight_dtype) || (seen >= 0 && seen != a.weight_dtype)) Py_RETURN_NONE;
+        seen = a.weight_dtype;
+        *weights[i] = w->data_ptr();
+    }
+    a.gate_act = (int32_t)PyLong_AsLong(v[5]);
+    if (v[4] != Py_None) {
+        const at::Tensor *g = tensor(v[4]);
+        if (!g || g->device() != y->device() || g->dim() < 1 || g->dim() > 2 || !act_dtype(*g, &a.gate_dtype)) Py_RETURN_NONE;
+        const bool two = g->dim() == 2;
+        const int64_t gm = two ? g->size(0) : 1, gn = g->size(two ? 1 : 0), inc = g->stride(two ? 1 : 0);
+        if ((gm != 1 && gm != m) || (gn != 1 && gn != n) || (gn > 1 && inc != 0 && inc != 1)) Py_RETURN_NONE;
+        a.gate = g->data_ptr();
+        a.ldg = gm > 1 ? g->stride(0) : 0;
+        a.gate_inc = gn > 1 ? (int32_t)inc : 0;
+    }
+    a.eps = (float)PyFloat_AsDouble(v[6]); a.weight_offset = (float)PyFloat_AsDouble(v[7]);
+    a.residual_scale = (float)PyFloat_AsDouble(v[8]); a.block_scale = (float)PyFloat_AsDouble(v[9]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!result_dtype(v[11], hidden_type, &hidden_type, &a.hidden_dtype) || !result_dtype(v[12], at::kBFloat16, &normed_type, &a.normed_dtype))
+        Py_RETURN_NONE;
+    CallOn on(*y, v[13]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor hidden, normed;
+    if (v[10] != Py_None) {
+        const at::Tensor *out = tensor(v[10]);
+        if (!rows(out, *y, m, n, &a.ldh) || !act_dtype(*out, &a.hidden_dtype)) Py_RETURN_NONE;
+        a.hidden = out->data_ptr();
+    } else {
+        hidden = new_like(*y, {m, n}, hidden_type);
+        a.hidden = hidden.data_ptr();
+        a.ldh = n;
+    }
+    if (a.next_weight) {
+        normed = new_like(*y, {m, n}, normed_type);
+        a.normed = normed.data_ptr();
+        a.ldn = n;
+    }
+    WS_CALL(st, ws_block_norm(&a, on.stream, nullptr, 0))
+    if (st != WS_OK) Py_RETURN_NONE;
+    PyObject *first = v[10], *second = Py_None;
+    if (hidden.defined()) first = THPVariable_Wrap(std::move(hidden));
+    else Py_INCREF(first);
+    if (normed.defined()) second = THPVariable_Wrap(std::move(normed));
+    else Py_INCREF(second);
+    PyObject *pair = PyTuple_Pack(2, first, second);
+    Py_DECREF(first);
+    Py_DECREF(second);
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
 #define WS_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {WS_METHOD(fp8), WS_METHOD(fp8_host), WS_METHOD(moe), WS_METHOD(head), WS_METHOD(fp8_group), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {WS_METHOD(fp8), WS_METHOD(fp8_host), WS_METHOD(moe), WS_METHOD(head), WS_METHOD(fp8_group), WS_METHOD(block_norm),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_ws_torch", "torch tensors -> libws_tp.so", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

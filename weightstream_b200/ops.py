@@ -1,0 +1,165 @@
+"""Operators between the tensor-parallel steps, on the tensors that the steps take and return.
+
+A decode engine does more between two reduction points than the steps of :mod:`weightstream_b200.tp`: it normalises a
+block's output, gates it, adds it to the residual stream and normalises that for the next block (:func:`block_norm`).
+
+Every function runs on the GPU that holds its tensors, on ``stream`` or the current stream, and does not synchronise.
+Results are allocated on that stream.  A tensor that a call reads has to live until the stream has passed the call, as
+with torch's own operators.  Wrong arguments raise ``TypeError`` or ``ValueError`` before anything is launched.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import BlockNormArgs, WsError, WS_ACT_BF16, WS_ACT_F32, WS_GATE_LINEAR, WS_GATE_SIGMOID, WS_OK
+
+_TYPES = {torch.bfloat16: WS_ACT_BF16, torch.float32: WS_ACT_F32}
+_GATES = {"none": WS_GATE_LINEAR, "sigmoid": WS_GATE_SIGMOID}
+
+
+def _code(t: torch.Tensor, name: str) -> int:
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise TypeError(f"{name} must be bf16 or fp32, got {t.dtype}") from None
+
+
+def _rows(t: torch.Tensor, name: str, m: int, n: int) -> int:
+    """Row stride of a [m, n] tensor whose rows are stored one value after the other."""
+    if t.dim() != 2 or t.shape[0] != m or t.shape[1] != n:
+        raise ValueError(f"{name} must be [{m}, {n}], got {list(t.shape)}")
+    if n > 1 and t.stride(1) != 1 and m:
+        raise ValueError(f"{name} needs unit inner stride")
+    if m > 1 and t.stride(0) < n:
+        raise ValueError(f"{name}: rows of {n} values lie {t.stride(0)} apart")
+    return t.stride(0) if m > 1 else n
+
+
+def _vector(t: torch.Tensor, name: str, n: int, dtype=None) -> None:
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of {n} values, got {list(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _same_device(first: torch.Tensor, *others) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+def _on(device: torch.device, stream):
+    """Current device and stream of a call: what it allocates belongs to the stream that writes it."""
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, got {device}")
+    both = contextlib.ExitStack()
+    both.enter_context(torch.cuda.device(device))
+    if stream is not None:
+        both.enter_context(torch.cuda.stream(stream))
+    return both
+
+
+def _call(name: str, args) -> None:
+    L, err = _lib.load(), C.create_string_buffer(256)
+    st = getattr(L, name)(C.byref(args), int(torch.cuda.current_stream().cuda_stream), err, len(err))
+    if st != WS_OK:
+        raise WsError(st, err.value.decode())
+
+
+def _handle(stream) -> Optional[int]:
+    return None if stream is None else int(stream.cuda_stream)
+
+
+def _dim(*sizes: int) -> None:
+    for v in sizes:
+        if v >= 2 ** 31:
+            raise ValueError(f"a dimension of {v} is beyond 31 bits")
+
+
+# ----------------------------------------------------------------------------- norms around a block
+def _block_norm_args(y, residual, post_weight, next_weight, gate, gate_act, eps, weight_offset, residual_scale, block_scale,
+                     out, out_dtype, normed_dtype) -> Tuple[BlockNormArgs, torch.dtype, torch.dtype]:
+    if y.dim() != 2 or y.shape[1] < 1:
+        raise ValueError(f"y must be [m, n] with n >= 1, got {list(y.shape)}")
+    m, n = y.shape
+    _dim(m, n)
+    a = BlockNormArgs()
+    a.m, a.n = m, n
+    a.y, a.ldy, a.y_dtype = y.data_ptr(), _rows(y, "y", m, n), _code(y, "y")
+    if residual is not None:
+        a.residual, a.ldr, a.residual_dtype = residual.data_ptr(), _rows(residual, "residual", m, n), _code(residual, "residual")
+    if gate_act not in _GATES:
+        raise ValueError(f"gate_act must be one of {sorted(_GATES)}, got {gate_act!r}")
+    if gate is not None:
+        if gate.dim() not in (1, 2):
+            raise ValueError("gate must be [n], [m, 1] or [m, n]")
+        g = gate if gate.dim() == 2 else gate.unsqueeze(0)
+        if g.shape[0] not in (1, m) or g.shape[1] not in (1, n):
+            raise ValueError(f"gate must be [{n}], [{m}, 1] or [{m}, {n}], got {list(gate.shape)}")
+        if g.shape[1] > 1 and g.stride(1) not in (0, 1):
+            raise ValueError("gate needs unit inner stride")
+        a.gate, a.gate_dtype, a.gate_act = g.data_ptr(), _code(gate, "gate"), _GATES[gate_act]
+        a.ldg = g.stride(0) if g.shape[0] > 1 else 0
+        a.gate_inc = g.stride(1) if g.shape[1] > 1 else 0
+    weights = [(w, name) for w, name in ((post_weight, "post_weight"), (next_weight, "next_weight")) if w is not None]
+    for w, name in weights:
+        _vector(w, name, n)
+        a.weight_dtype = _code(w, name)
+    if len(weights) == 2 and post_weight.dtype != next_weight.dtype:
+        raise TypeError("post_weight and next_weight must have one type")
+    a.post_weight = post_weight.data_ptr() if post_weight is not None else None
+    a.next_weight = next_weight.data_ptr() if next_weight is not None else None
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    a.eps, a.weight_offset, a.residual_scale, a.block_scale = eps, weight_offset, residual_scale, block_scale
+    hidden = out.dtype if out is not None else out_dtype or (residual.dtype if residual is not None else torch.bfloat16)
+    if out is not None:
+        a.hidden, a.ldh = out.data_ptr(), _rows(out, "out", m, n)
+    for dtype in (hidden, normed_dtype):
+        if dtype not in _TYPES:
+            raise TypeError(f"results are bf16 or fp32, not {dtype}")
+    a.hidden_dtype, a.normed_dtype = _TYPES[hidden], _TYPES[normed_dtype]
+    _same_device(y, residual, gate, post_weight, next_weight, out)
+    return a, hidden, normed_dtype
+
+
+def block_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post_weight: Optional[torch.Tensor] = None,
+               next_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, gate_act: str = "none",
+               eps: float = 1e-6, weight_offset: float = 0.0, residual_scale: float = 1.0, block_scale: float = 1.0,
+               out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+               normed_dtype: torch.dtype = torch.bfloat16, stream=None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Norms before and after a block, its gate, its residual scale and the residual stream, in one launch.
+
+    ``y`` [m, n] is what the block returned (the fp32 sums of a reduction point, or bf16)::
+
+        u      = y                                  with post_weight: y * rsqrt(mean(y^2) + eps) * (weight_offset + post_weight)
+        hidden = residual_scale * residual + block_scale * act(gate) * u
+        normed = hidden * rsqrt(mean(hidden^2) + eps) * (weight_offset + next_weight)
+
+    ``gate`` is one value per channel ([n]), per token ([m, 1]) or per element ([m, n]); ``gate_act`` is ``"none"`` or
+    ``"sigmoid"``.  ``weight_offset`` is 1 for models that keep their norm weights as a difference from one.  Everything
+    between the loads and the results is held in 32 bits; ``normed`` is taken from ``hidden`` before it is rounded.
+
+    Returns ``(hidden, normed)``; ``normed`` is None without ``next_weight``.  ``hidden`` has the residual's type, or
+    ``out_dtype``; ``out`` takes it and may be ``residual`` itself.
+    """
+    r = _lib.torch_front().block_norm(y, residual, post_weight, next_weight, gate, _GATES.get(gate_act, -1), eps, weight_offset,
+                                      residual_scale, block_scale, out, out_dtype, normed_dtype, _handle(stream))
+    if r is not None:
+        return r
+    a, hidden_dtype, normed_dtype = _block_norm_args(y, residual, post_weight, next_weight, gate, gate_act, eps, weight_offset,
+                                                     residual_scale, block_scale, out, out_dtype, normed_dtype)
+    with _on(y.device, stream):
+        hidden = out if out is not None else torch.empty((a.m, a.n), dtype=hidden_dtype, device=y.device)
+        a.hidden, a.ldh = hidden.data_ptr(), a.ldh or a.n
+        normed = None
+        if next_weight is not None:
+            normed = torch.empty((a.m, a.n), dtype=normed_dtype, device=y.device)
+            a.normed, a.ldn = normed.data_ptr(), a.n
+        _call("ws_block_norm", a)
+    return hidden, normed
