@@ -268,6 +268,28 @@ typedef struct {
 } ws_block_norm_args_t;
 ws_status_t ws_block_norm(const ws_block_norm_args_t *args, void *stream, char *err, size_t err_len);
 
+/* Scores of one given token a row on the vocabulary head's logits:
+ *   lse = log sum exp(logits);  logprob = logits[token] - lse;  entropy = lse - sum softmax(logits) * logits
+ *   rank = how many entries come before the token, larger ones first and equal ones by index (0: it is the argmax)
+ *   top_id, top_logprob: the `top` entries that come first; masked (-inf) and NaN logits are never among them,
+ *   places that stay empty hold -1 and -inf.
+ * A token outside [0, vocab) is none: logprob 0, rank -1.  A row that is masked whole has logprob -inf, entropy 0.
+ * NaN or +inf in a row make its logprob, entropy and top_logprob NaN; a token whose own logit is NaN has rank -1.
+ * Order of the entries as in argmax (crates/weightstream-ref/src/sample.rs:13-23). */
+#define WS_MAX_TOP 32
+typedef struct {
+    const void *logits;       /* [m, vocab], row stride ld (elements)   */
+    int64_t ld;
+    const void *tokens;       /* [m] int32 or int64 (token_bytes 4 or 8) */
+    float *logprob;           /* [m]                                     */
+    float *entropy;           /* [m]                                     */
+    int32_t *rank;            /* [m]                                     */
+    int32_t *top_id;          /* [m, top], NULL with top = 0             */
+    float *top_logprob;       /* [m, top], NULL with top = 0             */
+    int32_t m, vocab, top, dtype, token_bytes, reserved;
+} ws_token_logprobs_args_t;
+ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *args, void *stream, char *err, size_t err_len);
+
 const char *ws_version(void);
 
 #ifdef __cplusplus

@@ -17,6 +17,7 @@ WS_ERR_INVALID, WS_ERR_CUDA, WS_ERR_TIMEOUT, WS_ERR_SEQUENCE, WS_ERR_CAPACITY, W
 WS_SCALE_UE8M0, WS_SCALE_F32 = 0, 1
 WS_ACT_BF16, WS_ACT_F32 = 0, 1
 WS_GATE_LINEAR, WS_GATE_SIGMOID = 0, 1
+WS_MAX_TOP = 32
 
 STATUS_NAMES = {0: "WS_OK", -1: "WS_ERR_INVALID", -2: "WS_ERR_CUDA", -3: "WS_ERR_TIMEOUT",
                 -4: "WS_ERR_SEQUENCE", -5: "WS_ERR_CAPACITY", -6: "WS_ERR_UNSUPPORTED"}
@@ -32,7 +33,7 @@ EXPORTS = [
     "ws_allreduce_f32", "ws_allgather_f32", "ws_allreduce_f32_group", "ws_allgather_f32_group",
     "ws_allreduce_f32_host", "ws_allgather_f32_host", "ws_fp8_rowpar_gemm_allreduce_host",
     "ws_act_quant_fp8", "ws_tp_set_split", "ws_tp_set_kernel", "ws_fp8_gemm_static_scratch", "ws_fp8_gemm_static_scratch_check",
-    "ws_block_norm", "ws_version",
+    "ws_block_norm", "ws_token_logprobs", "ws_version",
 ]
 
 
@@ -81,6 +82,13 @@ class BlockNormArgs(C.Structure):
                 ("y_dtype", C.c_int32), ("residual_dtype", C.c_int32), ("gate_dtype", C.c_int32),
                 ("weight_dtype", C.c_int32), ("hidden_dtype", C.c_int32), ("normed_dtype", C.c_int32),
                 ("weight_offset", C.c_float), ("eps", C.c_float), ("residual_scale", C.c_float), ("block_scale", C.c_float)]
+
+
+class TokenLogprobsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("tokens", C.c_void_p), ("logprob", C.c_void_p),
+                ("entropy", C.c_void_p), ("rank", C.c_void_p), ("top_id", C.c_void_p), ("top_logprob", C.c_void_p),
+                ("m", C.c_int32), ("vocab", C.c_int32), ("top", C.c_int32), ("dtype", C.c_int32),
+                ("token_bytes", C.c_int32), ("reserved", C.c_int32)]
 
 
 _lib = None
@@ -174,7 +182,7 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     L.ws_fp8_gemm_static_scratch.argtypes = [C.POINTER(Fp8GemmArgs), C.c_int32, P, C.c_char_p, C.c_size_t]
     L.ws_fp8_gemm_static_scratch_check.restype = st
     L.ws_fp8_gemm_static_scratch_check.argtypes = [C.c_int32, P, C.c_char_p, C.c_size_t]
-    for name, args in (("ws_block_norm", BlockNormArgs),):
+    for name, args in (("ws_block_norm", BlockNormArgs), ("ws_token_logprobs", TokenLogprobsArgs)):
         getattr(L, name).restype = st
         getattr(L, name).argtypes = [C.POINTER(args), P, C.c_char_p, C.c_size_t]
     _lib = L

@@ -5,6 +5,7 @@
 #include <cstdio>
 
 #include "ws_norm_kernel.cuh"
+#include "ws_scores_kernel.cuh"
 
 using namespace ws;
 
@@ -85,6 +86,34 @@ ws_status_t ws_block_norm(const ws_block_norm_args_t *a, void *stream, char *err
     p.weight_offset = a->weight_offset; p.eps = a->eps; p.residual_scale = a->residual_scale; p.block_scale = a->block_scale;
     const unsigned threads = (unsigned)std::min(512, (p.n + 31) / 32 * 32);
     return launch(err, block_norm_any_kernel, dim3((unsigned)p.m), threads, 0, 1, stream, p);
+}
+
+ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *a, void *stream, char *err_text, size_t err_len) {
+    const Err err{err_text, err_len};
+    if (err_text && err_len) err_text[0] = 0;
+    if (!a) return err(WS_ERR_INVALID, "null args");
+    // (the kernel counts a row's values in 32 bits, up to a vector and a batch of vectors past its end)
+    if (a->m < 0 || a->m > INT32_MAX / kScoreMaxCluster || a->vocab < 1 || a->vocab > INT32_MAX - (1 << 16))
+        return err(WS_ERR_INVALID, "m=%d vocab=%d out of range", a->m, a->vocab);
+    if (a->top < 0 || a->top > WS_MAX_TOP) return err(WS_ERR_INVALID, "top=%d is not in 0..%d", a->top, WS_MAX_TOP);
+    if (!is_type(a->dtype) || (a->token_bytes != 4 && a->token_bytes != 8)) return err(WS_ERR_INVALID, "unknown type of a tensor");
+    if (a->m == 0) return WS_OK;
+    if (!a->logits || !a->tokens || !a->logprob || !a->entropy || !a->rank || (a->top && (!a->top_id || !a->top_logprob)))
+        return err(WS_ERR_INVALID, "a tensor is missing");
+    if (a->ld < a->vocab) return err(WS_ERR_INVALID, "the row stride %lld is shorter than the row of %d values", (long long)a->ld, a->vocab);
+    if (!natural(a->logits, a->dtype) || reinterpret_cast<uintptr_t>(a->tokens) % a->token_bytes)
+        return err(WS_ERR_INVALID, "a tensor is not aligned to its type");
+    ScoreParams p{};
+    p.logits = a->logits; p.tokens = a->tokens; p.ld = a->ld; p.m = a->m; p.vocab = a->vocab; p.top = a->top; p.token_bytes = a->token_bytes;
+    p.logprob = a->logprob; p.entropy = a->entropy; p.top_logprob = a->top_logprob; p.rank = a->rank; p.top_id = a->top_id;
+    const int per = (a->dtype == WS_ACT_F32 ? 4 : 8) * kScoreThreads;  // values of one round of a block
+    int c = 1;
+    while (c < kScoreMaxCluster && (int64_t)a->m * c * 2 <= 2 * 148 && a->vocab / (2 * c) >= per) c *= 2;
+    p.cluster = c;
+    const dim3 grid((unsigned)a->m * c);
+    auto *k = a->dtype == WS_ACT_F32 ? (a->top ? token_scores_kernel<true, true> : token_scores_kernel<true, false>)
+                                     : (a->top ? token_scores_kernel<false, true> : token_scores_kernel<false, false>);
+    return launch(err, k, grid, kScoreThreads, 0, (unsigned)c, stream, p);
 }
 
 }  // extern "C"

@@ -379,8 +379,44 @@ PyObject *py_block_norm(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// token_logprobs(logits, tokens, top, stream) -> (logprobs, entropy, rank, top_ids | None, top_logprobs | None)
+PyObject *py_token_logprobs(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 4) { PyErr_SetString(PyExc_TypeError, "token_logprobs takes 4 arguments"); return nullptr; }
+    const at::Tensor *x = tensor(v[0]), *tok = tensor(v[1]);
+    const long top = PyLong_AsLong(v[2]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!x || !tok || x->dim() != 2 || top < 0 || top > WS_MAX_TOP) Py_RETURN_NONE;
+    ws_token_logprobs_args_t a{};
+    const int64_t m = x->size(0), vocab = x->size(1);
+    if (m > INT32_MAX || vocab > INT32_MAX || !rows(x, *x, m, vocab, &a.ld) || !act_dtype(*x, &a.dtype) || !vec(tok, *x, m)) Py_RETURN_NONE;
+    if (tok->scalar_type() != at::kInt && tok->scalar_type() != at::kLong) Py_RETURN_NONE;
+    a.logits = x->data_ptr(); a.tokens = tok->data_ptr(); a.token_bytes = (int32_t)tok->element_size();
+    a.m = (int32_t)m; a.vocab = (int32_t)vocab; a.top = (int32_t)top;
+    CallOn on(*x, v[3]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor out[5];
+    out[0] = new_like(*x, {m}, at::kFloat); out[1] = new_like(*x, {m}, at::kFloat); out[2] = new_like(*x, {m}, at::kInt);
+    a.logprob = out[0].data_ptr<float>(); a.entropy = out[1].data_ptr<float>(); a.rank = out[2].data_ptr<int32_t>();
+    if (top) {
+        out[3] = new_like(*x, {m, top}, at::kInt); out[4] = new_like(*x, {m, top}, at::kFloat);
+        a.top_id = out[3].data_ptr<int32_t>(); a.top_logprob = out[4].data_ptr<float>();
+    }
+    WS_CALL(st, ws_token_logprobs(&a, on.stream, nullptr, 0))
+    if (st != WS_OK) Py_RETURN_NONE;
+    PyObject *res = PyTuple_New(5);
+    for (int i = 0; res && i < 5; ++i) {
+        PyObject *o = Py_None;
+        if (out[i].defined()) o = THPVariable_Wrap(std::move(out[i]));
+        else Py_INCREF(o);
+        PyTuple_SET_ITEM(res, i, o);
+    }
+    return res;
+    END_HANDLE_TH_ERRORS
+}
+
 #define WS_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {WS_METHOD(fp8), WS_METHOD(fp8_host), WS_METHOD(moe), WS_METHOD(head), WS_METHOD(fp8_group), WS_METHOD(block_norm),
+PyMethodDef methods[] = {WS_METHOD(fp8), WS_METHOD(fp8_host), WS_METHOD(moe), WS_METHOD(head), WS_METHOD(fp8_group), WS_METHOD(block_norm), WS_METHOD(token_logprobs),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_ws_torch", "torch tensors -> libws_tp.so", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

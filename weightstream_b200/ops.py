@@ -1,7 +1,8 @@
 """Operators between the tensor-parallel steps, on the tensors that the steps take and return.
 
 A decode engine does more between two reduction points than the steps of :mod:`weightstream_b200.tp`: it normalises a
-block's output, gates it, adds it to the residual stream and normalises that for the next block (:func:`block_norm`).
+block's output, gates it, adds it to the residual stream and normalises that for the next block (:func:`block_norm`),
+and it scores given tokens on the vocabulary head's logits (:func:`token_logprobs`).
 
 Every function runs on the GPU that holds its tensors, on ``stream`` or the current stream, and does not synchronise.
 Results are allocated on that stream.  A tensor that a call reads has to live until the stream has passed the call, as
@@ -11,12 +12,12 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import BlockNormArgs, WsError, WS_ACT_BF16, WS_ACT_F32, WS_GATE_LINEAR, WS_GATE_SIGMOID, WS_OK
+from ._lib import BlockNormArgs, TokenLogprobsArgs, WsError, WS_ACT_BF16, WS_ACT_F32, WS_GATE_LINEAR, WS_GATE_SIGMOID, WS_MAX_TOP, WS_OK
 
 _TYPES = {torch.bfloat16: WS_ACT_BF16, torch.float32: WS_ACT_F32}
 _GATES = {"none": WS_GATE_LINEAR, "sigmoid": WS_GATE_SIGMOID}
@@ -163,3 +164,56 @@ def block_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post
             a.normed, a.ldn = normed.data_ptr(), a.n
         _call("ws_block_norm", a)
     return hidden, normed
+
+
+# ----------------------------------------------------------------------------- scores of given tokens
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor                    # [m] fp32
+    entropy: torch.Tensor                     # [m] fp32, in nats
+    rank: torch.Tensor                        # [m] int32
+    top_ids: Optional[torch.Tensor]           # [m, top] int32, None with top = 0
+    top_logprobs: Optional[torch.Tensor]      # [m, top] fp32, None with top = 0
+
+
+def _token_logprobs_args(logits, tokens, top) -> TokenLogprobsArgs:
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be [m, vocab] with vocab >= 1, got {list(logits.shape)}")
+    m, vocab = logits.shape
+    _dim(m, vocab)
+    a = TokenLogprobsArgs()
+    a.m, a.vocab = m, vocab
+    a.logits, a.ld, a.dtype = logits.data_ptr(), _rows(logits, "logits", m, vocab), _code(logits, "logits")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"tokens must be int32 or int64, got {tokens.dtype}")
+    _vector(tokens, "tokens", m)
+    a.tokens, a.token_bytes = tokens.data_ptr(), tokens.element_size()
+    if not 0 <= top <= WS_MAX_TOP:
+        raise ValueError(f"top must be in 0..{WS_MAX_TOP}, got {top}")
+    a.top = top
+    _same_device(logits, tokens)
+    return a
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, stream=None) -> TokenLogprobs:
+    """Log probability of one given token a row, with the distribution's entropy, the token's rank and the ``top`` best
+    alternatives, from one pass over the logits [m, vocab] (fp32 as ``lm_head_allgather_argmax`` returns them, or bf16).
+
+    ``rank`` is the number of entries that come before the token, larger logits first and equal ones by index (0: the
+    token is the argmax); ``top_ids`` holds the first ``top`` (at most 32) entries in that order.  Masked (-inf) and NaN
+    logits are never alternatives; places that stay empty hold id -1 and log probability -inf.  A token outside
+    [0, vocab), such as -1 for padding, is none: log probability 0, rank -1.  A row that is masked whole has log
+    probability -inf and entropy 0; NaN or +inf in a row make its log probabilities and entropy NaN.
+    """
+    r = _lib.torch_front().token_logprobs(logits, tokens, top, _handle(stream))
+    if r is not None:
+        return TokenLogprobs(*r)
+    a = _token_logprobs_args(logits, tokens, top)
+    with _on(logits.device, stream):
+        new = lambda *shape, dtype: torch.empty(shape, dtype=dtype, device=logits.device)
+        r = TokenLogprobs(new(a.m, dtype=torch.float32), new(a.m, dtype=torch.float32), new(a.m, dtype=torch.int32),
+                          new(a.m, top, dtype=torch.int32) if top else None, new(a.m, top, dtype=torch.float32) if top else None)
+        a.logprob, a.entropy, a.rank = r.logprobs.data_ptr(), r.entropy.data_ptr(), r.rank.data_ptr()
+        if top:
+            a.top_id, a.top_logprob = r.top_ids.data_ptr(), r.top_logprobs.data_ptr()
+        _call("ws_token_logprobs", a)
+    return r
