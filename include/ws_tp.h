@@ -290,6 +290,36 @@ typedef struct {
 } ws_token_logprobs_args_t;
 ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *args, void *stream, char *err, size_t err_len);
 
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[t] = y[t] + scale[ids[t]] * b[ids[t]] (a[ids[t]] x[t])
+ * Tokens with an id outside [0, adapters), such as -1, have no adapter: out = y, shrunk rows are zeros.
+ * ws_lora_add is the whole; where the projection is sharded over K every rank calls ws_lora_shrink on its slice of x
+ * and of a, the ranks add the shrunk rows up (ws_allreduce_f32) and each calls ws_lora_expand.
+ * The adapters are bf16, the products' sums and the shrunk rows fp32.  Up to 256 tokens need no workspace; more take
+ * ws_lora_workspace(m, adapters) bytes (16-byte aligned) that the call writes first, so calls on one stream may share
+ * it, and at most 16384 adapters (WS_ERR_CAPACITY beyond). */
+#define WS_LORA_MAX_RANK 128
+typedef struct {
+    const void *x;            /* [m, k] activations, row stride ldx                 (add, shrink) */
+    int64_t ldx;
+    const void *y;            /* [m, n] the projection's result, row stride ldy     (add, expand) */
+    int64_t ldy;
+    void *out;                /* [m, n] of y's type, row stride ldo; may be y itself (add, expand) */
+    int64_t ldo;
+    const void *a;            /* [adapters, rank, k] bf16                            (add, shrink) */
+    const void *b;            /* [adapters, n, rank] bf16                            (add, expand) */
+    const int32_t *ids;       /* [m]                                                 (all)         */
+    const float *scale;       /* [adapters], or NULL: 1                              (add, expand) */
+    float *shrunk;            /* [m, rank] fp32          (shrink writes it, expand reads it)       */
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t m, k, n, rank, adapters, x_dtype, y_dtype, reserved;
+} ws_lora_args_t;
+int64_t ws_lora_workspace(int32_t m, int32_t adapters);
+ws_status_t ws_lora_add(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
+ws_status_t ws_lora_shrink(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
+ws_status_t ws_lora_expand(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
+
 const char *ws_version(void);
 
 #ifdef __cplusplus

@@ -18,6 +18,7 @@ WS_SCALE_UE8M0, WS_SCALE_F32 = 0, 1
 WS_ACT_BF16, WS_ACT_F32 = 0, 1
 WS_GATE_LINEAR, WS_GATE_SIGMOID = 0, 1
 WS_MAX_TOP = 32
+WS_LORA_MAX_RANK = 128
 
 STATUS_NAMES = {0: "WS_OK", -1: "WS_ERR_INVALID", -2: "WS_ERR_CUDA", -3: "WS_ERR_TIMEOUT",
                 -4: "WS_ERR_SEQUENCE", -5: "WS_ERR_CAPACITY", -6: "WS_ERR_UNSUPPORTED"}
@@ -33,7 +34,7 @@ EXPORTS = [
     "ws_allreduce_f32", "ws_allgather_f32", "ws_allreduce_f32_group", "ws_allgather_f32_group",
     "ws_allreduce_f32_host", "ws_allgather_f32_host", "ws_fp8_rowpar_gemm_allreduce_host",
     "ws_act_quant_fp8", "ws_tp_set_split", "ws_tp_set_kernel", "ws_fp8_gemm_static_scratch", "ws_fp8_gemm_static_scratch_check",
-    "ws_block_norm", "ws_token_logprobs", "ws_version",
+    "ws_block_norm", "ws_token_logprobs", "ws_lora_workspace", "ws_lora_add", "ws_lora_shrink", "ws_lora_expand", "ws_version",
 ]
 
 
@@ -89,6 +90,15 @@ class TokenLogprobsArgs(C.Structure):
                 ("entropy", C.c_void_p), ("rank", C.c_void_p), ("top_id", C.c_void_p), ("top_logprob", C.c_void_p),
                 ("m", C.c_int32), ("vocab", C.c_int32), ("top", C.c_int32), ("dtype", C.c_int32),
                 ("token_bytes", C.c_int32), ("reserved", C.c_int32)]
+
+
+class LoraArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("ldx", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("out", C.c_void_p), ("ldo", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p),
+                ("ids", C.c_void_p), ("scale", C.c_void_p), ("shrunk", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+                ("m", C.c_int32), ("k", C.c_int32), ("n", C.c_int32), ("rank", C.c_int32), ("adapters", C.c_int32),
+                ("x_dtype", C.c_int32), ("y_dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
 _lib = None
@@ -182,7 +192,10 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     L.ws_fp8_gemm_static_scratch.argtypes = [C.POINTER(Fp8GemmArgs), C.c_int32, P, C.c_char_p, C.c_size_t]
     L.ws_fp8_gemm_static_scratch_check.restype = st
     L.ws_fp8_gemm_static_scratch_check.argtypes = [C.c_int32, P, C.c_char_p, C.c_size_t]
-    for name, args in (("ws_block_norm", BlockNormArgs), ("ws_token_logprobs", TokenLogprobsArgs)):
+    L.ws_lora_workspace.restype = C.c_int64
+    L.ws_lora_workspace.argtypes = [C.c_int32, C.c_int32]
+    for name, args in (("ws_block_norm", BlockNormArgs), ("ws_token_logprobs", TokenLogprobsArgs), ("ws_lora_add", LoraArgs),
+                       ("ws_lora_shrink", LoraArgs), ("ws_lora_expand", LoraArgs)):
         getattr(L, name).restype = st
         getattr(L, name).argtypes = [C.POINTER(args), P, C.c_char_p, C.c_size_t]
     _lib = L

@@ -13,7 +13,7 @@ LIB = os.path.join(HERE, "libws_tp.so")
 TORCH_EXT = os.path.join(HERE, "_ws_torch.so")
 SOURCES = ["ws_api.cu", "ws_bootstrap.cu", "ws_ops.cu"]
 HEADERS = ["ws_device.cuh", "ws_fp8_kernel.cuh", "ws_fp8_gemv_kernel.cuh", "ws_fp8_bs_kernel.cuh", "ws_fp8_tile_kernel.cuh", "ws_moe_kernel.cuh", "ws_moe_gemv_kernel.cuh", "ws_moe_bs_kernel.cuh", "ws_misc_kernels.cuh",
-           "ws_norm_kernel.cuh", "ws_scores_kernel.cuh",
+           "ws_norm_kernel.cuh", "ws_scores_kernel.cuh", "ws_lora_kernel.cuh",
            os.path.join("..", "..", "include", "ws_tp.h")]
 
 

@@ -1,0 +1,406 @@
+// Low-rank adapters of many requests beside a shared projection:  out[t] = y[t] + scale[id] * B[id] (A[id] x[t]).
+//
+// A tile is up to 8 * NT tokens of one adapter.  A cluster of blocks takes a tile: every block shrinks a slice of K
+// (S = A x^T, ranks as the rows of the product and tokens as its columns), the slices meet through distributed shared
+// memory, and every block expands them to a slice of N (B S).  So a tile costs one launch, no workspace and no atomics;
+// the sums' order depends on the sizes alone.
+//
+// Both products are bf16 mma.sync with fp32 accumulators, fed straight from global memory: the order of a contraction's
+// terms is free, so a lane takes 8 consecutive values of a row, 16 bytes, as the terms that the instruction's fragment
+// layout gives it (4 lanes x 16 bytes are two whole sectors of a row), and no shared memory or shuffles lie between.
+// The operator is bound by memory at every rank it takes (2 m r (k + n) operations against m (2 k + 8 n) bytes: 32
+// operations a byte at rank 64), which mma.sync covers; tensor memory would add its round trip to calls of 4 us.
+//
+// fp32 operands (x, and S between the products) are split into three bf16 parts that add up to all 24 bits, and each
+// part is multiplied: nothing is rounded to 16 bits but the weights that are stored so.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include "ws_norm_kernel.cuh"
+
+namespace ws {
+
+constexpr int kLoraThreads = 256;
+constexpr int kLoraWarps = kLoraThreads / 32;
+constexpr int kLoraMaxRank = 128;
+constexpr int kLoraMaxCluster = 8;
+constexpr int kLoraDirect = kLoraThreads;    // up to this many tokens a block finds its tile by itself
+constexpr int kLoraMaxAdapters = 16384;      // of a sorted batch: two words of shared memory each
+
+struct LoraTile {
+    int32_t adapter, start, count, pad;      // adapter -1: tokens without one
+};
+struct LoraParams {
+    const void *x, *y;
+    void *out;
+    const uint16_t *a, *b;
+    const int32_t *ids;
+    const float *scale;        // or null: 1
+    const float *s_in;         // [m, r] shrunk rows to expand, or null: shrink x
+    float *s_out;              // [m, r] where shrunk rows go instead of being expanded, or null
+    int64_t ldx, ldy, ldo;
+    int32_t m, k, n, r, adapters;
+    int32_t y_dtype, cluster;
+    // sorted batches
+    int32_t *tiles_count, *perm;
+    LoraTile *tiles;
+    int32_t tile, skip_none;
+};
+
+__device__ __forceinline__ int lora_id(const LoraParams &p, int t) {
+    const int id = p.ids[t];
+    return id >= 0 && id < p.adapters ? id : -1;
+}
+
+// More tokens than a block looks through: they are grouped by adapter first.  The order of tokens within a group is the
+// atomics'; a token's result does not depend on its place in a tile.
+__global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__ LoraParams p) {
+    extern __shared__ int32_t lora_hist[];
+    int32_t *count = lora_hist, *first = lora_hist + p.adapters + 1;  // tokens of a bucket; its first place
+    int32_t *tile0 = first + p.adapters + 1;                          // its first tile
+    __shared__ int32_t warp_sum[32][2];
+    const int tid = threadIdx.x, lane = tid & 31, buckets = p.adapters + 1;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int i = tid; i < buckets; i += 1024) count[i] = 0;
+    wait_predecessor();
+    __syncthreads();
+    for (int t = tid; t < p.m; t += 1024) {
+        const int id = lora_id(p, t);
+        atomicAdd(&count[id < 0 ? p.adapters : id], 1);
+    }
+    __syncthreads();
+    const int per = (buckets + 1023) / 1024, b0 = tid * per, b1 = min(buckets, b0 + per);
+    int32_t tok = 0, til = 0;
+    for (int b = b0; b < b1; ++b) {
+        tok += count[b];
+        if (b < p.adapters || !p.skip_none) til += (count[b] + p.tile - 1) / p.tile;
+    }
+    int32_t st = tok, sl = til;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int32_t u = __shfl_up_sync(0xffffffffu, st, o), v = __shfl_up_sync(0xffffffffu, sl, o);
+        if (lane >= o) {
+            st += u;
+            sl += v;
+        }
+    }
+    if (lane == 31) {
+        warp_sum[tid >> 5][0] = st;
+        warp_sum[tid >> 5][1] = sl;
+    }
+    __syncthreads();
+    int32_t before_tok = st - tok, before_til = sl - til;
+    for (int w = 0; w < (tid >> 5); ++w) {
+        before_tok += warp_sum[w][0];
+        before_til += warp_sum[w][1];
+    }
+    if (tid == 1023) *p.tiles_count = before_til + til;
+    for (int b = b0; b < b1; ++b) {
+        const int c = count[b];
+        first[b] = before_tok;
+        tile0[b] = before_til;
+        before_tok += c;
+        if (b < p.adapters || !p.skip_none) before_til += (c + p.tile - 1) / p.tile;
+    }
+    __syncthreads();
+    for (int t = tid; t < p.m; t += 1024) {
+        const int id = lora_id(p, t), b = id < 0 ? p.adapters : id;
+        if (b == p.adapters && p.skip_none) continue;
+        const int left = atomicSub(&count[b], 1);                      // c, c - 1, .. 1
+        const int c = (b + 1 < buckets ? first[b + 1] : p.m) - first[b], at = c - left;
+        p.perm[first[b] + at] = t;
+        if (at % p.tile == 0) p.tiles[tile0[b] + at / p.tile] = LoraTile{id, first[b] + at, min(p.tile, c - at), 0};
+    }
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The leading eight bits of two floats as bf16 (a in the low half); the floats keep the rest.  Cut off, not rounded, so that
+// no finite value becomes infinite; an infinite one leaves nothing.
+__device__ __forceinline__ float after_bf16(float v) { return fabsf(v) == __uint_as_float(0x7F800000u) ? 0.0f : v - __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t cut_bf16x2(float &a, float &b) {
+    const uint32_t r = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    a = after_bf16(a);
+    b = after_bf16(b);
+    return r;
+}
+
+// Eight consecutive values of a bf16 row from `i`, those from `limit` on as zeros.  VEC: `limit` is a multiple of 8 and
+// the row 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ uint4 row8(const uint16_t *row, int i, int limit) {
+    if (VEC) return i < limit ? __ldg(reinterpret_cast<const uint4 *>(row + i)) : make_uint4(0, 0, 0, 0);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        w[j] = (i + 2 * j < limit ? (uint32_t)__ldg(row + i + 2 * j) : 0u) | (i + 2 * j + 1 < limit ? (uint32_t)__ldg(row + i + 2 * j + 1) << 16 : 0u);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void row8(const float *row, int i, int limit, float (&v)[8]) {
+    if (VEC) {
+        float4 a = make_float4(0, 0, 0, 0), b = a;
+        if (i < limit) {
+            a = __ldg(reinterpret_cast<const float4 *>(row + i));
+            b = __ldg(reinterpret_cast<const float4 *>(row + i) + 1);
+        }
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = i + j < limit ? __ldg(row + i + j) : 0.0f;
+    }
+}
+
+// Four consecutive outputs of a token.
+template <bool VEC>
+__device__ __forceinline__ void add4(const LoraParams &p, int64_t tok, int nn, float (&d)[4]) {
+    if (nn >= p.n) return;
+    if (VEC && p.y_dtype == WS_ACT_F32) {
+        const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.y) + tok * p.ldy + nn);
+        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + tok * p.ldo + nn) = make_float4(y.x + d[0], y.y + d[1], y.z + d[2], y.w + d[3]);
+    } else if (VEC) {
+        const uint2 y = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.y) + tok * p.ldy + nn);
+        const uint32_t lo = pack_bf16x2(__uint_as_float(y.x << 16) + d[0], __uint_as_float(y.x & 0xFFFF0000u) + d[1]);
+        const uint32_t hi = pack_bf16x2(__uint_as_float(y.y << 16) + d[2], __uint_as_float(y.y & 0xFFFF0000u) + d[3]);
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + tok * p.ldo + nn) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (nn + j < p.n) store1(p.out, p.y_dtype, tok * p.ldo + nn + j, load1(p.y, p.y_dtype, tok * p.ldy + nn + j) + d[j]);
+    }
+}
+
+template <int RT, int NT>
+struct LoraShape {
+    static constexpr int kTokens = NT * 8, kRanks = RT * 16;
+    static constexpr int kSums = RT * NT * 128;                              // values of S
+    // a token's ranks in bf16, padded so that a warp's fragment loads meet no bank twice
+    static constexpr int kRow = kRanks * 2 + (RT >= 4 ? 64 : 0);
+    static constexpr int kSplit = 3 * kTokens * kRow;
+    static constexpr int kScratch = kLoraWarps * kSums * 4 > kSplit ? kLoraWarps * kSums * 4 : kSplit;
+    static constexpr int kSmem = kScratch + kSums * 4;
+    static constexpr int kAhead = RT * NT <= 2 ? 4 : RT * NT <= 8 ? 2 : 1;   // steps of K requested together
+};
+
+template <int RT, int NT, bool XF32, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constant__ LoraParams p) {
+    namespace cg = cooperative_groups;
+    using S = LoraShape<RT, NT>;
+    extern __shared__ __align__(16) uint8_t lora_smem[];
+    float *const warps = reinterpret_cast<float *>(lora_smem);                      // [warp][kSums], then the split S
+    float *const sums = reinterpret_cast<float *>(lora_smem + S::kScratch);         // this block's S, read by the cluster
+    __shared__ int32_t toks[S::kTokens], found[kLoraWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int C = p.cluster, part = blockIdx.x % C, tile = blockIdx.x / C;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_predecessor();
+
+    // ---- the tile's tokens
+    int adapter;
+    if (p.tiles) {
+        if (tile >= *p.tiles_count) return;
+        const LoraTile q = p.tiles[tile];
+        adapter = q.adapter;
+        if (tid < S::kTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
+    } else {
+        // token `tile` leads a tile if the number of earlier tokens with its adapter is a multiple of the tile's size
+        adapter = lora_id(p, tile);
+        const bool same = tid < p.m && lora_id(p, tid) == adapter;
+        const uint32_t in_warp = __ballot_sync(0xffffffffu, same);
+        if (lane == 0) found[warp] = (int32_t)in_warp;
+        if (tid < S::kTokens) toks[tid] = -1;
+        __syncthreads();
+        int lead = 0, mine = __popc(in_warp & ((1u << lane) - 1));
+        for (int w = 0; w < kLoraWarps; ++w) {
+            const uint32_t f = (uint32_t)found[w];
+            lead += w < (tile >> 5) ? __popc(f) : w == (tile >> 5) ? __popc(f & ((1u << (tile & 31)) - 1)) : 0;
+            mine += w < warp ? __popc(f) : 0;
+        }
+        if (lead % S::kTokens != 0) return;  // (the same on all threads of the cluster)
+        if (same && mine >= lead && mine < lead + S::kTokens) toks[mine - lead] = tid;
+    }
+    __syncthreads();
+    if (adapter < 0) {  // nothing to add
+        for (int i = 0; i < S::kTokens; ++i) {
+            const int64_t tok = toks[i];
+            if (tok < 0) break;
+            const int n0 = (int)((int64_t)(p.s_out ? p.r : p.n) * part / C), n1 = (int)((int64_t)(p.s_out ? p.r : p.n) * (part + 1) / C);
+            for (int j = n0 + tid; j < n1; j += kLoraThreads) {
+                if (p.s_out) p.s_out[tok * p.r + j] = 0.0f;
+                else if (p.out != p.y) store1(p.out, p.y_dtype, tok * p.ldo + j, load1(p.y, p.y_dtype, tok * p.ldy + j));
+            }
+        }
+        return;
+    }
+
+    // ---- S = A x^T over this block's K, a step of 32 a warp
+    if (!p.s_in) {
+        float acc[RT][NT][4] = {};
+        const uint16_t *arow[RT][2];
+        bool aok[RT][2];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = i * 16 + h * 8 + g;
+                aok[i][h] = row < p.r;
+                arow[i][h] = p.a + ((int64_t)adapter * p.r + min(row, p.r - 1)) * p.k;
+            }
+        const char *xrow[NT];
+        bool xok[NT];
+#pragma unroll
+        for (int q = 0; q < NT; ++q) {
+            const int tok = toks[q * 8 + g];
+            xok[q] = tok >= 0;
+            xrow[q] = static_cast<const char *>(p.x) + (int64_t)max(tok, 0) * p.ldx * (XF32 ? 4 : 2);
+        }
+        const int steps = (p.k + 31) / 32, s0 = (int)((int64_t)steps * part / C), s1 = (int)((int64_t)steps * (part + 1) / C);
+        constexpr int U = S::kAhead;
+        for (int st = s0 + warp; st < s1; st += kLoraWarps * U) {
+            uint4 aw[U][RT][2], xw[U][NT];
+            float xf[XF32 ? U : 1][NT][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k0 = (st + u * kLoraWarps) * 32 + t4 * 8, limit = st + u * kLoraWarps < s1 ? p.k : 0;
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) aw[u][i][h] = row8<VEC>(arow[i][h], k0, aok[i][h] ? limit : 0);
+#pragma unroll
+                for (int q = 0; q < NT; ++q) {
+                    if (XF32) row8<VEC>(reinterpret_cast<const float *>(xrow[q]), k0, xok[q] ? limit : 0, xf[u % (XF32 ? U : 1)][q]);
+                    else xw[u][q] = row8<VEC>(reinterpret_cast<const uint16_t *>(xrow[q]), k0, xok[q] ? limit : 0);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int part3 = 0; part3 < (XF32 ? 3 : 1); ++part3)
+#pragma unroll
+                    for (int q = 0; q < NT; ++q) {
+                        uint4 xv;
+                        if (XF32) {
+                            float(&f)[8] = xf[u % (XF32 ? U : 1)][q];
+                            xv = make_uint4(cut_bf16x2(f[0], f[1]), cut_bf16x2(f[2], f[3]), cut_bf16x2(f[4], f[5]), cut_bf16x2(f[6], f[7]));
+                        } else {
+                            xv = xw[u][q];
+                        }
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            const uint4 &lo = aw[u][i][0], &hi = aw[u][i][1];
+                            mma_bf16(acc[i][q], lo.x, hi.x, lo.y, hi.y, xv.x, xv.y);
+                            mma_bf16(acc[i][q], lo.z, hi.z, lo.w, hi.w, xv.z, xv.w);
+                        }
+                    }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) warps[warp * S::kSums + ((i * NT + q) * 4 + e) * 32 + lane] = acc[i][q][e];
+        __syncthreads();
+        for (int j = tid; j < S::kSums; j += kLoraThreads) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kLoraWarps; ++w) s += warps[w * S::kSums + j];
+            sums[j] = s;
+        }
+    }
+    cg::cluster_group cl = cg::this_cluster();
+    if (C > 1 && !p.s_in) cl.sync();
+    else __syncthreads();
+
+    // ---- the whole S: the cluster's slices in order, in three bf16 parts of scale * S
+    uint8_t *const split = lora_smem;
+    const float scale = p.scale && !p.s_out ? p.scale[adapter] : 1.0f;
+    const int j0 = p.s_out ? S::kSums * part / C : 0, j1 = p.s_out ? S::kSums * (part + 1) / C : S::kSums;
+    for (int j = j0 + tid; j < j1; j += kLoraThreads) {
+        const int l = j & 31, e = (j >> 5) & 3, iq = j >> 7, i = iq / NT, q = iq % NT;
+        const int rank = i * 16 + (l >> 2) + (e >> 1) * 8, place = q * 8 + (l & 3) * 2 + (e & 1), tok = toks[place];
+        float s = 0.0f;
+        if (p.s_in) {
+            if (tok >= 0 && rank < p.r) s = p.s_in[(int64_t)tok * p.r + rank];
+        } else if (C > 1) {
+            for (int c = 0; c < C; ++c) s += cl.map_shared_rank(sums, c)[j];
+        } else {
+            s = sums[j];
+        }
+        if (p.s_out) {
+            if (tok >= 0 && rank < p.r) p.s_out[(int64_t)tok * p.r + rank] = s;
+            continue;
+        }
+        s *= scale;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+            *reinterpret_cast<uint16_t *>(split + (w * S::kTokens + place) * S::kRow + rank * 2) = (uint16_t)(__float_as_uint(s) >> 16);
+            s = after_bf16(s);
+        }
+    }
+    if (C > 1 && !p.s_in) cl.barrier_arrive();  // its slices are read; waited for at the end
+    __syncthreads();
+
+    // ---- out = y + B S over this block's N, 64 rows of B a warp: row h * 32 + g * 4 + j of them is row h * 8 + g of
+    // product j, so that a lane ends with four consecutive outputs
+    if (!p.s_out) {
+        constexpr int KP = RT >= 2 ? RT / 2 : 1;   // steps of 32 ranks (of 16 for RT = 1)
+        const int blocks = (p.n + 63) / 64, n0 = (int)((int64_t)blocks * part / C), n1 = (int)((int64_t)blocks * (part + 1) / C);
+        for (int nb = n0 + warp; nb < n1; nb += kLoraWarps) {
+            uint4 bw[4][2][KP];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = nb * 64 + h * 32 + g * 4 + j;
+                    const uint16_t *b = p.b + ((int64_t)adapter * p.n + min(row, p.n - 1)) * p.r;
+                    const int limit = row < p.n ? p.r : 0;
+                    if (RT >= 2) {
+#pragma unroll
+                        for (int q = 0; q < KP; ++q) bw[j][h][q] = row8<VEC>(b, q * 32 + t4 * 8, limit);
+                    } else if (VEC) {
+                        const uint2 v = t4 * 4 < limit ? __ldg(reinterpret_cast<const uint2 *>(b + t4 * 4)) : make_uint2(0, 0);
+                        bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
+                    } else {
+                        bw[j][h][0] = row8<false>(b, t4 * 4, min(limit, t4 * 4 + 4));
+                    }
+                }
+#pragma unroll
+            for (int q = 0; q < NT; ++q) {
+                float acc[4][4] = {};
+#pragma unroll
+                for (int w = 0; w < 3; ++w) {
+                    const uint8_t *srow = split + (w * S::kTokens + q * 8 + g) * S::kRow;
+#pragma unroll
+                    for (int kp = 0; kp < KP; ++kp) {
+                        if (RT >= 2) {
+                            const uint4 s = *reinterpret_cast<const uint4 *>(srow + kp * 64 + t4 * 16);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                mma_bf16(acc[j], bw[j][0][kp].x, bw[j][1][kp].x, bw[j][0][kp].y, bw[j][1][kp].y, s.x, s.y);
+                                mma_bf16(acc[j], bw[j][0][kp].z, bw[j][1][kp].z, bw[j][0][kp].w, bw[j][1][kp].w, s.z, s.w);
+                            }
+                        } else {
+                            const uint2 s = *reinterpret_cast<const uint2 *>(srow + t4 * 8);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][0].x, bw[j][1][0].x, bw[j][0][0].y, bw[j][1][0].y, s.x, s.y);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int tok = toks[q * 8 + t4 * 2 + (e & 1)];
+                    float d[4] = {acc[0][e], acc[1][e], acc[2][e], acc[3][e]};
+                    if (tok >= 0) add4<VEC>(p, tok, nb * 64 + (e >> 1) * 32 + g * 4, d);
+                }
+            }
+        }
+    }
+    if (C > 1 && !p.s_in) cl.barrier_wait();
+}
+
+}  // namespace ws

@@ -31,6 +31,11 @@ __device__ __forceinline__ uint32_t bf16_bits(float v) {  // to nearest even
     asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(b) : "f"(v));
     return b;
 }
+__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {  // to nearest even, a in the low half
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
 __device__ __forceinline__ void store1(void *p, int dtype, int64_t i, float v) {
     if (dtype == WS_ACT_F32) static_cast<float *>(p)[i] = v;
     else static_cast<uint16_t *>(p)[i] = (uint16_t)bf16_bits(v);

@@ -4,6 +4,7 @@
 #include <cstdarg>
 #include <cstdio>
 
+#include "ws_lora_kernel.cuh"
 #include "ws_norm_kernel.cuh"
 #include "ws_scores_kernel.cuh"
 
@@ -52,9 +53,109 @@ ws_status_t launch(const Err &err, void (*kernel)(P), dim3 grid, unsigned thread
     return e == cudaSuccess ? WS_OK : err(WS_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
 }
 
+// ---- adapters
+int64_t lora_max_tiles(int m, int adapters, int tile) { return ((int64_t)m + tile - 1) / tile + std::min((int64_t)adapters + 1, (int64_t)m); }
+int64_t lora_perm_bytes(int m) { return 16 + ((int64_t)m * 4 + 15) / 16 * 16; }
+
+template <int RT, int NT, bool XF32, bool VEC>
+ws_status_t launch_lora(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
+    using S = LoraShape<RT, NT>;
+    auto *k = lora_kernel<RT, NT, XF32, VEC>;
+    if (S::kSmem > 47 * 1024) {  // (48 KB with the static part)
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        if (e != cudaSuccess) return err(WS_ERR_CUDA, "shared memory of %d bytes: %s", S::kSmem, cudaGetErrorString(e));
+    }
+    return launch(err, k, dim3(tiles * (unsigned)p.cluster), kLoraThreads, S::kSmem, (unsigned)p.cluster, stream, p);
+}
+template <int RT, int NT>
+ws_status_t launch_lora(const Err &err, bool xf32, bool vec, unsigned tiles, void *stream, const LoraParams &p) {
+    if (!vec) return xf32 ? launch_lora<RT, NT, true, false>(err, tiles, stream, p) : launch_lora<RT, NT, false, false>(err, tiles, stream, p);
+    return xf32 ? launch_lora<RT, NT, true, true>(err, tiles, stream, p) : launch_lora<RT, NT, false, true>(err, tiles, stream, p);
+}
+template <int RT>
+ws_status_t launch_lora(const Err &err, int nt, bool xf32, bool vec, unsigned tiles, void *stream, const LoraParams &p) {
+    if (nt == 1) return launch_lora<RT, 1>(err, xf32, vec, tiles, stream, p);
+    if (nt == 2) return launch_lora<RT, 2>(err, xf32, vec, tiles, stream, p);
+    return launch_lora<RT, (RT < 8 ? 8 : 4)>(err, xf32, vec, tiles, stream, p);
+}
+
+enum class Lora { kAdd, kShrink, kExpand };
+
+ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_text, size_t err_len) {
+    const Err err{err_text, err_len};
+    if (err_text && err_len) err_text[0] = 0;
+    if (!a) return err(WS_ERR_INVALID, "null args");
+    const bool shrinks = what != Lora::kExpand, expands = what != Lora::kShrink;
+    // (the kernels count a row's values in 32 bits, up to a step past its end, and blocks in 31)
+    if (a->m < 0 || a->m > (1 << 26) || a->adapters < 1 || (shrinks && (a->k < 1 || a->k > INT32_MAX - 4096)) ||
+        (expands && (a->n < 1 || a->n > INT32_MAX - 4096)))
+        return err(WS_ERR_INVALID, "m=%d k=%d n=%d adapters=%d out of range", a->m, a->k, a->n, a->adapters);
+    if (a->rank < 1 || a->rank > WS_LORA_MAX_RANK) return err(WS_ERR_INVALID, "rank=%d is not in 1..%d", a->rank, WS_LORA_MAX_RANK);
+    if ((shrinks && !is_type(a->x_dtype)) || (expands && !is_type(a->y_dtype))) return err(WS_ERR_INVALID, "unknown type of a tensor");
+    if (a->m == 0) return WS_OK;
+    if (!a->ids || (shrinks && (!a->x || !a->a)) || (expands && (!a->y || !a->out || !a->b)) || (what != Lora::kAdd && !a->shrunk))
+        return err(WS_ERR_INVALID, "a tensor is missing");
+    if ((shrinks && a->ldx < a->k) || (expands && (a->ldy < a->n || a->ldo < a->n))) return err(WS_ERR_INVALID, "a row stride is shorter than its row");
+    if ((shrinks && (!natural(a->x, a->x_dtype) || !natural(a->a, WS_ACT_BF16))) ||
+        (expands && (!natural(a->y, a->y_dtype) || !natural(a->out, a->y_dtype) || !natural(a->b, WS_ACT_BF16))) ||
+        !natural(a->ids, WS_ACT_F32) || !natural(a->scale, WS_ACT_F32) || !natural(a->shrunk, WS_ACT_F32))
+        return err(WS_ERR_INVALID, "a tensor is not aligned to its type");
+    LoraParams p{};
+    if (shrinks) { p.x = a->x; p.a = static_cast<const uint16_t *>(a->a); p.ldx = a->ldx; p.k = a->k; }
+    if (expands) { p.y = a->y; p.out = a->out; p.b = static_cast<const uint16_t *>(a->b); p.ldy = a->ldy; p.ldo = a->ldo; p.n = a->n; p.scale = a->scale; p.y_dtype = a->y_dtype; }
+    if (what == Lora::kShrink) p.s_out = a->shrunk;
+    if (what == Lora::kExpand) p.s_in = a->shrunk;
+    p.ids = a->ids; p.m = a->m; p.r = a->rank; p.adapters = a->adapters;
+    p.skip_none = expands && a->y == a->out && a->ldy == a->ldo;
+    const bool xf32 = shrinks && a->x_dtype == WS_ACT_F32;
+    bool vec = a->rank % 8 == 0;
+    if (shrinks) vec = vec && a->k % 8 == 0 && aligned(a->x, a->ldx, a->x_dtype, 16) && aligned(a->a, a->k, WS_ACT_BF16, 16);
+    if (expands) {
+        const int64_t four = 4 * type_bytes(a->y_dtype);
+        vec = vec && a->n % 4 == 0 && aligned(a->y, a->ldy, a->y_dtype, four) && aligned(a->out, a->ldo, a->y_dtype, four) &&
+              aligned(a->b, a->rank, WS_ACT_BF16, 16);
+    }
+    const int rt = a->rank <= 16 ? 1 : a->rank <= 32 ? 2 : a->rank <= 64 ? 4 : 8;
+    const int nt = a->m <= 32 ? 1 : a->m <= kLoraDirect ? 2 : rt < 8 ? 8 : 4;
+    p.cluster = a->m <= 64 ? 8 : 4;
+    unsigned tiles = (unsigned)a->m;
+    if (a->m > kLoraDirect) {
+        if (a->adapters > kLoraMaxAdapters) return err(WS_ERR_CAPACITY, "%d adapters: at most %d with more than %d tokens", a->adapters, kLoraMaxAdapters, kLoraDirect);
+        if (!a->workspace || a->workspace_bytes < ws_lora_workspace(a->m, a->adapters) || reinterpret_cast<uintptr_t>(a->workspace) & 15)
+            return err(WS_ERR_INVALID, "%d tokens need a 16-byte aligned workspace of %lld bytes", a->m, (long long)ws_lora_workspace(a->m, a->adapters));
+        p.tile = nt * 8;
+        p.tiles_count = static_cast<int32_t *>(a->workspace);
+        p.perm = p.tiles_count + 4;
+        p.tiles = reinterpret_cast<LoraTile *>(static_cast<char *>(a->workspace) + lora_perm_bytes(a->m));
+        tiles = (unsigned)lora_max_tiles(a->m, a->adapters, p.tile);
+        const size_t smem = (size_t)(a->adapters + 1) * 12;
+        if (smem > 47 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kLoraMaxAdapters + 1) * 12);
+            if (e != cudaSuccess) return err(WS_ERR_CUDA, "shared memory: %s", cudaGetErrorString(e));
+        }
+        const ws_status_t st = launch(err, lora_plan_kernel, dim3(1), 1024, smem, 1, stream, p);
+        if (st != WS_OK) return st;
+    }
+    switch (rt) {
+        case 1: return launch_lora<1>(err, nt, xf32, vec, tiles, stream, p);
+        case 2: return launch_lora<2>(err, nt, xf32, vec, tiles, stream, p);
+        case 4: return launch_lora<4>(err, nt, xf32, vec, tiles, stream, p);
+        default: return launch_lora<8>(err, nt, xf32, vec, tiles, stream, p);
+    }
+}
+
 }  // namespace
 
 extern "C" {
+
+int64_t ws_lora_workspace(int32_t m, int32_t adapters) {
+    if (m <= kLoraDirect || adapters < 1) return 0;
+    return lora_perm_bytes(m) + lora_max_tiles(m, adapters, 32) * (int64_t)sizeof(LoraTile);
+}
+ws_status_t ws_lora_add(const ws_lora_args_t *a, void *stream, char *err, size_t err_len) { return lora(Lora::kAdd, a, stream, err, err_len); }
+ws_status_t ws_lora_shrink(const ws_lora_args_t *a, void *stream, char *err, size_t err_len) { return lora(Lora::kShrink, a, stream, err, err_len); }
+ws_status_t ws_lora_expand(const ws_lora_args_t *a, void *stream, char *err, size_t err_len) { return lora(Lora::kExpand, a, stream, err, err_len); }
+
 
 ws_status_t ws_block_norm(const ws_block_norm_args_t *a, void *stream, char *err_text, size_t err_len) {
     const Err err{err_text, err_len};

@@ -415,8 +415,82 @@ PyObject *py_token_logprobs(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// lora(what, y, x, a, b, ids, scale, shrunk, out, stream) -> out | shrunk; what: 0 add (y x a b), 1 shrink (x a), 2 expand (y b shrunk)
+PyObject *py_lora(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 10) { PyErr_SetString(PyExc_TypeError, "lora takes 10 arguments"); return nullptr; }
+    const long what = PyLong_AsLong(v[0]);
+    if (PyErr_Occurred()) return nullptr;
+    const bool shrinks = what != 2, expands = what != 1;
+    const at::Tensor *ids = tensor(v[5]);
+    if (!ids || ids->dim() != 1 || !ids->is_contiguous() || ids->scalar_type() != at::kInt) Py_RETURN_NONE;
+    const int64_t m = ids->size(0);
+    int64_t adapters = 0, rank = 0, k = 0, n = 0;
+    ws_lora_args_t a{};
+    a.ids = ids->data_ptr<int32_t>();
+    if (shrinks) {
+        const at::Tensor *x = tensor(v[2]), *w = tensor(v[3]);
+        if (!x || !w || w->dim() != 3 || !w->is_contiguous() || w->scalar_type() != at::kBFloat16 || w->device() != ids->device()) Py_RETURN_NONE;
+        adapters = w->size(0); rank = w->size(1); k = w->size(2);
+        if (!rows(x, *ids, m, k, &a.ldx) || !act_dtype(*x, &a.x_dtype)) Py_RETURN_NONE;
+        a.x = x->data_ptr(); a.a = w->data_ptr();
+    }
+    const at::Tensor *y = nullptr;
+    if (expands) {
+        const at::Tensor *w = tensor(v[4]);
+        y = tensor(v[1]);
+        if (!y || !w || w->dim() != 3 || !w->is_contiguous() || w->scalar_type() != at::kBFloat16 || w->device() != ids->device()) Py_RETURN_NONE;
+        if (shrinks && (w->size(0) != adapters || w->size(2) != rank)) Py_RETURN_NONE;
+        adapters = w->size(0); n = w->size(1); rank = w->size(2);
+        if (!rows(y, *ids, m, n, &a.ldy) || !act_dtype(*y, &a.y_dtype)) Py_RETURN_NONE;
+        a.y = y->data_ptr(); a.b = w->data_ptr();
+        if (v[6] != Py_None) {
+            const at::Tensor *s = tensor(v[6]);
+            if (!vec(s, *ids, adapters) || s->scalar_type() != at::kFloat) Py_RETURN_NONE;
+            a.scale = s->data_ptr<float>();
+        }
+    }
+    if (m > INT32_MAX || adapters > INT32_MAX || rank > INT32_MAX || k > INT32_MAX || n > INT32_MAX) Py_RETURN_NONE;
+    a.m = (int32_t)m; a.adapters = (int32_t)adapters; a.rank = (int32_t)rank; a.k = (int32_t)k; a.n = (int32_t)n;
+    if (what == 2) {
+        const at::Tensor *s = tensor(v[7]);
+        if (!s || s->dim() != 2 || s->size(0) != m || s->size(1) != rank || !s->is_contiguous() || s->scalar_type() != at::kFloat ||
+            s->device() != ids->device())
+            Py_RETURN_NONE;
+        a.shrunk = s->data_ptr<float>();
+    }
+    CallOn on(*ids, v[9]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor made;
+    if (expands && v[8] != Py_None) {
+        const at::Tensor *out = tensor(v[8]);
+        if (!rows(out, *ids, m, n, &a.ldo) || out->scalar_type() != y->scalar_type()) Py_RETURN_NONE;
+        a.out = out->data_ptr();
+    } else if (expands) {
+        made = new_like(*y, {m, n}, y->scalar_type());
+        a.out = made.data_ptr();
+        a.ldo = n;
+    } else {
+        made = new_like(*ids, {m, rank}, at::kFloat);
+        a.shrunk = made.data_ptr<float>();
+    }
+    at::Tensor work;
+    a.workspace_bytes = ws_lora_workspace(a.m, a.adapters);
+    if (a.workspace_bytes > 0) {
+        work = new_like(*ids, {a.workspace_bytes}, at::kByte);
+        a.workspace = work.data_ptr();
+    }
+    WS_CALL(st, what == 0 ? ws_lora_add(&a, on.stream, nullptr, 0) : what == 1 ? ws_lora_shrink(&a, on.stream, nullptr, 0)
+                                                                                : ws_lora_expand(&a, on.stream, nullptr, 0))
+    if (st != WS_OK) Py_RETURN_NONE;
+    if (made.defined()) return THPVariable_Wrap(std::move(made));
+    Py_INCREF(v[8]);
+    return v[8];
+    END_HANDLE_TH_ERRORS
+}
+
 #define WS_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {WS_METHOD(fp8), WS_METHOD(fp8_host), WS_METHOD(moe), WS_METHOD(head), WS_METHOD(fp8_group), WS_METHOD(block_norm), WS_METHOD(token_logprobs),
+PyMethodDef methods[] = {WS_METHOD(fp8), WS_METHOD(fp8_host), WS_METHOD(moe), WS_METHOD(head), WS_METHOD(fp8_group), WS_METHOD(block_norm), WS_METHOD(lora), WS_METHOD(token_logprobs),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_ws_torch", "torch tensors -> libws_tp.so", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

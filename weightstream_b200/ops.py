@@ -2,7 +2,8 @@
 
 A decode engine does more between two reduction points than the steps of :mod:`weightstream_b200.tp`: it normalises a
 block's output, gates it, adds it to the residual stream and normalises that for the next block (:func:`block_norm`),
-and it scores given tokens on the vocabulary head's logits (:func:`token_logprobs`).
+it adds the requests' low-rank adapters to a projection's result (:func:`lora_add`), and it scores given tokens on the
+vocabulary head's logits (:func:`token_logprobs`).
 
 Every function runs on the GPU that holds its tensors, on ``stream`` or the current stream, and does not synchronise.
 Results are allocated on that stream.  A tensor that a call reads has to live until the stream has passed the call, as
@@ -17,7 +18,8 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import BlockNormArgs, TokenLogprobsArgs, WsError, WS_ACT_BF16, WS_ACT_F32, WS_GATE_LINEAR, WS_GATE_SIGMOID, WS_MAX_TOP, WS_OK
+from ._lib import BlockNormArgs, LoraArgs, TokenLogprobsArgs, WsError, WS_ACT_BF16, WS_ACT_F32, WS_GATE_LINEAR, WS_GATE_SIGMOID, \
+    WS_LORA_MAX_RANK, WS_MAX_TOP, WS_OK
 
 _TYPES = {torch.bfloat16: WS_ACT_BF16, torch.float32: WS_ACT_F32}
 _GATES = {"none": WS_GATE_LINEAR, "sigmoid": WS_GATE_SIGMOID}
@@ -164,6 +166,110 @@ def block_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post
             a.normed, a.ldn = normed.data_ptr(), a.n
         _call("ws_block_norm", a)
     return hidden, normed
+
+
+# ----------------------------------------------------------------------------- adapters of many requests
+def _lora_args(ids, *, x=None, a=None, y=None, b=None, scale=None, shrunk=None, out=None) -> LoraArgs:
+    """Arguments of the whole (x, a, y, b), of the shrinking half (x, a) or of the expanding one (shrunk, y, b)."""
+    if ids.dtype != torch.int32:
+        raise TypeError(f"ids must be int32, got {ids.dtype}")
+    m = ids.shape[0] if ids.dim() == 1 else -1
+    _vector(ids, "ids", m)
+    r = LoraArgs()
+    r.m, r.ids = m, ids.data_ptr()
+    for t, name in ((a, "a"), (b, "b")):
+        if t is None:
+            continue
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be bf16, got {t.dtype}")
+        if t.dim() != 3 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous and 3-D, got {list(t.shape)}")
+    if a is not None:
+        r.adapters, r.rank, r.k = a.shape
+        r.a, r.x, r.ldx, r.x_dtype = a.data_ptr(), x.data_ptr(), _rows(x, "x", m, a.shape[2]), _code(x, "x")
+    if b is not None:
+        if a is not None and (b.shape[0], b.shape[2]) != (a.shape[0], a.shape[1]):
+            raise ValueError(f"a {list(a.shape)} and b {list(b.shape)} must be [adapters, rank, k] and [adapters, n, rank]")
+        r.adapters, r.n, r.rank = b.shape
+        r.b, r.y, r.ldy, r.y_dtype = b.data_ptr(), y.data_ptr(), _rows(y, "y", m, b.shape[1]), _code(y, "y")
+        if out is not None:
+            if out.dtype != y.dtype:
+                raise TypeError(f"out must be {y.dtype} as y, got {out.dtype}")
+            r.out, r.ldo = out.data_ptr(), _rows(out, "out", m, b.shape[1])
+        if scale is not None:
+            _vector(scale, "scale", r.adapters, torch.float32)
+            r.scale = scale.data_ptr()
+    _dim(m, *(a.shape if a is not None else ()), *(b.shape if b is not None else ()))
+    if r.adapters < 1 or not 1 <= r.rank <= WS_LORA_MAX_RANK:
+        raise ValueError(f"{r.adapters} adapters of rank {r.rank}: at least one, of rank 1..{WS_LORA_MAX_RANK}")
+    if (a is not None and r.k < 1) or (b is not None and r.n < 1):
+        raise ValueError("k and n must be at least 1")
+    if shrunk is not None:
+        if shrunk.dtype != torch.float32:
+            raise TypeError(f"shrunk must be fp32, got {shrunk.dtype}")
+        if list(shrunk.shape) != [m, r.rank] or not shrunk.is_contiguous():
+            raise ValueError(f"shrunk must be contiguous [{m}, {r.rank}], got {list(shrunk.shape)}")
+        r.shrunk = shrunk.data_ptr()
+    _same_device(ids, x, a, y, b, scale, shrunk, out)
+    return r
+
+
+def _lora_call(name: str, args: LoraArgs, device) -> None:
+    """On the current stream, whose memory the workspace is."""
+    size = _lib.load().ws_lora_workspace(args.m, args.adapters)
+    work = torch.empty(size, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = work.data_ptr(), size
+    _call(name, args)
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, scale: Optional[torch.Tensor] = None, *,
+             out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a shared projection: ``out[t] = y[t] + scale[i] * b[i] @ (a[i] @ x[t])``
+    with ``i = ids[t]``.
+
+    ``x`` [m, k] is what the projection read, ``y`` [m, n] what it returned (bf16 or fp32 each); ``a`` [adapters, rank, k]
+    and ``b`` [adapters, n, rank] are bf16, ``scale`` [adapters] fp32, ``ids`` [m] int32 in any order.  A token whose id is
+    outside [0, adapters), such as -1, has no adapter.  Ranks of 1 to 128; sums are fp32 and no activation is rounded on
+    the way.  Returns ``out``, of ``y``'s type, which may be ``y`` itself.
+    """
+    r = _lib.torch_front().lora(0, y, x, a, b, ids, scale, None, out, _handle(stream))
+    if r is not None:
+        return r
+    args = _lora_args(ids, x=x, a=a, y=y, b=b, scale=scale, out=out)
+    with _on(y.device, stream):
+        out = out if out is not None else torch.empty((args.m, args.n), dtype=y.dtype, device=y.device)
+        args.out, args.ldo = out.data_ptr(), args.ldo or args.n
+        _lora_call("ws_lora_add", args, y.device)
+    return out
+
+
+def lora_shrink(x: torch.Tensor, a: torch.Tensor, ids: torch.Tensor, *, stream=None) -> torch.Tensor:
+    """The first half of :func:`lora_add`, ``a[ids[t]] @ x[t]`` as fp32 [m, rank], for a projection whose K is sharded: each
+    rank shrinks its slice of ``x`` with its slice of ``a``, ``Endpoint.allreduce_`` adds the ranks' rows up, and
+    :func:`lora_expand` follows.  Rows of tokens without an adapter are zeros."""
+    r = _lib.torch_front().lora(1, None, x, a, None, ids, None, None, None, _handle(stream))
+    if r is not None:
+        return r
+    args = _lora_args(ids, x=x, a=a)
+    with _on(x.device, stream):
+        shrunk = torch.empty((args.m, args.rank), dtype=torch.float32, device=x.device)
+        args.shrunk = shrunk.data_ptr()
+        _lora_call("ws_lora_shrink", args, x.device)
+    return shrunk
+
+
+def lora_expand(y: torch.Tensor, shrunk: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, scale: Optional[torch.Tensor] = None, *,
+                out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """The second half of :func:`lora_add`: ``out[t] = y[t] + scale[i] * b[i] @ shrunk[t]`` with ``i = ids[t]``."""
+    r = _lib.torch_front().lora(2, y, None, None, b, ids, scale, shrunk, out, _handle(stream))
+    if r is not None:
+        return r
+    args = _lora_args(ids, y=y, b=b, scale=scale, shrunk=shrunk, out=out)
+    with _on(y.device, stream):
+        out = out if out is not None else torch.empty((args.m, args.n), dtype=y.dtype, device=y.device)
+        args.out, args.ldo = out.data_ptr(), args.ldo or args.n
+        _lora_call("ws_lora_expand", args, y.device)
+    return out
 
 
 # ----------------------------------------------------------------------------- scores of given tokens
