@@ -55,6 +55,123 @@ __device__ __forceinline__ float block_sum(float v, float *slot) {
     return v;
 }
 
+// Eight consecutive values of a row, of which `ok` says whether they are there.  fp32 rows are 32-byte aligned.
+__device__ __forceinline__ void unpack8(const uint4 &r, float (&v)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+template <bool F32>
+__device__ __forceinline__ void get8(const void *p, int64_t i, bool ok, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    if (!ok) return;
+    if (F32) {
+        asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "l"(static_cast<const float *>(p) + i) : "memory");
+    } else {
+        unpack8(*reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i), v);
+    }
+}
+__device__ __forceinline__ void get8(const void *p, int dtype, int64_t i, bool ok, float (&v)[8]) {
+    if (dtype == WS_ACT_F32) get8<true>(p, i, ok, v);
+    else get8<false>(p, i, ok, v);
+}
+__device__ __forceinline__ void put8(void *p, int dtype, int64_t i, const float (&v)[8]) {
+    if (dtype == WS_ACT_F32) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(static_cast<float *>(p) + i), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
+    } else {
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) =
+            make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    }
+}
+
+// A block a row, the row in registers: NV times eight values a thread.  VEC: eight consecutive ones; else (odd widths,
+// strides or addresses) a block apart, so that a warp's loads are consecutive all the same.
+template <int NV, bool VEC, bool YF32, bool RF32, bool WF32>
+__global__ void __launch_bounds__(NV == 1 ? 1024 : 512) block_norm_rows_kernel(const __grid_constant__ NormParams p) {
+    __shared__ float slots[64];
+    const int T = blockDim.x;
+    const int64_t row = blockIdx.x;
+    const int y_type = VEC ? (YF32 ? WS_ACT_F32 : WS_ACT_BF16) : p.y_dtype, r_type = VEC ? (RF32 ? WS_ACT_F32 : WS_ACT_BF16) : p.r_dtype;
+    const int w_type = VEC ? (WF32 ? WS_ACT_F32 : WS_ACT_BF16) : p.w_dtype;
+    auto at = [&](int j) { return VEC ? (j * T + (int)threadIdx.x) * 8 : j * 8 * T + (int)threadIdx.x; };
+    auto load = [&](const void *q, int dtype, int64_t row0, int j, float (&v)[8]) {
+        const int i = at(j);
+        if (VEC) get8(q, dtype, row0 + i, i < p.n, v);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = i + e * T < p.n ? load1(q, dtype, row0 + i + e * T) : 0.0f;
+    };
+    auto store = [&](void *q, int dtype, int64_t row0, int j, const float (&v)[8]) {
+        const int i = at(j);
+        if (VEC) {
+            if (i < p.n) put8(q, dtype, row0 + i, v);
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e * T < p.n) store1(q, dtype, row0 + i + e * T, v[e]);
+    };
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_predecessor();
+    const float inv_n = 1.0f / (float)p.n;
+    float h[NV][8], r[NV][8], g[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) load(p.y, y_type, row * p.ldy, j, h[j]);
+    if (p.residual)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) load(p.residual, r_type, row * p.ldr, j, r[j]);
+    const bool gates = p.gate && p.gate_inc;
+    if (gates)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) load(p.gate, p.g_dtype, row * p.ldg, j, g[j]);
+    float f = p.block_scale;
+    if (p.gate && !gates) f *= gate_value(load1(p.gate, p.g_dtype, row * p.ldg), p.gate_act);
+    if (p.post_weight) {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf(h[j][e], h[j][e], s);
+        f *= rsqrtf(fmaf(block_sum(s, slots), inv_n, p.eps));
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float w[8];
+            load(p.post_weight, w_type, 0, j, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[j][e] *= p.weight_offset + w[e];
+        }
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            h[j][e] *= f;
+            if (gates) h[j][e] *= gate_value(g[j][e], p.gate_act);
+            if (p.residual) h[j][e] = fmaf(p.residual_scale, r[j][e], h[j][e]);
+            s = fmaf(h[j][e], h[j][e], s);
+        }
+        if (p.hidden) store(p.hidden, p.h_dtype, row * p.ldh, j, h[j]);
+    }
+    if (!p.normed) return;
+    const float next = rsqrtf(fmaf(block_sum(s, slots + 32), inv_n, p.eps));
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float w[8];
+        load(p.next_weight, w_type, 0, j, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[j][e] *= next * (p.weight_offset + w[e]);
+        store(p.normed, p.n_dtype, row * p.ldn, j, h[j]);
+    }
+}
+
 // Any width, any alignment: a block a row, three passes over it (L2 serves the second and third).  The last pass reads
 // each value and writes its results on one thread, so that the stream may be updated in place.
 __global__ void __launch_bounds__(512) block_norm_any_kernel(const __grid_constant__ NormParams p) {

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 
 #include "ws_lora_kernel.cuh"
 #include "ws_norm_kernel.cuh"
@@ -51,6 +52,36 @@ ws_status_t launch(const Err &err, void (*kernel)(P), dim3 grid, unsigned thread
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params);
     return e == cudaSuccess ? WS_OK : err(WS_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+}
+
+// ---- norms
+template <int NV, bool VEC>
+auto norm_kernel(const NormParams &p) {
+    constexpr int F = WS_ACT_F32;
+    if constexpr (!VEC) return block_norm_rows_kernel<NV, false, true, true, true>;  // (types are looked at as it runs)
+    else if (p.y_dtype == F)
+        return p.r_dtype == F ? (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, true, true, true> : block_norm_rows_kernel<NV, VEC, true, true, false>)
+                              : (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, true, false, true> : block_norm_rows_kernel<NV, VEC, true, false, false>);
+    else
+        return p.r_dtype == F ? (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, false, true, true> : block_norm_rows_kernel<NV, VEC, false, true, false>)
+                          : (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, false, false, true> : block_norm_rows_kernel<NV, VEC, false, false, false>);
+}
+template <int NV>
+ws_status_t launch_norm(const Err &err, bool vec, const NormParams &p, void *stream) {
+    const unsigned threads = (unsigned)((p.n + NV * 8 * 32 - 1) / (NV * 8 * 32)) * 32;
+    return launch(err, vec ? norm_kernel<NV, true>(p) : norm_kernel<NV, false>(p), dim3((unsigned)p.m), threads, 0, 1, stream, p);
+}
+ws_status_t norm(const Err &err, const NormParams &p, void *stream) {
+    auto wide = [](const void *q, int64_t ld, int32_t type) { return !q || aligned(q, ld, type, 8 * type_bytes(type)); };
+    const bool vec = p.n % 8 == 0 && wide(p.y, p.ldy, p.y_dtype) && wide(p.residual, p.ldr, p.r_dtype) && (!p.gate_inc || wide(p.gate, p.ldg, p.g_dtype)) &&
+                     wide(p.post_weight, 0, p.w_dtype) && wide(p.next_weight, 0, p.w_dtype) && wide(p.hidden, p.ldh, p.h_dtype) && wide(p.normed, p.ldn, p.n_dtype);
+    static const char *ev = getenv("NV");
+    int nv = ev ? atoi(ev) : p.m <= 296 ? 1 : 2;
+    if (nv < 4 && p.n > 8192) nv = 4;
+    if (p.n > 16384) {
+        return launch(err, block_norm_any_kernel, dim3((unsigned)p.m), 512, 0, 1, stream, p);
+    }
+    return nv == 1 ? launch_norm<1>(err, vec, p, stream) : nv == 2 ? launch_norm<2>(err, vec, p, stream) : launch_norm<4>(err, vec, p, stream);
 }
 
 // ---- adapters
@@ -185,8 +216,7 @@ ws_status_t ws_block_norm(const ws_block_norm_args_t *a, void *stream, char *err
     p.y_dtype = a->y_dtype; p.r_dtype = a->residual_dtype; p.g_dtype = a->gate_dtype; p.w_dtype = a->weight_dtype;
     p.h_dtype = a->hidden_dtype; p.n_dtype = a->normed_dtype;
     p.weight_offset = a->weight_offset; p.eps = a->eps; p.residual_scale = a->residual_scale; p.block_scale = a->block_scale;
-    const unsigned threads = (unsigned)std::min(512, (p.n + 31) / 32 * 32);
-    return launch(err, block_norm_any_kernel, dim3((unsigned)p.m), threads, 0, 1, stream, p);
+    return norm(err, p, stream);
 }
 
 ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *a, void *stream, char *err_text, size_t err_len) {

@@ -227,15 +227,30 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
             }
         }
         if (big >= mine) {
+            // the batch lies before the token, where equal values count, or behind it, or around it (or holds places
+            // outside the row that look like a masked token)
+            const int32_t i0 = x.first(v), i1 = x.first(v + (kScoreBatch - 1) * kScoreThreads) + E;
+            const bool front = i1 <= tok && mine > kNegInf, behind = i0 > tok;
+            if (front || behind) {
 #pragma unroll
-            for (int j = 0; j < kScoreBatch; ++j) {
-                float c[E];
-                Row::values(raw[j], c);
-                const int32_t i0 = x.first(v + j * kScoreThreads);
+                for (int j = 0; j < kScoreBatch; ++j) {
+                    float c[E];
+                    Row::values(raw[j], c);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int32_t i = i0 + e;
-                    a.before += (c[e] > mine || (c[e] == mine && i < tok)) && i >= 0 && i < p.vocab && v + j * kScoreThreads < v1;
+                    for (int e = 0; e < E; ++e) a.before += front ? c[e] >= mine : c[e] > mine;
+                }
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < kScoreBatch; ++j) {
+                    const int32_t w = v + j * kScoreThreads;
+                    if (w >= v1) break;
+                    float c[E];
+                    Row::values(x.raw(w), c);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const int32_t i = x.first(w) + e;
+                        a.before += (c[e] > mine || (c[e] == mine && i < tok)) && i >= 0 && i < p.vocab;
+                    }
                 }
             }
         }
