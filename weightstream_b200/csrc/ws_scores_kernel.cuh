@@ -4,9 +4,11 @@
 // both rescaled when M moves:  lse = M + ln s,  entropy = ln s - t / s.  A row is read by a cluster of 1 to 8 blocks,
 // whose statistics meet in the first block's shared memory.
 //
-// The alternatives cost the pass nothing but the vector in which a thread's maximum lies: the k-th best of 64 groups'
-// maxima is a lower bound of the k-th best value, and only threads whose maximum reaches it can hold an alternative.
-// Their values (about k threads') are read once more, and what reaches the bound is ranked in shared memory.
+// The alternatives cost the pass little: the k-th best of 64 groups' maxima is a lower bound of the k-th best value, and
+// only threads whose maximum reaches it can hold an alternative.  After a quarter of the row the bound is taken for the
+// first time, and values that reach it are noted as they pass; at the end it is taken again, the first quarter's values
+// of the threads whose maximum reaches it (about k threads) are read once more, and what is left is ranked in shared
+// memory.  A short row's share of a block is read once more whole.
 //
 // Order of values: larger first, equal ones by index, as argmax has it (crates/weightstream-ref/src/sample.rs:13-23).
 // -inf (masked) and NaN are never alternatives.
@@ -18,8 +20,8 @@
 
 namespace ws {
 
-constexpr int kScoreThreads = 512;
-constexpr int kScoreGroups = kScoreThreads / 8;   // groups of eight lanes whose maxima give the bound
+constexpr int kScoreThreads = 256;
+constexpr int kScoreGroups = kScoreThreads / 4;   // groups of four lanes whose maxima give the bound
 constexpr int kScoreBatch = 4;                    // vectors a thread requests together
 constexpr int kScoreMaxTop = 32;
 constexpr int kScoreMaxCluster = 8;
@@ -44,6 +46,23 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of t
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
+}
+// Two floats at a time: the sums of a pass are issue-bound otherwise.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(r) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
+    return *reinterpret_cast<float2 *>(&r);
 }
 // (value, index) as one number that is larger for what comes first; 0 is below all of them.  -0 and 0 are equal.
 __device__ __forceinline__ uint64_t score_key(float v, uint32_t idx) {
@@ -113,15 +132,15 @@ __device__ __forceinline__ void rebase(ScoreStats &a, float to) {
     a.m = to;
 }
 
+constexpr int kScoreNoted = 1024;                     // values noted in passing; more: all are read once more
 struct ScoreShared {
-    uint64_t buf[kScoreThreads + kScoreThreads * 8];  // values that reach the bound: a round adds at most eight a thread
+    uint64_t buf[kScoreNoted + kScoreThreads * 8];    // values that reach the bound: a round of reading adds at most eight a thread
     uint64_t best[kScoreMaxTop];                      // this block's alternatives in order, 0 where there are no more
     uint64_t group[kScoreGroups];
     uint64_t bound;
     ScoreStats stats;                                 // this block's
-    float warp_m[kScoreThreads / 32], warp_s[kScoreThreads / 32], warp_t[kScoreThreads / 32];
-    int32_t warp_before[kScoreThreads / 32];
-    int32_t list[kScoreThreads], listed, found;
+    ScoreStats warp[kScoreThreads / 32];
+    int32_t list[kScoreThreads], listed, found, kept;
 };
 
 // The `top` first of buf[0, n), n <= kScoreThreads, in order into best[]; the rest of best[] is 0.
@@ -169,11 +188,36 @@ __device__ __noinline__ void shrink_candidates(ScoreShared &sh, int n, int top) 
     __syncthreads();
 }
 
+// Bound of single values: the top-th best of the groups' maxima, given as (value, vector) of every thread, and of that
+// vector its last value.
+template <typename Row>
+__device__ __forceinline__ uint64_t take_bound(ScoreShared &sh, const Row &x, uint64_t key, int top) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int o = 2; o; o >>= 1) {
+        const uint64_t c = __shfl_xor_sync(0xffffffffu, key, o);
+        if (c > key) key = c;
+    }
+    if ((tid & 3) == 0) sh.group[tid >> 2] = key;
+    __syncthreads();
+    // every group is compared with sixteen others by each of four threads
+    const int i = tid >> 2, j0 = (tid & 3) * (kScoreGroups / 4);
+    const uint64_t g = sh.group[i];
+    int r = 0;
+#pragma unroll
+    for (int j = j0; j < j0 + kScoreGroups / 4; ++j) r += sh.group[j] > g || (sh.group[j] == g && j < i);
+    r += __shfl_xor_sync(0xffffffffu, r, 1);
+    r += __shfl_xor_sync(0xffffffffu, r, 2);
+    if ((tid & 3) == 0 && r == top - 1) sh.bound = g == 0 ? 1 : (g & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)(x.first(key_index(g)) + Row::E - 1));
+    __syncthreads();
+    return sh.bound;
+}
+
 template <bool F32, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __grid_constant__ ScoreParams p) {
+__global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __grid_constant__ ScoreParams p) {
     namespace cg = cooperative_groups;
     using Row = ScoreRow<F32>;
-    constexpr int E = Row::E;
+    constexpr int E = Row::E, kStep = kScoreBatch * kScoreThreads;
     __shared__ ScoreShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int part = blockIdx.x % p.cluster;
@@ -181,23 +225,40 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     wait_predecessor();
     const Row x(static_cast<const char *>(p.logits) + row * p.ld * (F32 ? 4 : 2), p.vocab);
-    const int64_t tok = p.token_bytes == 8 ? static_cast<const int64_t *>(p.tokens)[row] : static_cast<const int32_t *>(p.tokens)[row];
-    const bool has_tok = tok >= 0 && tok < p.vocab;
-    const float mine = has_tok ? load1(p.logits, F32 ? WS_ACT_F32 : WS_ACT_BF16, row * p.ld + tok) : __uint_as_float(0x7FC00000u);
     const int64_t all = x.vectors();
     const int32_t v0 = (int32_t)(all * part / p.cluster), v1 = (int32_t)(all * (part + 1) / p.cluster);
-
-    ScoreStats a{kLowest, 0.0f, 0.0f, 0};
-    float best = kNegInf;   // maximum of this thread's values, and the first vector that holds it
-    int32_t best_v = 0;
-    for (int32_t v = v0 + tid; v < v1; v += kScoreBatch * kScoreThreads) {
-        uint4 raw[kScoreBatch];
+    // a batch of vectors is requested while the one before it is worked on
+    uint4 next[kScoreBatch];
+    auto request = [&](int32_t v) {
 #pragma unroll
         for (int j = 0; j < kScoreBatch; ++j) {
             const int32_t w = v + j * kScoreThreads;
-            raw[j] = F32 ? make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u) : make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
-            if (w < v1) raw[j] = x.raw(w);
+            next[j] = F32 ? make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u) : make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
+            if (w < v1) next[j] = x.raw(w);
         }
+    };
+    request(v0 + tid);
+    const int64_t tok = p.token_bytes == 8 ? static_cast<const int64_t *>(p.tokens)[row] : static_cast<const int32_t *>(p.tokens)[row];
+    const bool has_tok = tok >= 0 && tok < p.vocab;
+    const float mine = has_tok ? load1(p.logits, F32 ? WS_ACT_F32 : WS_ACT_BF16, row * p.ld + tok) : __uint_as_float(0x7FC00000u);
+
+    const int batches = (v1 - v0 + kStep - 1) / kStep;   // the same for all threads of the block
+    const int early = TOP && batches >= 8 ? batches / 4 : batches;
+    if (TOP && tid == 0) sh.listed = sh.found = sh.kept = 0;
+    float m = kLowest, best = kNegInf;   // best: maximum of this thread's values; m: what s and t refer to
+    int32_t best_v = 0, before = 0;      // the first vector that holds it
+    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;
+    float note = __uint_as_float(0x7FC00000u);  // values from here on are noted; NaN: none
+    for (int b = 0; b < batches; ++b) {
+        if (TOP && b == early) {
+            const uint64_t k = take_bound(sh, x, best > kNegInf ? score_key(best, (uint32_t)best_v) : 0, p.top);
+            note = k == 1 ? kNegInf : key_value(k);  // 1: too few groups hold anything yet, so all that follows counts
+        }
+        const int32_t v = v0 + tid + b * kStep;
+        uint4 raw[kScoreBatch];
+#pragma unroll
+        for (int j = 0; j < kScoreBatch; ++j) raw[j] = next[j];
+        if (b + 1 < batches) request(v + kStep);
         float most[kScoreBatch], big = kNegInf;
 #pragma unroll
         for (int j = 0; j < kScoreBatch; ++j) {
@@ -210,34 +271,51 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
         }
         if (big > best) {
             best = big;
-            rebase(a, big);
+            const float d = fmaxf(m - big, kFarBelow), f = ex2f(d * 1.44269504f);
+            const float2 d2 = make_float2(d, d), f2 = make_float2(f, f);
+            t2 = mul2(f2, fma2(d2, s2, t2));
+            s2 = mul2(f2, s2);
+            m = big;
 #pragma unroll
             for (int j = kScoreBatch - 1; j >= 0; --j)
                 if (most[j] == big) best_v = v + j * kScoreThreads;
         }
+        const float2 m2 = make_float2(-m, -m);
 #pragma unroll
         for (int j = 0; j < kScoreBatch; ++j) {
             float c[E];
             Row::values(raw[j], c);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float d = max_nan(c[e] - a.m, kFarBelow), q = ex2f(d * 1.44269504f);
-                a.s += q;
-                a.t = fmaf(q, d, a.t);
+            for (int e = 0; e < E; e += 2) {
+                float2 d = add2(make_float2(c[e], c[e + 1]), m2);
+                d.x = max_nan(d.x, kFarBelow);
+                d.y = max_nan(d.y, kFarBelow);
+                float2 q = mul2(d, make_float2(1.44269504f, 1.44269504f));
+                q.x = ex2f(q.x);
+                q.y = ex2f(q.y);
+                s2 = add2(s2, q);
+                t2 = fma2(q, d, t2);
             }
         }
         if (big >= mine) {
             // the batch lies before the token, where equal values count, or behind it, or around it (or holds places
             // outside the row that look like a masked token)
             const int32_t i0 = x.first(v), i1 = x.first(v + (kScoreBatch - 1) * kScoreThreads) + E;
-            const bool front = i1 <= tok && mine > kNegInf, behind = i0 > tok;
-            if (front || behind) {
+            if (i0 > tok) {
 #pragma unroll
                 for (int j = 0; j < kScoreBatch; ++j) {
                     float c[E];
                     Row::values(raw[j], c);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) a.before += front ? c[e] >= mine : c[e] > mine;
+                    for (int e = 0; e < E; ++e) before += c[e] > mine;
+                }
+            } else if (i1 <= tok && mine > kNegInf) {
+#pragma unroll
+                for (int j = 0; j < kScoreBatch; ++j) {
+                    float c[E];
+                    Row::values(raw[j], c);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) before += c[e] >= mine;
                 }
             } else {
 #pragma unroll 1
@@ -249,53 +327,56 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         const int32_t i = x.first(w) + e;
-                        a.before += (c[e] > mine || (c[e] == mine && i < tok)) && i >= 0 && i < p.vocab;
+                        before += (c[e] > mine || (c[e] == mine && i < tok)) && i >= 0 && i < p.vocab;
                     }
                 }
             }
         }
+        if (TOP && big >= note) {
+#pragma unroll
+            for (int j = 0; j < kScoreBatch; ++j) {
+                if (!(most[j] >= note)) continue;
+                float c[E];
+                Row::values(raw[j], c);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (c[e] >= note && c[e] > kNegInf) {
+                        const int at = atomicAdd(&sh.found, 1);
+                        if (at < kScoreNoted) sh.buf[at] = score_key(c[e], (uint32_t)(x.first(v + j * kScoreThreads) + e));
+                    }
+            }
+        }
     }
+    ScoreStats a{m, s2.x + s2.y, t2.x + t2.y, before};
 
     // the block's statistics
-    float m = a.m;
+    float wm = a.m;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    rebase(a, m);
+    for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+    rebase(a, wm);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
         a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
         a.before += __shfl_xor_sync(0xffffffffu, a.before, o);
     }
-    if (lane == 0) {
-        sh.warp_m[warp] = a.m;
-        sh.warp_s[warp] = a.s;
-        sh.warp_t[warp] = a.t;
-        sh.warp_before[warp] = a.before;
-    }
-    uint64_t key = 0;
+    if (lane == 0) sh.warp[warp] = a;
+    uint64_t key = 0, bound = 0;
     if (TOP) {
         key = best > kNegInf ? score_key(best, (uint32_t)best_v) : 0;
-        uint64_t g = key;
-#pragma unroll
-        for (int o = 4; o; o >>= 1) {
-            const uint64_t c = __shfl_xor_sync(0xffffffffu, g, o);
-            if (c > g) g = c;
-        }
-        if ((lane & 7) == 0) sh.group[tid >> 3] = g;
-        if (tid == 0) sh.listed = sh.found = 0;
+        bound = take_bound(sh, x, key, p.top);
+    } else {
+        __syncthreads();
     }
-    __syncthreads();
     if (warp == 0) {
         constexpr int W = kScoreThreads / 32;
-        ScoreStats b{lane < W ? sh.warp_m[lane] : kLowest, lane < W ? sh.warp_s[lane] : 0.0f, lane < W ? sh.warp_t[lane] : 0.0f,
-                     lane < W ? sh.warp_before[lane] : 0};
+        ScoreStats b = lane < W ? sh.warp[lane] : ScoreStats{kLowest, 0.0f, 0.0f, 0};
         float bm = b.m;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
+        for (int o = W / 2; o; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
         rebase(b, bm);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
+        for (int o = W / 2; o; o >>= 1) {
             b.s += __shfl_xor_sync(0xffffffffu, b.s, o);
             b.t += __shfl_xor_sync(0xffffffffu, b.t, o);
             b.before += __shfl_xor_sync(0xffffffffu, b.before, o);
@@ -303,23 +384,32 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
         if (lane == 0) sh.stats = b;
     }
     if (TOP) {
-        // the top-th best of the groups' maxima: every group is compared with eight others by each of eight threads
-        const int i = tid >> 3, j0 = (tid & 7) * (kScoreGroups / 8);
-        const uint64_t g = sh.group[i];
-        int r = 0;
+        // of what was noted, what reaches the bound now
+        const int noted = sh.found;
+        const bool again = noted > kScoreNoted;  // not all of it is there
+        uint64_t keep[kScoreNoted / kScoreThreads];
 #pragma unroll
-        for (int j = j0; j < j0 + kScoreGroups / 8; ++j) r += sh.group[j] > g || (sh.group[j] == g && j < i);
-#pragma unroll
-        for (int o = 4; o; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
-        // ... as a bound on single values: the last value of that vector
-        if ((tid & 7) == 0 && r == p.top - 1) sh.bound = g == 0 ? 1 : (g & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)(x.first(key_index(g)) + E - 1));
-        __syncthreads();
-        uint64_t bound = sh.bound;
-        // (this thread's best vector as a single value: its first, so that none of the vector is lost)
+        for (int i = 0; i < kScoreNoted / kScoreThreads; ++i) {
+            const int at = tid + i * kScoreThreads;
+            keep[i] = !again && at < noted ? sh.buf[at] : 0;
+        }
+        // threads whose best vector (its first value, so that none of it is lost) reaches it
         if (key != 0 && ((key & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)max(x.first(best_v), 0))) >= bound) sh.list[atomicAdd(&sh.listed, 1)] = tid;
         __syncthreads();
-        const int rounds = (v1 - v0 + kScoreThreads - 1) / kScoreThreads, items = sh.listed * rounds;
-        for (int w0 = 0; w0 < items; w0 += kScoreThreads) {
+#pragma unroll
+        for (int i = 0; i < kScoreNoted / kScoreThreads; ++i)
+            if (keep[i] >= bound) sh.buf[atomicAdd(&sh.kept, 1)] = keep[i];
+        __syncthreads();
+        const int rounds = again ? batches * kScoreBatch : early * kScoreBatch, items = sh.listed * rounds;
+        if (tid == 0) sh.found = sh.kept;
+        __syncthreads();
+        for (int w0 = 0;; w0 += kScoreThreads) {
+            if (sh.found > kScoreThreads) {
+                shrink_candidates(sh, sh.found, p.top);
+                bound = sh.bound;
+            }
+            __syncthreads();
+            if (w0 >= items) break;
             const int w = w0 + tid;
             if (w < items) {
                 const int32_t v = v0 + sh.list[w / rounds] + (w % rounds) * kScoreThreads;
@@ -333,11 +423,6 @@ __global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const __gri
                         if (k >= bound) sh.buf[atomicAdd(&sh.found, 1)] = k;
                     }
                 }
-            }
-            __syncthreads();
-            if (sh.found > kScoreThreads) {
-                shrink_candidates(sh, sh.found, p.top);
-                bound = sh.bound;
             }
             __syncthreads();
         }
