@@ -84,6 +84,18 @@ ws_status_t norm(const Err &err, const NormParams &p, void *stream) {
     return nv == 1 ? launch_norm<1>(err, vec, p, stream) : nv == 2 ? launch_norm<2>(err, vec, p, stream) : launch_norm<4>(err, vec, p, stream);
 }
 
+// ---- scores
+template <int T>
+ws_status_t launch_scores(const Err &err, bool f32, const ScoreParams &p, void *stream) {
+    auto *k = f32 ? (p.top ? token_scores_kernel<T, true, true> : token_scores_kernel<T, true, false>)
+                  : (p.top ? token_scores_kernel<T, false, true> : token_scores_kernel<T, false, false>);
+    if (p.cluster > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return err(WS_ERR_CUDA, "clusters of %d: %s", p.cluster, cudaGetErrorString(e));
+    }
+    return launch(err, k, dim3((unsigned)p.m * p.cluster), T, 0, (unsigned)p.cluster, stream, p);
+}
+
 // ---- adapters
 int64_t lora_max_tiles(int m, int adapters, int tile) { return ((int64_t)m + tile - 1) / tile + std::min((int64_t)adapters + 1, (int64_t)m); }
 int64_t lora_perm_bytes(int m) { return 16 + ((int64_t)m * 4 + 15) / 16 * 16; }
@@ -237,14 +249,14 @@ ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *a, void *stream, c
     ScoreParams p{};
     p.logits = a->logits; p.tokens = a->tokens; p.ld = a->ld; p.m = a->m; p.vocab = a->vocab; p.top = a->top; p.token_bytes = a->token_bytes;
     p.logprob = a->logprob; p.entropy = a->entropy; p.top_logprob = a->top_logprob; p.rank = a->rank; p.top_id = a->top_id;
-    const int per = (a->dtype == WS_ACT_F32 ? 4 : 8) * kScoreThreads;  // values of one round of a block
-    int c = 1;
-    while (c < kScoreMaxCluster && (int64_t)a->m * c * 2 <= 2 * 148 && a->vocab / (2 * c) >= per) c *= 2;
+    static const char *ec = getenv("SC"), *et = getenv("ST");
+    int c = 1, t = 256;
+    const int per = (a->dtype == WS_ACT_F32 ? 4 : 8) * t;  // values of one round of a block
+    while (c < 8 && (int64_t)a->m * c * 2 <= 2 * 148 && a->vocab / (2 * c) >= per) c *= 2;
+    if (ec) c = atoi(ec);
+    if (et) t = atoi(et);
     p.cluster = c;
-    const dim3 grid((unsigned)a->m * c);
-    auto *k = a->dtype == WS_ACT_F32 ? (a->top ? token_scores_kernel<true, true> : token_scores_kernel<true, false>)
-                                     : (a->top ? token_scores_kernel<false, true> : token_scores_kernel<false, false>);
-    return launch(err, k, grid, kScoreThreads, 0, (unsigned)c, stream, p);
+    return t == 512 ? launch_scores<512>(err, a->dtype == WS_ACT_F32, p, stream) : launch_scores<256>(err, a->dtype == WS_ACT_F32, p, stream);
 }
 
 }  // extern "C"

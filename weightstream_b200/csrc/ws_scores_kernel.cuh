@@ -20,11 +20,9 @@
 
 namespace ws {
 
-constexpr int kScoreThreads = 256;
-constexpr int kScoreGroups = kScoreThreads / 4;   // groups of four lanes whose maxima give the bound
-constexpr int kScoreBatch = 4;                    // vectors a thread requests together
+constexpr int kScoreGroups = 64;                  // groups of neighbouring threads whose maxima give the bound
 constexpr int kScoreMaxTop = 32;
-constexpr int kScoreMaxCluster = 8;
+constexpr int kScoreMaxCluster = 16;
 constexpr float kLowest = -3.402823466e+38f, kNegInf = -__builtin_huge_valf();
 constexpr float kFarBelow = -10000.0f;            // exp of it is 0 and its product with 0 is 0, as exp(-inf) (-inf) is not
 static_assert(kScoreMaxTop <= kScoreGroups, "the bound needs a group for every alternative");
@@ -133,37 +131,48 @@ __device__ __forceinline__ void rebase(ScoreStats &a, float to) {
 }
 
 constexpr int kScoreNoted = 1024;                     // values noted in passing; more: all are read once more
+template <int T>
 struct ScoreShared {
-    uint64_t buf[kScoreNoted + kScoreThreads * 8];    // values that reach the bound: a round of reading adds at most eight a thread
+    uint64_t buf[kScoreNoted + T * 8];    // values that reach the bound: a round of reading adds at most eight a thread
     uint64_t best[kScoreMaxTop];                      // this block's alternatives in order, 0 where there are no more
     uint64_t group[kScoreGroups];
     uint64_t bound;
     ScoreStats stats;                                 // this block's
-    ScoreStats warp[kScoreThreads / 32];
-    int32_t list[kScoreThreads], listed, found, kept;
+    ScoreStats warp[T / 32];
+    int32_t list[T], listed, found, kept;
 };
 
-// The `top` first of buf[0, n), n <= kScoreThreads, in order into best[]; the rest of best[] is 0.
-__device__ __forceinline__ void rank_candidates(const uint64_t *buf, int n, int top, uint64_t *best) {
+// The `top` first of the distinct keys of buf[0, n), n <= T, in order into best[]; the rest of best[] is 0.  Zeros of buf
+// are no keys.
+template <int T>
+__device__ __forceinline__ void rank_candidates(ScoreShared<T> &sh, int n, int top) {
     const int tid = threadIdx.x;
-    if (tid < top && tid >= n) best[tid] = 0;
-    if (tid < n) {
-        const uint64_t k = buf[tid];
+    if (tid < top) sh.best[tid] = 0;
+    if (tid == T - 1) sh.buf[n] = 0;  // n may be odd
+    __syncthreads();
+    const uint64_t k = tid < n ? sh.buf[tid] : 0;
+    if (k) {
         int r = 0;
-        for (int j = 0; j < n; ++j) r += buf[j] > k || (buf[j] == k && j < tid);
-        if (r < top) best[r] = k;
+#pragma unroll 4
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(sh.buf + j);
+            r += c.x > k;
+            r += c.y > k;
+        }
+        if (r < top) sh.best[r] = k;
     }
     __syncthreads();
 }
 
 // Too many values reach the bound (many equal maxima, or few threads hold all large values): the `top` first of buf[0, n)
 // by repeated maxima, back into buf[0, top).  The bound rises to the last of them.
-__device__ __noinline__ void shrink_candidates(ScoreShared &sh, int n, int top) {
+template <int T>
+__device__ __noinline__ void shrink_candidates(ScoreShared<T> &sh, int n, int top) {
     const int tid = threadIdx.x, lane = tid & 31;
     uint64_t last = ~(uint64_t)0;
     for (int r = 0; r < top; ++r) {
         uint64_t k = 0;
-        for (int i = tid; i < n; i += kScoreThreads) {
+        for (int i = tid; i < n; i += T) {
             const uint64_t c = sh.buf[i];
             if (c < last && c > k) k = c;
         }
@@ -174,7 +183,7 @@ __device__ __noinline__ void shrink_candidates(ScoreShared &sh, int n, int top) 
         }
         if (lane == 0) sh.group[tid >> 5] = k;
         __syncthreads();
-        for (int w = 0; w < kScoreThreads / 32; ++w)
+        for (int w = 0; w < T / 32; ++w)
             if (sh.group[w] > k) k = sh.group[w];
         if (tid == 0) sh.best[r] = k;
         last = k;
@@ -190,35 +199,36 @@ __device__ __noinline__ void shrink_candidates(ScoreShared &sh, int n, int top) 
 
 // Bound of single values: the top-th best of the groups' maxima, given as (value, vector) of every thread, and of that
 // vector its last value.
-template <typename Row>
-__device__ __forceinline__ uint64_t take_bound(ScoreShared &sh, const Row &x, uint64_t key, int top) {
+template <int T, typename Row>
+__device__ __forceinline__ uint64_t take_bound(ScoreShared<T> &sh, const Row &x, uint64_t key, int top) {
+    constexpr int G = T / kScoreGroups;   // threads of a group
     const int tid = threadIdx.x;
 #pragma unroll
-    for (int o = 2; o; o >>= 1) {
+    for (int o = G / 2; o; o >>= 1) {
         const uint64_t c = __shfl_xor_sync(0xffffffffu, key, o);
         if (c > key) key = c;
     }
-    if ((tid & 3) == 0) sh.group[tid >> 2] = key;
+    if (tid % G == 0) sh.group[tid / G] = key;
     __syncthreads();
-    // every group is compared with sixteen others by each of four threads
-    const int i = tid >> 2, j0 = (tid & 3) * (kScoreGroups / 4);
+    // every group is compared with all, a part of them by each of its threads
+    const int i = tid / G, j0 = tid % G * (kScoreGroups / G);
     const uint64_t g = sh.group[i];
     int r = 0;
 #pragma unroll
-    for (int j = j0; j < j0 + kScoreGroups / 4; ++j) r += sh.group[j] > g || (sh.group[j] == g && j < i);
-    r += __shfl_xor_sync(0xffffffffu, r, 1);
-    r += __shfl_xor_sync(0xffffffffu, r, 2);
-    if ((tid & 3) == 0 && r == top - 1) sh.bound = g == 0 ? 1 : (g & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)(x.first(key_index(g)) + Row::E - 1));
+    for (int j = j0; j < j0 + kScoreGroups / G; ++j) r += sh.group[j] > g || (sh.group[j] == g && j < i);
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+    if (tid % G == 0 && r == top - 1) sh.bound = g == 0 ? 1 : (g & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)(x.first(key_index(g)) + Row::E - 1));
     __syncthreads();
     return sh.bound;
 }
 
-template <bool F32, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __grid_constant__ ScoreParams p) {
+template <int T, bool F32, bool TOP>
+__global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const __grid_constant__ ScoreParams p) {
     namespace cg = cooperative_groups;
     using Row = ScoreRow<F32>;
-    constexpr int E = Row::E, kStep = kScoreBatch * kScoreThreads;
-    __shared__ ScoreShared sh;
+    constexpr int E = Row::E, kBatch = F32 ? 4 : 2, kStep = kBatch * T;   // vectors a thread requests together
+    __shared__ __align__(16) ScoreShared<T> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int part = blockIdx.x % p.cluster;
     const int64_t row = blockIdx.x / p.cluster;
@@ -228,11 +238,11 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
     const int64_t all = x.vectors();
     const int32_t v0 = (int32_t)(all * part / p.cluster), v1 = (int32_t)(all * (part + 1) / p.cluster);
     // a batch of vectors is requested while the one before it is worked on
-    uint4 next[kScoreBatch];
+    uint4 next[kBatch];
     auto request = [&](int32_t v) {
 #pragma unroll
-        for (int j = 0; j < kScoreBatch; ++j) {
-            const int32_t w = v + j * kScoreThreads;
+        for (int j = 0; j < kBatch; ++j) {
+            const int32_t w = v + j * T;
             next[j] = F32 ? make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u) : make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
             if (w < v1) next[j] = x.raw(w);
         }
@@ -255,13 +265,13 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
             note = k == 1 ? kNegInf : key_value(k);  // 1: too few groups hold anything yet, so all that follows counts
         }
         const int32_t v = v0 + tid + b * kStep;
-        uint4 raw[kScoreBatch];
+        uint4 raw[kBatch];
 #pragma unroll
-        for (int j = 0; j < kScoreBatch; ++j) raw[j] = next[j];
+        for (int j = 0; j < kBatch; ++j) raw[j] = next[j];
         if (b + 1 < batches) request(v + kStep);
-        float most[kScoreBatch], big = kNegInf;
+        float most[kBatch], big = kNegInf;
 #pragma unroll
-        for (int j = 0; j < kScoreBatch; ++j) {
+        for (int j = 0; j < kBatch; ++j) {
             float c[E];
             Row::values(raw[j], c);
             most[j] = c[0];
@@ -277,12 +287,12 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
             s2 = mul2(f2, s2);
             m = big;
 #pragma unroll
-            for (int j = kScoreBatch - 1; j >= 0; --j)
-                if (most[j] == big) best_v = v + j * kScoreThreads;
+            for (int j = kBatch - 1; j >= 0; --j)
+                if (most[j] == big) best_v = v + j * T;
         }
         const float2 m2 = make_float2(-m, -m);
 #pragma unroll
-        for (int j = 0; j < kScoreBatch; ++j) {
+        for (int j = 0; j < kBatch; ++j) {
             float c[E];
             Row::values(raw[j], c);
 #pragma unroll
@@ -300,10 +310,10 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
         if (big >= mine) {
             // the batch lies before the token, where equal values count, or behind it, or around it (or holds places
             // outside the row that look like a masked token)
-            const int32_t i0 = x.first(v), i1 = x.first(v + (kScoreBatch - 1) * kScoreThreads) + E;
+            const int32_t i0 = x.first(v), i1 = x.first(v + (kBatch - 1) * T) + E;
             if (i0 > tok) {
 #pragma unroll
-                for (int j = 0; j < kScoreBatch; ++j) {
+                for (int j = 0; j < kBatch; ++j) {
                     float c[E];
                     Row::values(raw[j], c);
 #pragma unroll
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
                 }
             } else if (i1 <= tok && mine > kNegInf) {
 #pragma unroll
-                for (int j = 0; j < kScoreBatch; ++j) {
+                for (int j = 0; j < kBatch; ++j) {
                     float c[E];
                     Row::values(raw[j], c);
 #pragma unroll
@@ -319,8 +329,8 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
                 }
             } else {
 #pragma unroll 1
-                for (int j = 0; j < kScoreBatch; ++j) {
-                    const int32_t w = v + j * kScoreThreads;
+                for (int j = 0; j < kBatch; ++j) {
+                    const int32_t w = v + j * T;
                     if (w >= v1) break;
                     float c[E];
                     Row::values(x.raw(w), c);
@@ -334,7 +344,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
         }
         if (TOP && big >= note) {
 #pragma unroll
-            for (int j = 0; j < kScoreBatch; ++j) {
+            for (int j = 0; j < kBatch; ++j) {
                 if (!(most[j] >= note)) continue;
                 float c[E];
                 Row::values(raw[j], c);
@@ -342,7 +352,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
                 for (int e = 0; e < E; ++e)
                     if (c[e] >= note && c[e] > kNegInf) {
                         const int at = atomicAdd(&sh.found, 1);
-                        if (at < kScoreNoted) sh.buf[at] = score_key(c[e], (uint32_t)(x.first(v + j * kScoreThreads) + e));
+                        if (at < kScoreNoted) sh.buf[at] = score_key(c[e], (uint32_t)(x.first(v + j * T) + e));
                     }
             }
         }
@@ -369,7 +379,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
         __syncthreads();
     }
     if (warp == 0) {
-        constexpr int W = kScoreThreads / 32;
+        constexpr int W = T / 32;
         ScoreStats b = lane < W ? sh.warp[lane] : ScoreStats{kLowest, 0.0f, 0.0f, 0};
         float bm = b.m;
 #pragma unroll
@@ -387,24 +397,24 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
         // of what was noted, what reaches the bound now
         const int noted = sh.found;
         const bool again = noted > kScoreNoted;  // not all of it is there
-        uint64_t keep[kScoreNoted / kScoreThreads];
+        uint64_t keep[kScoreNoted / T];
 #pragma unroll
-        for (int i = 0; i < kScoreNoted / kScoreThreads; ++i) {
-            const int at = tid + i * kScoreThreads;
+        for (int i = 0; i < kScoreNoted / T; ++i) {
+            const int at = tid + i * T;
             keep[i] = !again && at < noted ? sh.buf[at] : 0;
         }
         // threads whose best vector (its first value, so that none of it is lost) reaches it
         if (key != 0 && ((key & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)max(x.first(best_v), 0))) >= bound) sh.list[atomicAdd(&sh.listed, 1)] = tid;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kScoreNoted / kScoreThreads; ++i)
+        for (int i = 0; i < kScoreNoted / T; ++i)
             if (keep[i] >= bound) sh.buf[atomicAdd(&sh.kept, 1)] = keep[i];
         __syncthreads();
-        const int rounds = again ? batches * kScoreBatch : early * kScoreBatch, items = sh.listed * rounds;
+        const int rounds = again ? batches * kBatch : early * kBatch, items = sh.listed * rounds;
         if (tid == 0) sh.found = sh.kept;
         __syncthreads();
-        for (int w0 = 0;; w0 += kScoreThreads) {
-            if (sh.found > kScoreThreads) {
+        for (int w0 = 0;; w0 += T) {
+            if (sh.found > T) {
                 shrink_candidates(sh, sh.found, p.top);
                 bound = sh.bound;
             }
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
             if (w0 >= items) break;
             const int w = w0 + tid;
             if (w < items) {
-                const int32_t v = v0 + sh.list[w / rounds] + (w % rounds) * kScoreThreads;
+                const int32_t v = v0 + sh.list[w / rounds] + (w % rounds) * T;
                 if (v < v1) {
                     float c[E];
                     Row::values(x.raw(v), c);
@@ -426,7 +436,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
             }
             __syncthreads();
         }
-        rank_candidates(sh.buf, sh.found, p.top, sh.best);
+        rank_candidates(sh, sh.found, p.top);
     } else {
         __syncthreads();
     }
@@ -454,7 +464,7 @@ __global__ void __launch_bounds__(kScoreThreads, 3) token_scores_kernel(const __
         }
         cl.sync();  // no block leaves while its shared memory is read
         if (part != 0) return;
-        if (TOP) rank_candidates(sh.buf, p.cluster * p.top, p.top, sh.best);
+        if (TOP) rank_candidates(sh, p.cluster * p.top, p.top);
     }
     const float ln_s = logf(b.s);
     if (tid == 0) {
