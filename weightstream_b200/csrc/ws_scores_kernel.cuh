@@ -1,14 +1,14 @@
 // Scores of given tokens on a row of logits: log probability, entropy, rank, and the best alternatives, from one pass.
 //
 // Every thread keeps the running maximum M of what it has seen with  s = sum exp(x - M)  and  t = sum exp(x - M) (x - M),
-// both rescaled when M moves:  lse = M + ln s,  entropy = ln s - t / s.  A row is read by a cluster of 1 to 8 blocks,
-// whose statistics meet in the first block's shared memory.
+// both rescaled when M moves:  lse = M + ln s,  entropy = ln s - t / s.  A row is read by a cluster of 1 to 16 blocks,
+// which store their statistics and alternatives into the first block's shared memory.
 //
 // The alternatives cost the pass little: the k-th best of 64 groups' maxima is a lower bound of the k-th best value, and
-// only threads whose maximum reaches it can hold an alternative.  After a quarter of the row the bound is taken for the
-// first time, and values that reach it are noted as they pass; at the end it is taken again, the first quarter's values
-// of the threads whose maximum reaches it (about k threads) are read once more, and what is left is ranked in shared
-// memory.  A short row's share of a block is read once more whole.
+// only threads whose maximum reaches it can hold an alternative.  After a sixteenth and a quarter of the row the bound is
+// taken, and values that reach it are noted as they pass; at the end it is taken again, the first sixteenth's values of
+// the threads whose maximum reaches it (about k threads) are read once more (a row that is one batch still has them in
+// registers), and what is left is ranked in shared memory.
 //
 // Order of values: larger first, equal ones by index, as argmax has it (crates/weightstream-ref/src/sample.rs:13-23).
 // -inf (masked) and NaN are never alternatives.
@@ -44,6 +44,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of t
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
+}
+__device__ __forceinline__ float warp_max(float v) {  // on all lanes; NaN counts as nothing
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 // Two floats at a time: the sums of a pass are issue-bound otherwise.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -133,35 +138,31 @@ __device__ __forceinline__ void rebase(ScoreStats &a, float to) {
 constexpr int kScoreNoted = 1024;                     // values noted in passing; more: all are read once more
 template <int T>
 struct ScoreShared {
-    uint64_t buf[kScoreNoted + T * 8];    // values that reach the bound: a round of reading adds at most eight a thread
-    uint64_t best[kScoreMaxTop];                      // this block's alternatives in order, 0 where there are no more
+    // values that reach the bound: up to T wait while a round of reading adds at most eight a thread
+    uint64_t buf[T + T * 8];
+    uint64_t best[T];                                 // in the first block: every block's alternatives in order, 0 where there are no more
     uint64_t group[kScoreGroups];
     uint64_t bound;
-    ScoreStats stats;                                 // this block's
-    ScoreStats warp[T / 32];
+    ScoreStats warp[kScoreMaxCluster * T / 32];       // in the first block: those of the cluster's warps
     int32_t list[T], listed, found, kept;
 };
 
-// The `top` first of the distinct keys of buf[0, n), n <= T, in order into best[]; the rest of best[] is 0.  Zeros of buf
-// are no keys.
+// The `top` first of the distinct keys buf[0, n), n <= T, in order into best[]; the rest of best[] is 0.
 template <int T>
-__device__ __forceinline__ void rank_candidates(ScoreShared<T> &sh, int n, int top) {
+__device__ __forceinline__ void rank_candidates(const uint64_t *buf, int n, int top, uint64_t *best) {
     const int tid = threadIdx.x;
-    if (tid < top) sh.best[tid] = 0;
-    if (tid == T - 1) sh.buf[n] = 0;  // n may be odd
-    __syncthreads();
-    const uint64_t k = tid < n ? sh.buf[tid] : 0;
-    if (k) {
-        int r = 0;
+    int g = 1;  // threads to a key
+    while (g < 32 && n * g * 2 <= T) g *= 2;
+    const int i = tid / g;
+    int r = 0;
+    const uint64_t k = i < n ? buf[i] : 0;
+    if (i < n) {
 #pragma unroll 4
-        for (int j = 0; j < n; j += 2) {
-            const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(sh.buf + j);
-            r += c.x > k;
-            r += c.y > k;
-        }
-        if (r < top) sh.best[r] = k;
+        for (int j = tid % g; j < n; j += g) r += buf[j] > k;
     }
-    __syncthreads();
+    for (int o = g / 2; o; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+    if (i < n && tid % g == 0 && r < top) best[r] = k;
+    if (tid >= n && tid < top) best[tid] = 0;
 }
 
 // Too many values reach the bound (many equal maxima, or few threads hold all large values): the `top` first of buf[0, n)
@@ -169,7 +170,7 @@ __device__ __forceinline__ void rank_candidates(ScoreShared<T> &sh, int n, int t
 template <int T>
 __device__ __noinline__ void shrink_candidates(ScoreShared<T> &sh, int n, int top) {
     const int tid = threadIdx.x, lane = tid & 31;
-    uint64_t last = ~(uint64_t)0;
+    uint64_t last = ~(uint64_t)0, mine = 0;  // (thread r keeps the r-th)
     for (int r = 0; r < top; ++r) {
         uint64_t k = 0;
         for (int i = tid; i < n; i += T) {
@@ -185,11 +186,11 @@ __device__ __noinline__ void shrink_candidates(ScoreShared<T> &sh, int n, int to
         __syncthreads();
         for (int w = 0; w < T / 32; ++w)
             if (sh.group[w] > k) k = sh.group[w];
-        if (tid == 0) sh.best[r] = k;
+        if (tid == r) mine = k;
         last = k;
         __syncthreads();
     }
-    if (tid < top) sh.buf[tid] = sh.best[tid];
+    if (tid < top) sh.buf[tid] = mine;
     if (tid == 0) {
         sh.found = top;
         sh.bound = last;
@@ -232,6 +233,8 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int part = blockIdx.x % p.cluster;
     const int64_t row = blockIdx.x / p.cluster;
+    cg::cluster_group cl = cg::this_cluster();
+    if (p.cluster > 1) cl.barrier_arrive();  // waited for before the first block's shared memory is written
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     wait_predecessor();
     const Row x(static_cast<const char *>(p.logits) + row * p.ld * (F32 ? 4 : 2), p.vocab);
@@ -253,19 +256,19 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
     const float mine = has_tok ? load1(p.logits, F32 ? WS_ACT_F32 : WS_ACT_BF16, row * p.ld + tok) : __uint_as_float(0x7FC00000u);
 
     const int batches = (v1 - v0 + kStep - 1) / kStep;   // the same for all threads of the block
-    const int early = TOP && batches >= 8 ? batches / 4 : batches;
+    const int early = TOP && batches > 2 ? (batches + 15) / 16 : batches, later = 4 * early;
     if (TOP && tid == 0) sh.listed = sh.found = sh.kept = 0;
     float m = kLowest, best = kNegInf;   // best: maximum of this thread's values; m: what s and t refer to
     int32_t best_v = 0, before = 0;      // the first vector that holds it
     float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;
     float note = __uint_as_float(0x7FC00000u);  // values from here on are noted; NaN: none
+    uint4 raw[kBatch];
     for (int b = 0; b < batches; ++b) {
-        if (TOP && b == early) {
+        if (TOP && (b == early || b == later)) {
             const uint64_t k = take_bound(sh, x, best > kNegInf ? score_key(best, (uint32_t)best_v) : 0, p.top);
             note = k == 1 ? kNegInf : key_value(k);  // 1: too few groups hold anything yet, so all that follows counts
         }
         const int32_t v = v0 + tid + b * kStep;
-        uint4 raw[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) raw[j] = next[j];
         if (b + 1 < batches) request(v + kStep);
@@ -359,113 +362,119 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
     }
     ScoreStats a{m, s2.x + s2.y, t2.x + t2.y, before};
 
-    // the block's statistics
-    float wm = a.m;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    rebase(a, wm);
+    // the warps' statistics, into the first block
+    ScoreShared<T> *const first = p.cluster > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
+    rebase(a, warp_max(a.m));
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
         a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
-        a.before += __shfl_xor_sync(0xffffffffu, a.before, o);
     }
-    if (lane == 0) sh.warp[warp] = a;
-    uint64_t key = 0, bound = 0;
+    a.before = __reduce_add_sync(0xffffffffu, a.before);
+    if (p.cluster > 1) cl.barrier_wait();
+    if (lane == 0) first->warp[part * (T / 32) + warp] = a;
     if (TOP) {
-        key = best > kNegInf ? score_key(best, (uint32_t)best_v) : 0;
-        bound = take_bound(sh, x, key, p.top);
-    } else {
-        __syncthreads();
-    }
-    if (warp == 0) {
-        constexpr int W = T / 32;
-        ScoreStats b = lane < W ? sh.warp[lane] : ScoreStats{kLowest, 0.0f, 0.0f, 0};
-        float bm = b.m;
+        const uint64_t key = best > kNegInf ? score_key(best, (uint32_t)best_v) : 0;
+        uint64_t bound = take_bound(sh, x, key, p.top);
+        // threads whose best vector (its first value, so that none of it is lost) reaches the bound
+        const bool reaches = key != 0 && ((key & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)max(x.first(best_v), 0))) >= bound;
+        if (batches == 1) {
+            // (the threads of at most `top` groups, 16 values each: half of the threads' at the most, which buf holds)
+            if (reaches) {
 #pragma unroll
-        for (int o = W / 2; o; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
-        rebase(b, bm);
-#pragma unroll
-        for (int o = W / 2; o; o >>= 1) {
-            b.s += __shfl_xor_sync(0xffffffffu, b.s, o);
-            b.t += __shfl_xor_sync(0xffffffffu, b.t, o);
-            b.before += __shfl_xor_sync(0xffffffffu, b.before, o);
-        }
-        if (lane == 0) sh.stats = b;
-    }
-    if (TOP) {
-        // of what was noted, what reaches the bound now
-        const int noted = sh.found;
-        const bool again = noted > kScoreNoted;  // not all of it is there
-        uint64_t keep[kScoreNoted / T];
-#pragma unroll
-        for (int i = 0; i < kScoreNoted / T; ++i) {
-            const int at = tid + i * T;
-            keep[i] = !again && at < noted ? sh.buf[at] : 0;
-        }
-        // threads whose best vector (its first value, so that none of it is lost) reaches it
-        if (key != 0 && ((key & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)max(x.first(best_v), 0))) >= bound) sh.list[atomicAdd(&sh.listed, 1)] = tid;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kScoreNoted / T; ++i)
-            if (keep[i] >= bound) sh.buf[atomicAdd(&sh.kept, 1)] = keep[i];
-        __syncthreads();
-        const int rounds = again ? batches * kBatch : early * kBatch, items = sh.listed * rounds;
-        if (tid == 0) sh.found = sh.kept;
-        __syncthreads();
-        for (int w0 = 0;; w0 += T) {
-            if (sh.found > T) {
-                shrink_candidates(sh, sh.found, p.top);
-                bound = sh.bound;
-            }
-            __syncthreads();
-            if (w0 >= items) break;
-            const int w = w0 + tid;
-            if (w < items) {
-                const int32_t v = v0 + sh.list[w / rounds] + (w % rounds) * T;
-                if (v < v1) {
+                for (int j = 0; j < kBatch; ++j) {
                     float c[E];
-                    Row::values(x.raw(v), c);
+                    Row::values(raw[j], c);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        if (!(c[e] > kNegInf)) continue;
-                        const uint64_t k = score_key(c[e], (uint32_t)(x.first(v) + e));
-                        if (k >= bound) sh.buf[atomicAdd(&sh.found, 1)] = k;
+                        const uint64_t k = score_key(c[e], (uint32_t)(x.first(v0 + tid + j * T) + e));
+                        if (c[e] > kNegInf && k >= bound) sh.buf[atomicAdd(&sh.found, 1)] = k;
                     }
                 }
             }
             __syncthreads();
-        }
-        rank_candidates(sh, sh.found, p.top);
-    } else {
-        __syncthreads();
-    }
-
-    // the row's
-    ScoreStats b = sh.stats;
-    if (p.cluster > 1) {
-        cg::cluster_group cl = cg::this_cluster();
-        cl.sync();
-        if (part == 0) {
-            float bm = kLowest;
-            for (int c = 0; c < p.cluster; ++c) bm = fmaxf(bm, cl.map_shared_rank(&sh, c)->stats.m);
-            b = ScoreStats{bm, 0.0f, 0.0f, 0};
-            for (int c = 0; c < p.cluster; ++c) {
-                ScoreStats o = cl.map_shared_rank(&sh, c)->stats;
-                rebase(o, bm);
-                b.s += o.s;
-                b.t += o.t;
-                b.before += o.before;
+            if (sh.found > T) shrink_candidates(sh, sh.found, p.top);
+        } else {
+            // of what was noted, what reaches the bound now
+            const int noted = sh.found;
+            const bool again = noted > kScoreNoted;  // not all of it is there
+            if (reaches) sh.list[atomicAdd(&sh.listed, 1)] = tid;
+            if (noted && !again) {
+                uint64_t keep[kScoreNoted / T];
+#pragma unroll
+                for (int i = 0; i < kScoreNoted / T; ++i) keep[i] = tid + i * T < noted ? sh.buf[tid + i * T] : 0;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kScoreNoted / T; ++i)
+                    if (keep[i] >= bound) sh.buf[atomicAdd(&sh.kept, 1)] = keep[i];
             }
-            if (TOP) {
-                if (tid < p.cluster * p.top) sh.buf[tid] = cl.map_shared_rank(&sh, tid / p.top)->best[tid % p.top];
+            __syncthreads();
+            const int rounds = (again ? batches : early) * kBatch, items = sh.listed * rounds;
+            if (tid == 0) sh.found = sh.kept;
+            __syncthreads();
+            for (int w0 = 0;; w0 += T) {
+                if (sh.found > T) {
+                    shrink_candidates(sh, sh.found, p.top);
+                    bound = sh.bound;
+                }
+                __syncthreads();
+                if (w0 >= items) break;
+                const int w = w0 + tid;
+                if (w < items) {
+                    const int32_t v = v0 + sh.list[w / rounds] + (w % rounds) * T;
+                    if (v < v1) {
+                        float c[E];
+                        Row::values(x.raw(v), c);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const uint64_t k = score_key(c[e], (uint32_t)(x.first(v) + e));
+                            if (c[e] > kNegInf && k >= bound) sh.buf[atomicAdd(&sh.found, 1)] = k;
+                        }
+                    }
+                }
                 __syncthreads();
             }
         }
-        cl.sync();  // no block leaves while its shared memory is read
-        if (part != 0) return;
-        if (TOP) rank_candidates(sh, p.cluster * p.top, p.top);
+        rank_candidates<T>(sh.buf, sh.found, p.top, first->best + part * p.top);
     }
+
+    // the row's
+    if (p.cluster > 1) cl.sync();
+    else __syncthreads();
+    if (part != 0) return;
+    if (TOP && p.cluster > 1) {
+        // the best of the blocks' last ones is a bound again
+        uint64_t bound = 1;
+        for (int c = 0; c < p.cluster; ++c) {
+            const uint64_t k = sh.best[c * p.top + p.top - 1];
+            if (k > bound) bound = k;
+        }
+        const uint64_t k = tid < p.cluster * p.top ? sh.best[tid] : 0;
+        if (tid == 0) sh.found = 0;
+        __syncthreads();
+        if (k >= bound) sh.buf[atomicAdd(&sh.found, 1)] = k;
+        __syncthreads();
+        rank_candidates<T>(sh.buf, sh.found, p.top, sh.best);
+        __syncthreads();
+    }
+    if (warp != 0) return;
+    ScoreStats b{kLowest, 0.0f, 0.0f, 0};
+    const int warps = p.cluster * (T / 32);
+    for (int w = lane; w < warps; w += 32) b.m = fmaxf(b.m, sh.warp[w].m);
+    b.m = warp_max(b.m);
+    for (int w = lane; w < warps; w += 32) {
+        ScoreStats o = sh.warp[w];
+        rebase(o, b.m);
+        b.s += o.s;
+        b.t += o.t;
+        b.before += o.before;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        b.s += __shfl_xor_sync(0xffffffffu, b.s, o);
+        b.t += __shfl_xor_sync(0xffffffffu, b.t, o);
+    }
+    b.before = __reduce_add_sync(0xffffffffu, b.before);
     const float ln_s = logf(b.s);
     if (tid == 0) {
         const bool none = b.s == 0.0f;
