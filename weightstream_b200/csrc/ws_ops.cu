@@ -89,11 +89,10 @@ template <int T>
 ws_status_t launch_scores(const Err &err, bool f32, const ScoreParams &p, void *stream) {
     auto *k = f32 ? (p.top ? token_scores_kernel<T, true, true> : token_scores_kernel<T, true, false>)
                   : (p.top ? token_scores_kernel<T, false, true> : token_scores_kernel<T, false, false>);
-    if (p.cluster > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return err(WS_ERR_CUDA, "clusters of %d: %s", p.cluster, cudaGetErrorString(e));
-    }
-    return launch(err, k, dim3((unsigned)p.m * p.cluster), T, 0, (unsigned)p.cluster, stream, p);
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmem<T>);
+    if (e == cudaSuccess && p.cluster > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return err(WS_ERR_CUDA, "clusters of %d blocks with %d bytes of shared memory: %s", p.cluster, kScoreSmem<T>, cudaGetErrorString(e));
+    return launch(err, k, dim3((unsigned)p.m * p.cluster), T, kScoreSmem<T>, (unsigned)p.cluster, stream, p);
 }
 
 // ---- adapters

@@ -1,7 +1,7 @@
 // Scores of given tokens on a row of logits: log probability, entropy, rank, and the best alternatives, from one pass.
 //
-// Every thread keeps the running maximum M of what it has seen with  s = sum exp(x - M)  and  t = sum exp(x - M) (x - M),
-// both rescaled when M moves:  lse = M + ln s,  entropy = ln s - t / s.  A row is read by a cluster of 1 to 16 blocks,
+// Every thread keeps  s = sum exp(x - M)  and  t = sum exp(x - M) (x - M)  for an M near the maximum of what it has seen
+// (up to 16 below it: exp(16) times the values' count is far from the type's end), both rescaled when M moves:  lse = M + ln s,  entropy = ln s - t / s.  A row is read by a cluster of 1 to 16 blocks,
 // which store their statistics and alternatives into the first block's shared memory.
 //
 // The alternatives cost the pass little: the k-th best of 64 groups' maxima is a lower bound of the k-th best value, and
@@ -21,9 +21,13 @@
 namespace ws {
 
 constexpr int kScoreGroups = 64;                  // groups of neighbouring threads whose maxima give the bound
+constexpr int kScoreBatch = 4;                    // vectors a thread works on together
 constexpr int kScoreMaxTop = 32;
+template <int T>
+constexpr int kScoreRings = T == 512 ? 2 : 3;     // batches in flight and at work
 constexpr int kScoreMaxCluster = 16;
 constexpr float kLowest = -3.402823466e+38f, kNegInf = -__builtin_huge_valf();
+constexpr float kScoreSlack = 16.0f;
 constexpr float kFarBelow = -10000.0f;            // exp of it is 0 and its product with 0 is 0, as exp(-inf) (-inf) is not
 static_assert(kScoreMaxTop <= kScoreGroups, "the bound needs a group for every alternative");
 
@@ -67,6 +71,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "=l"(r) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
     return *reinterpret_cast<float2 *>(&r);
 }
+__device__ __forceinline__ void async_copy16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // (value, index) as one number that is larger for what comes first; 0 is below all of them.  -0 and 0 are equal.
 __device__ __forceinline__ uint64_t score_key(float v, uint32_t idx) {
     const uint32_t b = __float_as_uint(v + 0.0f);
@@ -139,7 +149,7 @@ constexpr int kScoreNoted = 1024;                     // values noted in passing
 template <int T>
 struct ScoreShared {
     // values that reach the bound: up to T wait while a round of reading adds at most eight a thread
-    uint64_t buf[T + T * 8];
+    alignas(16) uint64_t buf[T + T * 8];
     uint64_t best[T];                                 // in the first block: every block's alternatives in order, 0 where there are no more
     uint64_t group[kScoreGroups];
     uint64_t bound;
@@ -198,10 +208,10 @@ __device__ __noinline__ void shrink_candidates(ScoreShared<T> &sh, int n, int to
     __syncthreads();
 }
 
-// Bound of single values: the top-th best of the groups' maxima, given as (value, vector) of every thread, and of that
-// vector its last value.
-template <int T, typename Row>
-__device__ __forceinline__ uint64_t take_bound(ScoreShared<T> &sh, const Row &x, uint64_t key, int top) {
+// Bound of single values: the top-th best of the groups' maxima, given as (value, batch) of every thread, and of that
+// batch its last value.
+template <int T, typename F>
+__device__ __forceinline__ uint64_t take_bound(ScoreShared<T> &sh, const F &last_of, uint64_t key, int top) {
     constexpr int G = T / kScoreGroups;   // threads of a group
     const int tid = threadIdx.x;
 #pragma unroll
@@ -219,17 +229,24 @@ __device__ __forceinline__ uint64_t take_bound(ScoreShared<T> &sh, const Row &x,
     for (int j = j0; j < j0 + kScoreGroups / G; ++j) r += sh.group[j] > g || (sh.group[j] == g && j < i);
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
-    if (tid % G == 0 && r == top - 1) sh.bound = g == 0 ? 1 : (g & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)(x.first(key_index(g)) + Row::E - 1));
+    if (tid % G == 0 && r == top - 1) sh.bound = g == 0 ? 1 : (g & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)last_of(key_index(g)));
     __syncthreads();
     return sh.bound;
 }
+
+template <int T>
+constexpr int kScoreSmem = sizeof(ScoreShared<T>) + kScoreRings<T> * kScoreBatch * T * 16;
 
 template <int T, bool F32, bool TOP>
 __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const __grid_constant__ ScoreParams p) {
     namespace cg = cooperative_groups;
     using Row = ScoreRow<F32>;
-    constexpr int E = Row::E, kBatch = F32 ? 4 : 2, kStep = kBatch * T;   // vectors a thread requests together
-    __shared__ __align__(16) ScoreShared<T> sh;
+    constexpr int E = Row::E, kBatch = kScoreBatch, kStep = kBatch * T;
+    constexpr int kScoreRing = kScoreRings<T>;
+    constexpr uint32_t kMasked = F32 ? 0xFF800000u : 0xFF80FF80u;
+    extern __shared__ __align__(16) uint8_t score_smem[];
+    ScoreShared<T> &sh = *reinterpret_cast<ScoreShared<T> *>(score_smem);
+    uint4 *const ring = reinterpret_cast<uint4 *>(score_smem + sizeof(ScoreShared<T>));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int part = blockIdx.x % p.cluster;
     const int64_t row = blockIdx.x / p.cluster;
@@ -240,38 +257,46 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
     const Row x(static_cast<const char *>(p.logits) + row * p.ld * (F32 ? 4 : 2), p.vocab);
     const int64_t all = x.vectors();
     const int32_t v0 = (int32_t)(all * part / p.cluster), v1 = (int32_t)(all * (part + 1) / p.cluster);
-    // a batch of vectors is requested while the one before it is worked on
-    uint4 next[kBatch];
-    auto request = [&](int32_t v) {
+    // Batches are requested a ring's length ahead, straight into shared memory; a thread reads back what it asked for.
+    const int batches = (v1 - v0 + kStep - 1) / kStep;   // the same for all threads of the block
+    auto vector = [&](int b, int j) { return v0 + b * kStep + j * T + tid; };
+    auto request = [&](int b) {
+        if (b < batches) {
+            uint4 *slot = ring + (b % kScoreRing) * kStep + tid;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const int32_t w = v + j * T;
-            next[j] = F32 ? make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u) : make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
-            if (w < v1) next[j] = x.raw(w);
+            for (int j = 0; j < kBatch; ++j) {
+                const int32_t v = vector(b, j), i0 = x.first(v);
+                if (v >= v1) slot[j * T] = make_uint4(kMasked, kMasked, kMasked, kMasked);
+                else if (i0 >= 0 && i0 <= p.vocab - E) async_copy16(slot + j * T, x.base + (int64_t)v * 16);
+                else slot[j * T] = x.raw(v);
+            }
         }
+        async_commit();
     };
-    request(v0 + tid);
+#pragma unroll
+    for (int b = 0; b + 1 < kScoreRing; ++b) request(b);
     const int64_t tok = p.token_bytes == 8 ? static_cast<const int64_t *>(p.tokens)[row] : static_cast<const int32_t *>(p.tokens)[row];
     const bool has_tok = tok >= 0 && tok < p.vocab;
     const float mine = has_tok ? load1(p.logits, F32 ? WS_ACT_F32 : WS_ACT_BF16, row * p.ld + tok) : __uint_as_float(0x7FC00000u);
 
-    const int batches = (v1 - v0 + kStep - 1) / kStep;   // the same for all threads of the block
+    auto last_of = [&](int b) { return x.first(min(v0 + (b + 1) * kStep, v1)) - 1; };
     const int early = TOP && batches > 2 ? (batches + 15) / 16 : batches, later = 4 * early;
     if (TOP && tid == 0) sh.listed = sh.found = sh.kept = 0;
-    float m = kLowest, best = kNegInf;   // best: maximum of this thread's values; m: what s and t refer to
-    int32_t best_v = 0, before = 0;      // the first vector that holds it
+    float m = kLowest, best = kNegInf;   // m: what s and t refer to; best: maximum of this thread's values
+    int32_t best_b = 0, before = 0;      // the first batch that holds it
     float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;
     float note = __uint_as_float(0x7FC00000u);  // values from here on are noted; NaN: none
     uint4 raw[kBatch];
     for (int b = 0; b < batches; ++b) {
         if (TOP && (b == early || b == later)) {
-            const uint64_t k = take_bound(sh, x, best > kNegInf ? score_key(best, (uint32_t)best_v) : 0, p.top);
+            const uint64_t k = take_bound(sh, last_of, best > kNegInf ? score_key(best, (uint32_t)best_b) : 0, p.top);
             note = k == 1 ? kNegInf : key_value(k);  // 1: too few groups hold anything yet, so all that follows counts
         }
-        const int32_t v = v0 + tid + b * kStep;
+        const int32_t v = vector(b, 0);
+        request(b + kScoreRing - 1);
+        async_wait<kScoreRing - 1>();
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) raw[j] = next[j];
-        if (b + 1 < batches) request(v + kStep);
+        for (int j = 0; j < kBatch; ++j) raw[j] = ring[(b % kScoreRing) * kStep + j * T + tid];
         float most[kBatch], big = kNegInf;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -284,14 +309,14 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
         }
         if (big > best) {
             best = big;
+            best_b = b;
+        }
+        if (big > m + kScoreSlack) {
             const float d = fmaxf(m - big, kFarBelow), f = ex2f(d * 1.44269504f);
             const float2 d2 = make_float2(d, d), f2 = make_float2(f, f);
             t2 = mul2(f2, fma2(d2, s2, t2));
             s2 = mul2(f2, s2);
             m = big;
-#pragma unroll
-            for (int j = kBatch - 1; j >= 0; --j)
-                if (most[j] == big) best_v = v + j * T;
         }
         const float2 m2 = make_float2(-m, -m);
 #pragma unroll
@@ -364,7 +389,7 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
 
     // the warps' statistics, into the first block
     ScoreShared<T> *const first = p.cluster > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
-    rebase(a, warp_max(a.m));
+    rebase(a, fmaxf(warp_max(best), kLowest));
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
@@ -374,26 +399,29 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
     if (p.cluster > 1) cl.barrier_wait();
     if (lane == 0) first->warp[part * (T / 32) + warp] = a;
     if (TOP) {
-        const uint64_t key = best > kNegInf ? score_key(best, (uint32_t)best_v) : 0;
-        uint64_t bound = take_bound(sh, x, key, p.top);
-        // threads whose best vector (its first value, so that none of it is lost) reaches the bound
-        const bool reaches = key != 0 && ((key & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)max(x.first(best_v), 0))) >= bound;
+        const uint64_t key = best > kNegInf ? score_key(best, (uint32_t)best_b) : 0;
+        uint64_t bound = take_bound(sh, last_of, key, p.top);
+        // threads whose best batch (by its first value, so that none of it is lost) reaches the bound
+        const bool reaches = key != 0 && ((key & 0xFFFFFFFF00000000ull) | (0xFFFFFFFFu - (uint32_t)max(x.first(v0 + best_b * kStep), 0))) >= bound;
         if (batches == 1) {
-            // (the threads of at most `top` groups, 16 values each: half of the threads' at the most, which buf holds)
-            if (reaches) {
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
+            for (int j = 0; j < kBatch; ++j) {
+                if (reaches) {
                     float c[E];
                     Row::values(raw[j], c);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const uint64_t k = score_key(c[e], (uint32_t)(x.first(v0 + tid + j * T) + e));
+                        const uint64_t k = score_key(c[e], (uint32_t)(x.first(vector(0, j)) + e));
                         if (c[e] > kNegInf && k >= bound) sh.buf[atomicAdd(&sh.found, 1)] = k;
                     }
                 }
+                __syncthreads();
+                if (sh.found > T) {
+                    shrink_candidates(sh, sh.found, p.top);
+                    bound = sh.bound;
+                }
+                __syncthreads();
             }
-            __syncthreads();
-            if (sh.found > T) shrink_candidates(sh, sh.found, p.top);
         } else {
             // of what was noted, what reaches the bound now
             const int noted = sh.found;
