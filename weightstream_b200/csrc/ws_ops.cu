@@ -89,9 +89,8 @@ template <int T>
 ws_status_t launch_scores(const Err &err, bool f32, const ScoreParams &p, void *stream) {
     auto *k = f32 ? (p.top ? token_scores_kernel<T, true, true> : token_scores_kernel<T, true, false>)
                   : (p.top ? token_scores_kernel<T, false, true> : token_scores_kernel<T, false, false>);
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmem<T>);
-    if (e == cudaSuccess && p.cluster > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return err(WS_ERR_CUDA, "clusters of %d blocks with %d bytes of shared memory: %s", p.cluster, kScoreSmem<T>, cudaGetErrorString(e));
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmem<T>);
+    if (e != cudaSuccess) return err(WS_ERR_CUDA, "%d bytes of shared memory: %s", kScoreSmem<T>, cudaGetErrorString(e));
     return launch(err, k, dim3((unsigned)p.m * p.cluster), T, kScoreSmem<T>, (unsigned)p.cluster, stream, p);
 }
 
@@ -248,13 +247,15 @@ ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *a, void *stream, c
     ScoreParams p{};
     p.logits = a->logits; p.tokens = a->tokens; p.ld = a->ld; p.m = a->m; p.vocab = a->vocab; p.top = a->top; p.token_bytes = a->token_bytes;
     p.logprob = a->logprob; p.entropy = a->entropy; p.top_logprob = a->top_logprob; p.rank = a->rank; p.top_id = a->top_id;
-    static const char *ec = getenv("SC"), *et = getenv("ST");
-    int c = 1, t = 256;
-    const int per = (a->dtype == WS_ACT_F32 ? 4 : 8) * t;  // values of one round of a block
-    while (c < 8 && (int64_t)a->m * c * 2 <= 2 * 148 && a->vocab / (2 * c) >= per) c *= 2;
-    if (ec) c = atoi(ec);
-    if (et) t = atoi(et);
+    // Few rows: a row is cut over a cluster, as long as two blocks an SM take them all (64 rows: 17 us with four blocks a
+    // row, 23 with two, 29 with eight) and a thread of each has a vector.  Blocks of 512 threads then have the shorter way
+    // (one row 9 us against 12, 64 rows 17 against 21); three blocks of 256 an SM stream faster when there are more (2000
+    // rows 157 us against 161, with 20 alternatives 193 against 217).
+    const int vector = a->dtype == WS_ACT_F32 ? 4 : 8;
+    int c = 1;
+    while (c < 8 && (int64_t)a->m * c * 2 <= 320 && a->vocab / (2 * c) >= vector * 256) c *= 2;
     p.cluster = c;
+    const int t = (int64_t)a->m * c <= 296 ? 512 : 256;
     return t == 512 ? launch_scores<512>(err, a->dtype == WS_ACT_F32, p, stream) : launch_scores<256>(err, a->dtype == WS_ACT_F32, p, stream);
 }
 

@@ -1,7 +1,7 @@
 // Scores of given tokens on a row of logits: log probability, entropy, rank, and the best alternatives, from one pass.
 //
 // Every thread keeps  s = sum exp(x - M)  and  t = sum exp(x - M) (x - M)  for an M near the maximum of what it has seen
-// (up to 16 below it: exp(16) times the values' count is far from the type's end), both rescaled when M moves:  lse = M + ln s,  entropy = ln s - t / s.  A row is read by a cluster of 1 to 16 blocks,
+// (up to 16 below it: exp(16) times the values' count is far from the type's end), both rescaled when M moves:  lse = M + ln s,  entropy = ln s - t / s.  A row is read by a cluster of 1 to 8 blocks,
 // which store their statistics and alternatives into the first block's shared memory.
 //
 // The alternatives cost the pass little: the k-th best of 64 groups' maxima is a lower bound of the k-th best value, and
@@ -25,7 +25,7 @@ constexpr int kScoreBatch = 4;                    // vectors a thread works on t
 constexpr int kScoreMaxTop = 32;
 template <int T>
 constexpr int kScoreRings = T == 512 ? 2 : 3;     // batches in flight and at work
-constexpr int kScoreMaxCluster = 16;
+constexpr int kScoreMaxCluster = 8;
 constexpr float kLowest = -3.402823466e+38f, kNegInf = -__builtin_huge_valf();
 constexpr float kScoreSlack = 16.0f;
 constexpr float kFarBelow = -10000.0f;            // exp of it is 0 and its product with 0 is 0, as exp(-inf) (-inf) is not
@@ -70,6 +70,16 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;"
         : "=l"(r) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
     return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float one_gt(float a, float b) {  // 1 where it holds, else 0
+    float r;
+    asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float one_ge(float a, float b) {
+    float r;
+    asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 __device__ __forceinline__ void async_copy16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -260,18 +270,25 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
     // Batches are requested a ring's length ahead, straight into shared memory; a thread reads back what it asked for.
     const int batches = (v1 - v0 + kStep - 1) / kStep;   // the same for all threads of the block
     auto vector = [&](int b, int j) { return v0 + b * kStep + j * T + tid; };
+    // batches [inner0, inner1) hold nothing but whole vectors of the row
+    const int inner0 = x.first(v0) < 0 ? 1 : 0, inner1 = (min(v1, (p.vocab + x.lead) / E) - v0) / kStep;
+    int slot_in = 0, slot_out = 0;   // places of the ring
+    const char *ahead = x.base + ((int64_t)v0 + tid) * 16;
     auto request = [&](int b) {
-        if (b < batches) {
-            uint4 *slot = ring + (b % kScoreRing) * kStep + tid;
+        uint4 *slot = ring + slot_in * kStep + tid;
+        if (b >= inner0 && b < inner1) {
 #pragma unroll
+            for (int j = 0; j < kBatch; ++j) async_copy16(slot + j * T, ahead + j * T * 16);
+        } else if (b < batches) {
+#pragma unroll 1
             for (int j = 0; j < kBatch; ++j) {
-                const int32_t v = vector(b, j), i0 = x.first(v);
-                if (v >= v1) slot[j * T] = make_uint4(kMasked, kMasked, kMasked, kMasked);
-                else if (i0 >= 0 && i0 <= p.vocab - E) async_copy16(slot + j * T, x.base + (int64_t)v * 16);
-                else slot[j * T] = x.raw(v);
+                const int32_t v = vector(b, j);
+                slot[j * T] = v < v1 ? x.raw(v) : make_uint4(kMasked, kMasked, kMasked, kMasked);
             }
         }
         async_commit();
+        ahead += kStep * 16;
+        slot_in = slot_in + 1 == kScoreRing ? 0 : slot_in + 1;
     };
 #pragma unroll
     for (int b = 0; b + 1 < kScoreRing; ++b) request(b);
@@ -284,7 +301,7 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
     if (TOP && tid == 0) sh.listed = sh.found = sh.kept = 0;
     float m = kLowest, best = kNegInf;   // m: what s and t refer to; best: maximum of this thread's values
     int32_t best_b = 0, before = 0;      // the first batch that holds it
-    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;
+    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2, many = s2;  // many: counts, whole numbers far below 2^24 (checked: a thread's share of a row)
     float note = __uint_as_float(0x7FC00000u);  // values from here on are noted; NaN: none
     uint4 raw[kBatch];
     for (int b = 0; b < batches; ++b) {
@@ -296,7 +313,8 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
         request(b + kScoreRing - 1);
         async_wait<kScoreRing - 1>();
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) raw[j] = ring[(b % kScoreRing) * kStep + j * T + tid];
+        for (int j = 0; j < kBatch; ++j) raw[j] = ring[slot_out * kStep + j * T + tid];
+        slot_out = slot_out + 1 == kScoreRing ? 0 : slot_out + 1;
         float most[kBatch], big = kNegInf;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -345,7 +363,7 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
                     float c[E];
                     Row::values(raw[j], c);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) before += c[e] > mine;
+                    for (int e = 0; e < E; e += 2) many = add2(many, make_float2(one_gt(c[e], mine), one_gt(c[e + 1], mine)));
                 }
             } else if (i1 <= tok && mine > kNegInf) {
 #pragma unroll
@@ -353,7 +371,7 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
                     float c[E];
                     Row::values(raw[j], c);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) before += c[e] >= mine;
+                    for (int e = 0; e < E; e += 2) many = add2(many, make_float2(one_ge(c[e], mine), one_ge(c[e + 1], mine)));
                 }
             } else {
 #pragma unroll 1
@@ -385,7 +403,7 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : 3) token_scores_kernel(const
             }
         }
     }
-    ScoreStats a{m, s2.x + s2.y, t2.x + t2.y, before};
+    ScoreStats a{m, s2.x + s2.y, t2.x + t2.y, before + (int32_t)many.x + (int32_t)many.y};
 
     // the warps' statistics, into the first block
     ScoreShared<T> *const first = p.cluster > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
