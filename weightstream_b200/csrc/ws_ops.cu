@@ -1,6 +1,7 @@
 // C entry points of the operators between the tensor-parallel steps (include/ws_tp.h): checks of arguments, choice of
 // kernel, launch.
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -33,6 +34,20 @@ bool aligned(const void *p, int64_t ld, int32_t type, int64_t bytes) {  // first
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * type_bytes(type) % bytes == 0;
 }
 bool natural(const void *p, int32_t type) { return reinterpret_cast<uintptr_t>(p) % type_bytes(type) == 0; }
+
+// Raises a kernel's limit of dynamic shared memory, once a device.
+template <auto K>
+ws_status_t allow_smem(const Err &err, int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e == cudaSuccess && (device > 63 || !(done.load(std::memory_order_relaxed) & bit))) {
+        e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return e == cudaSuccess ? WS_OK : err(WS_ERR_CUDA, "%d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+}
 
 // The kernels begin with griddepcontrol.wait, so their launch may overlap the end of the kernel before them.
 template <typename P>
@@ -85,13 +100,16 @@ ws_status_t norm(const Err &err, const NormParams &p, void *stream) {
 }
 
 // ---- scores
+template <int T, bool F32, bool TOP>
+ws_status_t launch_scores(const Err &err, const ScoreParams &p, void *stream) {
+    constexpr auto k = token_scores_kernel<T, F32, TOP>;
+    const ws_status_t st = allow_smem<k>(err, kScoreSmem<T>);
+    return st != WS_OK ? st : launch(err, k, dim3((unsigned)p.m * p.cluster), T, kScoreSmem<T>, (unsigned)p.cluster, stream, p);
+}
 template <int T>
 ws_status_t launch_scores(const Err &err, bool f32, const ScoreParams &p, void *stream) {
-    auto *k = f32 ? (p.top ? token_scores_kernel<T, true, true> : token_scores_kernel<T, true, false>)
-                  : (p.top ? token_scores_kernel<T, false, true> : token_scores_kernel<T, false, false>);
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmem<T>);
-    if (e != cudaSuccess) return err(WS_ERR_CUDA, "%d bytes of shared memory: %s", kScoreSmem<T>, cudaGetErrorString(e));
-    return launch(err, k, dim3((unsigned)p.m * p.cluster), T, kScoreSmem<T>, (unsigned)p.cluster, stream, p);
+    if (f32) return p.top ? launch_scores<T, true, true>(err, p, stream) : launch_scores<T, true, false>(err, p, stream);
+    return p.top ? launch_scores<T, false, true>(err, p, stream) : launch_scores<T, false, false>(err, p, stream);
 }
 
 // ---- adapters
@@ -101,10 +119,10 @@ int64_t lora_perm_bytes(int m) { return 16 + ((int64_t)m * 4 + 15) / 16 * 16; }
 template <int RT, int NT, bool XF32, bool VEC>
 ws_status_t launch_lora(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
     using S = LoraShape<RT, NT>;
-    auto *k = lora_kernel<RT, NT, XF32, VEC>;
+    constexpr auto k = lora_kernel<RT, NT, XF32, VEC>;
     if (S::kSmem > 47 * 1024) {  // (48 KB with the static part)
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-        if (e != cudaSuccess) return err(WS_ERR_CUDA, "shared memory of %d bytes: %s", S::kSmem, cudaGetErrorString(e));
+        const ws_status_t st = allow_smem<k>(err, S::kSmem);
+        if (st != WS_OK) return st;
     }
     return launch(err, k, dim3(tiles * (unsigned)p.cluster), kLoraThreads, S::kSmem, (unsigned)p.cluster, stream, p);
 }
@@ -171,8 +189,8 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
         tiles = (unsigned)lora_max_tiles(a->m, a->adapters, p.tile);
         const size_t smem = (size_t)(a->adapters + 1) * 12;
         if (smem > 47 * 1024) {
-            const cudaError_t e = cudaFuncSetAttribute(lora_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kLoraMaxAdapters + 1) * 12);
-            if (e != cudaSuccess) return err(WS_ERR_CUDA, "shared memory: %s", cudaGetErrorString(e));
+            const ws_status_t st = allow_smem<lora_plan_kernel>(err, (kLoraMaxAdapters + 1) * 12);
+            if (st != WS_OK) return st;
         }
         const ws_status_t st = launch(err, lora_plan_kernel, dim3(1), 1024, smem, 1, stream, p);
         if (st != WS_OK) return st;

@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -301,8 +302,9 @@ bool result_dtype(PyObject *o, at::ScalarType otherwise, at::ScalarType *out, in
     *code = *out == at::kFloat ? WS_ACT_F32 : WS_ACT_BF16;
     return *out == at::kFloat || *out == at::kBFloat16;
 }
+// (the dispatcher's way to the same takes three times as long)
 at::Tensor new_like(const at::Tensor &like, at::IntArrayRef sizes, at::ScalarType t) {
-    return at::empty(sizes, like.options().dtype(t).requires_grad(false));
+    return at::detail::empty_cuda(sizes, t, like.device(), std::nullopt);
 }
 
 // block_norm(y, residual, post_weight, next_weight, gate, gate_act, eps, weight_offset, residual_scale, block_scale, out,

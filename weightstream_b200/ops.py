@@ -74,8 +74,13 @@ def _call(name: str, args) -> None:
         raise WsError(st, err.value.decode())
 
 
-def _handle(stream) -> Optional[int]:
-    return None if stream is None else int(stream.cuda_stream)
+_native = None  # the front end for torch tensors, once it is loaded
+
+
+def _load():
+    global _native
+    _native = _lib.torch_front()
+    return _native
 
 
 def _dim(*sizes: int) -> None:
@@ -151,8 +156,8 @@ def block_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post
     Returns ``(hidden, normed)``; ``normed`` is None without ``next_weight``.  ``hidden`` has the residual's type, or
     ``out_dtype``; ``out`` takes it and may be ``residual`` itself.
     """
-    r = _lib.torch_front().block_norm(y, residual, post_weight, next_weight, gate, _GATES.get(gate_act, -1), eps, weight_offset,
-                                      residual_scale, block_scale, out, out_dtype, normed_dtype, _handle(stream))
+    r = (_native or _load()).block_norm(y, residual, post_weight, next_weight, gate, _GATES.get(gate_act, -1), eps, weight_offset,
+                                      residual_scale, block_scale, out, out_dtype, normed_dtype, None if stream is None else stream.cuda_stream)
     if r is not None:
         return r
     a, hidden_dtype, normed_dtype = _block_norm_args(y, residual, post_weight, next_weight, gate, gate_act, eps, weight_offset,
@@ -232,7 +237,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     outside [0, adapters), such as -1, has no adapter.  Ranks of 1 to 128; sums are fp32 and no activation is rounded on
     the way.  Returns ``out``, of ``y``'s type, which may be ``y`` itself.
     """
-    r = _lib.torch_front().lora(0, y, x, a, b, ids, scale, None, out, _handle(stream))
+    r = (_native or _load()).lora(0, y, x, a, b, ids, scale, None, out, None if stream is None else stream.cuda_stream)
     if r is not None:
         return r
     args = _lora_args(ids, x=x, a=a, y=y, b=b, scale=scale, out=out)
@@ -247,7 +252,7 @@ def lora_shrink(x: torch.Tensor, a: torch.Tensor, ids: torch.Tensor, *, stream=N
     """The first half of :func:`lora_add`, ``a[ids[t]] @ x[t]`` as fp32 [m, rank], for a projection whose K is sharded: each
     rank shrinks its slice of ``x`` with its slice of ``a``, ``Endpoint.allreduce_`` adds the ranks' rows up, and
     :func:`lora_expand` follows.  Rows of tokens without an adapter are zeros."""
-    r = _lib.torch_front().lora(1, None, x, a, None, ids, None, None, None, _handle(stream))
+    r = (_native or _load()).lora(1, None, x, a, None, ids, None, None, None, None if stream is None else stream.cuda_stream)
     if r is not None:
         return r
     args = _lora_args(ids, x=x, a=a)
@@ -261,7 +266,7 @@ def lora_shrink(x: torch.Tensor, a: torch.Tensor, ids: torch.Tensor, *, stream=N
 def lora_expand(y: torch.Tensor, shrunk: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, scale: Optional[torch.Tensor] = None, *,
                 out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """The second half of :func:`lora_add`: ``out[t] = y[t] + scale[i] * b[i] @ shrunk[t]`` with ``i = ids[t]``."""
-    r = _lib.torch_front().lora(2, y, None, None, b, ids, scale, shrunk, out, _handle(stream))
+    r = (_native or _load()).lora(2, y, None, None, b, ids, scale, shrunk, out, None if stream is None else stream.cuda_stream)
     if r is not None:
         return r
     args = _lora_args(ids, y=y, b=b, scale=scale, shrunk=shrunk, out=out)
@@ -310,9 +315,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     [0, vocab), such as -1 for padding, is none: log probability 0, rank -1.  A row that is masked whole has log
     probability -inf and entropy 0; NaN or +inf in a row make its log probabilities and entropy NaN.
     """
-    r = _lib.torch_front().token_logprobs(logits, tokens, top, _handle(stream))
+    r = (_native or _load()).token_logprobs(logits, tokens, top, None if stream is None else stream.cuda_stream)
     if r is not None:
-        return TokenLogprobs(*r)
+        return tuple.__new__(TokenLogprobs, r)
     a = _token_logprobs_args(logits, tokens, top)
     with _on(logits.device, stream):
         new = lambda *shape, dtype: torch.empty(shape, dtype=dtype, device=logits.device)
