@@ -295,7 +295,7 @@ ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *args, void *stream
  * Tokens with an id outside [0, adapters), such as -1, have no adapter: out = y, shrunk rows are zeros.
  * ws_lora_add is the whole; where the projection is sharded over K every rank calls ws_lora_shrink on its slice of x
  * and of a, the ranks add the shrunk rows up (ws_allreduce_f32) and each calls ws_lora_expand.
- * The adapters are bf16, the products' sums and the shrunk rows fp32.  Up to 256 tokens need no workspace; more take
+ * The adapters are bf16, the products' sums and the shrunk rows fp32.  Up to 512 tokens need no workspace; more take
  * ws_lora_workspace(m, adapters) bytes (16-byte aligned) that the call writes first, so calls on one stream may share
  * it, and at most 16384 adapters (WS_ERR_CAPACITY beyond). */
 #define WS_LORA_MAX_RANK 128

@@ -85,7 +85,7 @@ def check(dev, m, k, n, rank, adapters, xt=BF16, yt=F32, scaled=True, pad=0, ids
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rank", [1, 4, 8, 16, 24, 32, 56, 64, 72, 128])
-@pytest.mark.parametrize("m", [1, 9, 40, 256, 257, 700])
+@pytest.mark.parametrize("m", [1, 9, 40, 256, 257, 512, 513, 700])
 def test_ranks_and_batches(dev, rank, m):
     check(dev, m, 640, 520, rank, 7)
 
@@ -110,13 +110,13 @@ def test_types(dev, xt, yt, rank, m):
 @pytest.mark.gpu
 @pytest.mark.parametrize("pad", [1, 2, 8, 24])
 def test_strides(dev, pad):
-    for m in (6, 70, 290):
+    for m in (6, 70, 290, 600):
         check(dev, m, 512, 256, 16, 4, pad=pad)
         check(dev, m, 512, 256, 64, 4, xt=F32, yt=BF16, pad=pad)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [1, 8, 65, 256, 257, 1100])
+@pytest.mark.parametrize("m", [1, 8, 65, 256, 257, 512, 1100])
 def test_ids(dev, m):
     full = lambda v: torch.full((m,), v, dtype=torch.int32, device=dev)
     check(dev, m, 256, 192, 16, 3, ids=full(-1))                      # nobody has one
@@ -131,12 +131,13 @@ def test_ids(dev, m):
 def test_many_adapters(dev):
     from weightstream_b200 import ops
     check(dev, 500, 64, 32, 8, 16384)
-    x, y = torch.zeros((257, 8), dtype=BF16, device=dev), torch.zeros((257, 4), device=dev)
+    m = 513  # a batch that is sorted
+    x, y = torch.zeros((m, 8), dtype=BF16, device=dev), torch.zeros((m, 4), device=dev)
     a, b = torch.zeros((16385, 8, 8), dtype=BF16, device=dev), torch.zeros((16385, 4, 8), dtype=BF16, device=dev)
-    ids = torch.zeros(257, dtype=torch.int32, device=dev)
+    ids = torch.zeros(m, dtype=torch.int32, device=dev)
     with pytest.raises(RuntimeError, match="CAPACITY"):
         ops.lora_add(y, x, a, b, ids)
-    ops.lora_add(y[:256], x[:256], a, b, ids[:256])
+    ops.lora_add(y[:512], x[:512], a, b, ids[:512])
 
 
 @pytest.mark.gpu
@@ -314,7 +315,7 @@ def test_c_entry_refuses_a_short_workspace(dev):
     import ctypes as C
     from weightstream_b200 import _lib, ops
     L, err = _lib.load(), C.create_string_buffer(256)
-    m = 300
+    m = 513
     p = dict(y=torch.zeros((m, 16), device=dev), x=torch.zeros((m, 32), dtype=BF16, device=dev), a=torch.zeros((2, 8, 32), dtype=BF16, device=dev),
              b=torch.zeros((2, 16, 8), dtype=BF16, device=dev), ids=torch.zeros(m, dtype=torch.int32, device=dev))
     a = ops._lora_args(**p)

@@ -25,7 +25,7 @@ constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
 constexpr int kLoraMaxRank = 128;
 constexpr int kLoraMaxCluster = 8;
-constexpr int kLoraDirect = kLoraThreads;    // up to this many tokens a block finds its tile by itself
+constexpr int kLoraDirect = 512;             // up to this many tokens a block finds its tile by itself
 constexpr int kLoraMaxAdapters = 16384;      // of a sorted batch: two words of shared memory each
 
 struct LoraTile {
@@ -156,23 +156,127 @@ __device__ __forceinline__ void row8(const float *row, int i, int limit, float (
     }
 }
 
-// Four consecutive outputs of a token.
+// Four consecutive values of a token's y, and of its result.
 template <bool VEC>
-__device__ __forceinline__ void add4(const LoraParams &p, int64_t tok, int nn, float (&d)[4]) {
+__device__ __forceinline__ void get4(const LoraParams &p, int64_t tok, int nn, float (&v)[4]) {
     if (nn >= p.n) return;
     if (VEC && p.y_dtype == WS_ACT_F32) {
         const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.y) + tok * p.ldy + nn);
-        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + tok * p.ldo + nn) = make_float4(y.x + d[0], y.y + d[1], y.z + d[2], y.w + d[3]);
+        v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
     } else if (VEC) {
         const uint2 y = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.y) + tok * p.ldy + nn);
-        const uint32_t lo = pack_bf16x2(__uint_as_float(y.x << 16) + d[0], __uint_as_float(y.x & 0xFFFF0000u) + d[1]);
-        const uint32_t hi = pack_bf16x2(__uint_as_float(y.y << 16) + d[2], __uint_as_float(y.y & 0xFFFF0000u) + d[3]);
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + tok * p.ldo + nn) = make_uint2(lo, hi);
+        v[0] = __uint_as_float(y.x << 16); v[1] = __uint_as_float(y.x & 0xFFFF0000u);
+        v[2] = __uint_as_float(y.y << 16); v[3] = __uint_as_float(y.y & 0xFFFF0000u);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = nn + j < p.n ? load1(p.y, p.y_dtype, tok * p.ldy + nn + j) : 0.0f;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void put4(const LoraParams &p, int64_t tok, int nn, const float (&v)[4]) {
+    if (nn >= p.n) return;
+    if (VEC && p.y_dtype == WS_ACT_F32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + tok * p.ldo + nn) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (VEC) {
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + tok * p.ldo + nn) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (nn + j < p.n) store1(p.out, p.y_dtype, tok * p.ldo + nn + j, load1(p.y, p.y_dtype, tok * p.ldy + nn + j) + d[j]);
+            if (nn + j < p.n) store1(p.out, p.y_dtype, tok * p.ldo + nn + j, v[j]);
     }
+}
+
+// Tokens without an adapter: their y as it is, or zeros for shrunk rows.  A block's slice of all of them together, four
+// loads a thread under way.
+template <bool VEC>
+__device__ __forceinline__ void lora_none(const LoraParams &p, const int32_t *toks, int most, int part) {
+    const int n = p.s_out ? p.r : VEC ? p.n / 4 : p.n, n0 = (int)((int64_t)n * part / p.cluster), n1 = (int)((int64_t)n * (part + 1) / p.cluster);
+    int count = 0;
+    while (count < most && toks[count] >= 0) ++count;
+    const int items = count * (n1 - n0);
+    if (p.s_out) {
+        for (int i = threadIdx.x; i < items; i += kLoraThreads) p.s_out[(int64_t)toks[i / (n1 - n0)] * p.r + n0 + i % (n1 - n0)] = 0.0f;
+        return;
+    }
+    if (p.out == p.y && p.ldo == p.ldy) return;
+    for (int i0 = threadIdx.x; i0 < items; i0 += 4 * kLoraThreads) {
+        float v[4][4];
+        int64_t tok[4];
+        int at[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * kLoraThreads;
+            tok[u] = -1;
+            if (i >= items) break;
+            tok[u] = toks[i / (n1 - n0)];
+            at[u] = n0 + i % (n1 - n0);
+            if (VEC) get4<true>(p, tok[u], at[u] * 4, v[u]);
+            else v[u][0] = load1(p.y, p.y_dtype, tok[u] * p.ldy + at[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (tok[u] < 0) break;
+            if (VEC) put4<true>(p, tok[u], at[u] * 4, v[u]);
+            else store1(p.out, p.y_dtype, tok[u] * p.ldo + at[u], v[u][0]);
+        }
+    }
+}
+
+// The tokens of tile number `tile` and their adapter; false: there are fewer tiles.  A token leads a tile if the number of
+// earlier tokens with its adapter is a multiple of the tile's size; tiles are numbered by their leaders' places, so the
+// blocks that have work come first.
+template <int TOKENS>
+__device__ __forceinline__ bool find_tile(const LoraParams &p, int tile, int32_t *toks, int &adapter) {
+    constexpr int H = kLoraDirect / kLoraThreads;   // tokens a thread looks after
+    __shared__ __align__(16) int32_t ids[kLoraDirect];
+    __shared__ uint32_t leads[kLoraDirect / 32];
+    __shared__ int32_t lead_id, lead_before;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int id[H], before[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const int i = tid + h * kLoraThreads;
+        id[h] = i < p.m ? lora_id(p, i) : -2;
+        ids[i] = id[h];
+    }
+    if (tid < TOKENS) toks[tid] = -1;
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const int i = tid + h * kLoraThreads;
+        before[h] = 0;
+        if (h * kLoraThreads >= p.m) break;
+        if (i < p.m)
+#pragma unroll 4
+            for (int j = 0; j < i; j += 4) {
+                const int4 o = *reinterpret_cast<const int4 *>(ids + j);
+                before[h] += (o.x == id[h]) + (o.y == id[h] && j + 1 < i) + (o.z == id[h] && j + 2 < i) + (o.w == id[h] && j + 3 < i);
+            }
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const bool leader = id[h] != -2 && before[h] % TOKENS == 0 && !(id[h] == -1 && p.skip_none);
+        const uint32_t all = __ballot_sync(0xffffffffu, leader);
+        if (lane == 0) leads[h * kLoraWarps + warp] = all;
+    }
+    __syncthreads();
+    int count = 0;
+    for (int w = 0; w < kLoraDirect / 32; ++w) {
+        const uint32_t all = leads[w];
+        const int n = __popc(all);
+        if (tile >= count && tile < count + n && (w % kLoraWarps) == warp && (all >> lane & 1) && __popc(all & ((1u << lane) - 1)) == tile - count) {
+            lead_id = id[w / kLoraWarps];
+            lead_before = before[w / kLoraWarps];
+        }
+        count += n;
+    }
+    if (tile >= count) return false;
+    __syncthreads();
+    adapter = lead_id;
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+        if (id[h] == adapter && before[h] >= lead_before && before[h] < lead_before + TOKENS) toks[before[h] - lead_before] = tid + h * kLoraThreads;
+    return true;
 }
 
 template <int RT, int NT>
@@ -183,7 +287,7 @@ struct LoraShape {
     static constexpr int kRow = kRanks * 2 + (RT >= 4 ? 64 : 0);
     static constexpr int kSplit = 3 * kTokens * kRow;
     static constexpr int kScratch = kLoraWarps * kSums * 4 > kSplit ? kLoraWarps * kSums * 4 : kSplit;
-    static constexpr int kSmem = kScratch + kSums * 4;
+    static constexpr int kSmem = kScratch + kLoraMaxCluster * kSums * 4;
     static constexpr int kAhead = RT * NT <= 2 ? 4 : RT * NT <= 8 ? 2 : 1;   // steps of K requested together
 };
 
@@ -193,10 +297,13 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     using S = LoraShape<RT, NT>;
     extern __shared__ __align__(16) uint8_t lora_smem[];
     float *const warps = reinterpret_cast<float *>(lora_smem);                      // [warp][kSums], then the split S
-    float *const sums = reinterpret_cast<float *>(lora_smem + S::kScratch);         // this block's S, read by the cluster
-    __shared__ int32_t toks[S::kTokens], found[kLoraWarps];
+    float *const sums = reinterpret_cast<float *>(lora_smem + S::kScratch);         // the S of the cluster's blocks, [block][kSums]
+    __shared__ int32_t toks[S::kTokens];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int C = p.cluster, part = blockIdx.x % C, tile = blockIdx.x / C;
+    cg::cluster_group cl = cg::this_cluster();
+    const bool meets = C > 1 && !p.s_in;
+    if (meets) cl.barrier_arrive();  // waited for before another block's shared memory is written
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     wait_predecessor();
 
@@ -207,34 +314,12 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
         const LoraTile q = p.tiles[tile];
         adapter = q.adapter;
         if (tid < S::kTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
-    } else {
-        // token `tile` leads a tile if the number of earlier tokens with its adapter is a multiple of the tile's size
-        adapter = lora_id(p, tile);
-        const bool same = tid < p.m && lora_id(p, tid) == adapter;
-        const uint32_t in_warp = __ballot_sync(0xffffffffu, same);
-        if (lane == 0) found[warp] = (int32_t)in_warp;
-        if (tid < S::kTokens) toks[tid] = -1;
-        __syncthreads();
-        int lead = 0, mine = __popc(in_warp & ((1u << lane) - 1));
-        for (int w = 0; w < kLoraWarps; ++w) {
-            const uint32_t f = (uint32_t)found[w];
-            lead += w < (tile >> 5) ? __popc(f) : w == (tile >> 5) ? __popc(f & ((1u << (tile & 31)) - 1)) : 0;
-            mine += w < warp ? __popc(f) : 0;
-        }
-        if (lead % S::kTokens != 0) return;  // (the same on all threads of the cluster)
-        if (same && mine >= lead && mine < lead + S::kTokens) toks[mine - lead] = tid;
+    } else if (!find_tile<S::kTokens>(p, tile, toks, adapter)) {
+        return;  // (the same on all threads of the cluster)
     }
     __syncthreads();
     if (adapter < 0) {  // nothing to add
-        for (int i = 0; i < S::kTokens; ++i) {
-            const int64_t tok = toks[i];
-            if (tok < 0) break;
-            const int n0 = (int)((int64_t)(p.s_out ? p.r : p.n) * part / C), n1 = (int)((int64_t)(p.s_out ? p.r : p.n) * (part + 1) / C);
-            for (int j = n0 + tid; j < n1; j += kLoraThreads) {
-                if (p.s_out) p.s_out[tok * p.r + j] = 0.0f;
-                else if (p.out != p.y) store1(p.out, p.y_dtype, tok * p.ldo + j, load1(p.y, p.y_dtype, tok * p.ldy + j));
-            }
-        }
+        lora_none<VEC>(p, toks, S::kTokens, part);
         return;
     }
 
@@ -305,15 +390,49 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
 #pragma unroll
                 for (int e = 0; e < 4; ++e) warps[warp * S::kSums + ((i * NT + q) * 4 + e) * 32 + lane] = acc[i][q][e];
         __syncthreads();
+        if (meets) cl.barrier_wait();
         for (int j = tid; j < S::kSums; j += kLoraThreads) {
             float s = 0.0f;
 #pragma unroll
             for (int w = 0; w < kLoraWarps; ++w) s += warps[w * S::kSums + j];
-            sums[j] = s;
+            for (int c = 0; c < C; ++c) (meets ? cl.map_shared_rank(sums, c) : sums)[part * S::kSums + j] = s;
         }
     }
-    cg::cluster_group cl = cg::this_cluster();
-    if (C > 1 && !p.s_in) cl.sync();
+
+    // ---- this warp's first 64 rows of B and its tokens' y are on their way while the blocks meet
+    constexpr int KP = RT >= 2 ? RT / 2 : 1;   // steps of 32 ranks (of 16 for RT = 1)
+    const int blocks = (p.n + 63) / 64, n1 = (int)((int64_t)blocks * (part + 1) / C);
+    int nb = p.s_out ? n1 : (int)((int64_t)blocks * part / C) + warp;
+    uint4 bw[4][2][KP];
+    float yv[NT][4][4];
+    auto request = [&]() {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = nb * 64 + h * 32 + g * 4 + j;
+                const uint16_t *b = p.b + ((int64_t)adapter * p.n + min(row, p.n - 1)) * p.r;
+                const int limit = row < p.n ? p.r : 0;
+                if (RT >= 2) {
+#pragma unroll
+                    for (int q = 0; q < KP; ++q) bw[j][h][q] = row8<VEC>(b, q * 32 + t4 * 8, limit);
+                } else if (VEC) {
+                    const uint2 v = t4 * 4 < limit ? __ldg(reinterpret_cast<const uint2 *>(b + t4 * 4)) : make_uint2(0, 0);
+                    bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
+                } else {
+                    bw[j][h][0] = row8<false>(b, t4 * 4, min(limit, t4 * 4 + 4));
+                }
+            }
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int tok = toks[q * 8 + t4 * 2 + (e & 1)];
+                if (tok >= 0) get4<VEC>(p, tok, nb * 64 + (e >> 1) * 32 + g * 4, yv[q][e]);
+            }
+    };
+    if (nb < n1) request();
+    if (meets) cl.sync();
     else __syncthreads();
 
     // ---- the whole S: the cluster's slices in order, in three bf16 parts of scale * S
@@ -326,10 +445,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
         float s = 0.0f;
         if (p.s_in) {
             if (tok >= 0 && rank < p.r) s = p.s_in[(int64_t)tok * p.r + rank];
-        } else if (C > 1) {
-            for (int c = 0; c < C; ++c) s += cl.map_shared_rank(sums, c)[j];
         } else {
-            s = sums[j];
+            for (int c = 0; c < C; ++c) s += sums[c * S::kSums + j];
         }
         if (p.s_out) {
             if (tok >= 0 && rank < p.r) p.s_out[(int64_t)tok * p.r + rank] = s;
@@ -342,65 +459,51 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
             s = after_bf16(s);
         }
     }
-    if (C > 1 && !p.s_in) cl.barrier_arrive();  // its slices are read; waited for at the end
     __syncthreads();
 
     // ---- out = y + B S over this block's N, 64 rows of B a warp: row h * 32 + g * 4 + j of them is row h * 8 + g of
     // product j, so that a lane ends with four consecutive outputs
-    if (!p.s_out) {
-        constexpr int KP = RT >= 2 ? RT / 2 : 1;   // steps of 32 ranks (of 16 for RT = 1)
-        const int blocks = (p.n + 63) / 64, n0 = (int)((int64_t)blocks * part / C), n1 = (int)((int64_t)blocks * (part + 1) / C);
-        for (int nb = n0 + warp; nb < n1; nb += kLoraWarps) {
-            uint4 bw[4][2][KP];
+    for (; nb < n1;) {
+        float acc[NT][4][4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int q = 0; q < NT; ++q)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = nb * 64 + h * 32 + g * 4 + j;
-                    const uint16_t *b = p.b + ((int64_t)adapter * p.n + min(row, p.n - 1)) * p.r;
-                    const int limit = row < p.n ? p.r : 0;
+            for (int w = 0; w < 3; ++w) {
+                const uint8_t *srow = split + (w * S::kTokens + q * 8 + g) * S::kRow;
+#pragma unroll
+                for (int kp = 0; kp < KP; ++kp) {
                     if (RT >= 2) {
+                        const uint4 s = *reinterpret_cast<const uint4 *>(srow + kp * 64 + t4 * 16);
 #pragma unroll
-                        for (int q = 0; q < KP; ++q) bw[j][h][q] = row8<VEC>(b, q * 32 + t4 * 8, limit);
-                    } else if (VEC) {
-                        const uint2 v = t4 * 4 < limit ? __ldg(reinterpret_cast<const uint2 *>(b + t4 * 4)) : make_uint2(0, 0);
-                        bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
-                    } else {
-                        bw[j][h][0] = row8<false>(b, t4 * 4, min(limit, t4 * 4 + 4));
-                    }
-                }
-#pragma unroll
-            for (int q = 0; q < NT; ++q) {
-                float acc[4][4] = {};
-#pragma unroll
-                for (int w = 0; w < 3; ++w) {
-                    const uint8_t *srow = split + (w * S::kTokens + q * 8 + g) * S::kRow;
-#pragma unroll
-                    for (int kp = 0; kp < KP; ++kp) {
-                        if (RT >= 2) {
-                            const uint4 s = *reinterpret_cast<const uint4 *>(srow + kp * 64 + t4 * 16);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                mma_bf16(acc[j], bw[j][0][kp].x, bw[j][1][kp].x, bw[j][0][kp].y, bw[j][1][kp].y, s.x, s.y);
-                                mma_bf16(acc[j], bw[j][0][kp].z, bw[j][1][kp].z, bw[j][0][kp].w, bw[j][1][kp].w, s.z, s.w);
-                            }
-                        } else {
-                            const uint2 s = *reinterpret_cast<const uint2 *>(srow + t4 * 8);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][0].x, bw[j][1][0].x, bw[j][0][0].y, bw[j][1][0].y, s.x, s.y);
+                        for (int j = 0; j < 4; ++j) {
+                            mma_bf16(acc[q][j], bw[j][0][kp].x, bw[j][1][kp].x, bw[j][0][kp].y, bw[j][1][kp].y, s.x, s.y);
+                            mma_bf16(acc[q][j], bw[j][0][kp].z, bw[j][1][kp].z, bw[j][0][kp].w, bw[j][1][kp].w, s.z, s.w);
                         }
-                    }
-                }
+                    } else {
+                        const uint2 s = *reinterpret_cast<const uint2 *>(srow + t4 * 8);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int tok = toks[q * 8 + t4 * 2 + (e & 1)];
-                    float d[4] = {acc[0][e], acc[1][e], acc[2][e], acc[3][e]};
-                    if (tok >= 0) add4<VEC>(p, tok, nb * 64 + (e >> 1) * 32 + g * 4, d);
+                        for (int j = 0; j < 4; ++j) mma_bf16(acc[q][j], bw[j][0][0].x, bw[j][1][0].x, bw[j][0][0].y, bw[j][1][0].y, s.x, s.y);
+                    }
                 }
             }
-        }
+        float sum[NT][4][4];
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[q][e][j] = yv[q][e][j] + acc[q][j][e];
+        const int at = nb * 64 + g * 4;
+        nb += kLoraWarps;
+        if (nb < n1) request();
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int tok = toks[q * 8 + t4 * 2 + (e & 1)];
+                if (tok >= 0) put4<VEC>(p, tok, at + (e >> 1) * 32, sum[q][e]);
+            }
     }
-    if (C > 1 && !p.s_in) cl.barrier_wait();
 }
 
 }  // namespace ws

@@ -133,9 +133,7 @@ ws_status_t launch_lora(const Err &err, bool xf32, bool vec, unsigned tiles, voi
 }
 template <int RT>
 ws_status_t launch_lora(const Err &err, int nt, bool xf32, bool vec, unsigned tiles, void *stream, const LoraParams &p) {
-    if (nt == 1) return launch_lora<RT, 1>(err, xf32, vec, tiles, stream, p);
-    if (nt == 2) return launch_lora<RT, 2>(err, xf32, vec, tiles, stream, p);
-    return launch_lora<RT, (RT < 8 ? 8 : 4)>(err, xf32, vec, tiles, stream, p);
+    return nt == 1 ? launch_lora<RT, 1>(err, xf32, vec, tiles, stream, p) : launch_lora<RT, 2>(err, xf32, vec, tiles, stream, p);
 }
 
 enum class Lora { kAdd, kShrink, kExpand };
@@ -175,9 +173,9 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
               aligned(a->b, a->rank, WS_ACT_BF16, 16);
     }
     const int rt = a->rank <= 16 ? 1 : a->rank <= 32 ? 2 : a->rank <= 64 ? 4 : 8;
-    const int nt = a->m <= 32 ? 1 : a->m <= kLoraDirect ? 2 : rt < 8 ? 8 : 4;
+    const int nt = a->m <= 32 ? 1 : 2;
     p.cluster = a->m <= 64 ? 8 : 4;
-    unsigned tiles = (unsigned)a->m;
+    unsigned tiles = (unsigned)std::min((int64_t)a->m, lora_max_tiles(a->m, a->adapters, nt * 8));
     if (a->m > kLoraDirect) {
         if (a->adapters > kLoraMaxAdapters) return err(WS_ERR_CAPACITY, "%d adapters: at most %d with more than %d tokens", a->adapters, kLoraMaxAdapters, kLoraDirect);
         if (!a->workspace || a->workspace_bytes < ws_lora_workspace(a->m, a->adapters) || reinterpret_cast<uintptr_t>(a->workspace) & 15)
@@ -209,7 +207,7 @@ extern "C" {
 
 int64_t ws_lora_workspace(int32_t m, int32_t adapters) {
     if (m <= kLoraDirect || adapters < 1) return 0;
-    return lora_perm_bytes(m) + lora_max_tiles(m, adapters, 32) * (int64_t)sizeof(LoraTile);
+    return lora_perm_bytes(m) + lora_max_tiles(m, adapters, 16) * (int64_t)sizeof(LoraTile);
 }
 ws_status_t ws_lora_add(const ws_lora_args_t *a, void *stream, char *err, size_t err_len) { return lora(Lora::kAdd, a, stream, err, err_len); }
 ws_status_t ws_lora_shrink(const ws_lora_args_t *a, void *stream, char *err, size_t err_len) { return lora(Lora::kShrink, a, stream, err, err_len); }
