@@ -131,9 +131,21 @@ __device__ __forceinline__ uint32_t cut_bf16x2(float &a, float &b) {
 
 // Eight consecutive values of a bf16 row from `i`, those from `limit` on as zeros.  VEC: `limit` is a multiple of 8 and
 // the row 16-byte aligned.
+// (Predicated loads: behind branches the compiler waits for one before it issues the next.)
+__device__ __forceinline__ uint4 load16_if(const void *p, bool ok) {
+    uint4 r = make_uint4(0, 0, 0, 0);
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w) : "l"(p), "r"((int)ok));
+    return r;
+}
+__device__ __forceinline__ uint2 load8_if(const void *p, bool ok) {
+    uint2 r = make_uint2(0, 0);
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}" : "+r"(r.x), "+r"(r.y) : "l"(p), "r"((int)ok));
+    return r;
+}
 template <bool VEC>
 __device__ __forceinline__ uint4 row8(const uint16_t *row, int i, int limit) {
-    if (VEC) return i < limit ? __ldg(reinterpret_cast<const uint4 *>(row + i)) : make_uint4(0, 0, 0, 0);
+    if (VEC) return load16_if(row + i, i < limit);
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -143,34 +155,43 @@ __device__ __forceinline__ uint4 row8(const uint16_t *row, int i, int limit) {
 template <bool VEC>
 __device__ __forceinline__ void row8(const float *row, int i, int limit, float (&v)[8]) {
     if (VEC) {
-        float4 a = make_float4(0, 0, 0, 0), b = a;
-        if (i < limit) {
-            a = __ldg(reinterpret_cast<const float4 *>(row + i));
-            b = __ldg(reinterpret_cast<const float4 *>(row + i) + 1);
-        }
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        const uint4 a = load16_if(row + i, i < limit), b = load16_if(row + i + 4, i < limit);
+        v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+        v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = i + j < limit ? __ldg(row + i + j) : 0.0f;
     }
 }
 
-// Four consecutive values of a token's y, and of its result.
+// Four consecutive values of a token's y as they are stored, as numbers, and of its result.  tok < 0: none.
 template <bool VEC>
-__device__ __forceinline__ void get4(const LoraParams &p, int64_t tok, int nn, float (&v)[4]) {
-    if (nn >= p.n) return;
-    if (VEC && p.y_dtype == WS_ACT_F32) {
-        const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.y) + tok * p.ldy + nn);
-        v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
-    } else if (VEC) {
-        const uint2 y = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p.y) + tok * p.ldy + nn);
-        v[0] = __uint_as_float(y.x << 16); v[1] = __uint_as_float(y.x & 0xFFFF0000u);
-        v[2] = __uint_as_float(y.y << 16); v[3] = __uint_as_float(y.y & 0xFFFF0000u);
-    } else {
+__device__ __forceinline__ uint4 get4(const LoraParams &p, int64_t tok, int nn) {
+    const bool f32 = p.y_dtype == WS_ACT_F32, ok = tok >= 0 && nn < p.n;
+    const int64_t at = ok ? tok * p.ldy + nn : 0;
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (VEC) {
+        // (y may be out: not a read-only load)
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+                     "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t@q ld.global.v2.b32 {%0, %1}, [%4];\n\t}"
+                     : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
+                     : "l"(static_cast<const char *>(p.y) + at * (f32 ? 4 : 2)), "r"((int)(ok && f32)), "r"((int)(ok && !f32)) : "memory");
+    } else if (ok) {
+        uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = nn + j < p.n ? load1(p.y, p.y_dtype, tok * p.ldy + nn + j) : 0.0f;
+        for (int j = 0; j < 4; ++j)
+            if (nn + j < p.n) v[j] = __float_as_uint(load1(p.y, p.y_dtype, at + j));
+        r = make_uint4(v[0], v[1], v[2], v[3]);
     }
+    return r;
+}
+template <bool VEC>
+__device__ __forceinline__ void numbers4(const LoraParams &p, const uint4 &r, float (&v)[4]) {
+    const bool bf16 = VEC && p.y_dtype != WS_ACT_F32;
+    v[0] = __uint_as_float(bf16 ? r.x << 16 : r.x);
+    v[1] = __uint_as_float(bf16 ? r.x & 0xFFFF0000u : r.y);
+    v[2] = __uint_as_float(bf16 ? r.y << 16 : r.z);
+    v[3] = __uint_as_float(bf16 ? r.y & 0xFFFF0000u : r.w);
 }
 template <bool VEC>
 __device__ __forceinline__ void put4(const LoraParams &p, int64_t tok, int nn, const float (&v)[4]) {
@@ -200,24 +221,24 @@ __device__ __forceinline__ void lora_none(const LoraParams &p, const int32_t *to
     }
     if (p.out == p.y && p.ldo == p.ldy) return;
     for (int i0 = threadIdx.x; i0 < items; i0 += 4 * kLoraThreads) {
-        float v[4][4];
+        uint4 v[4];
         int64_t tok[4];
         int at[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int i = i0 + u * kLoraThreads;
-            tok[u] = -1;
-            if (i >= items) break;
-            tok[u] = toks[i / (n1 - n0)];
-            at[u] = n0 + i % (n1 - n0);
-            if (VEC) get4<true>(p, tok[u], at[u] * 4, v[u]);
-            else v[u][0] = load1(p.y, p.y_dtype, tok[u] * p.ldy + at[u]);
+            tok[u] = i < items ? toks[i / (n1 - n0)] : -1;
+            at[u] = i < items ? n0 + i % (n1 - n0) : 0;
+            if (VEC) v[u] = get4<true>(p, tok[u], at[u] * 4);
+            else v[u].x = tok[u] >= 0 ? __float_as_uint(load1(p.y, p.y_dtype, tok[u] * p.ldy + at[u])) : 0u;
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (tok[u] < 0) break;
-            if (VEC) put4<true>(p, tok[u], at[u] * 4, v[u]);
-            else store1(p.out, p.y_dtype, tok[u] * p.ldo + at[u], v[u][0]);
+            if (tok[u] < 0) continue;
+            float f[4];
+            numbers4<VEC>(p, v[u], f);
+            if (VEC) put4<true>(p, tok[u], at[u] * 4, f);
+            else store1(p.out, p.y_dtype, tok[u] * p.ldo + at[u], f[0]);
         }
     }
 }
@@ -226,32 +247,44 @@ __device__ __forceinline__ void lora_none(const LoraParams &p, const int32_t *to
 // earlier tokens with its adapter is a multiple of the tile's size; tiles are numbered by their leaders' places, so the
 // blocks that have work come first.
 template <int TOKENS>
-__device__ __forceinline__ bool find_tile(const LoraParams &p, int tile, int32_t *toks, int &adapter) {
+__device__ __forceinline__ bool find_tile(const LoraParams &p, int tile, uint8_t *scratch, int32_t *toks, int &adapter) {
     constexpr int H = kLoraDirect / kLoraThreads;   // tokens a thread looks after
-    __shared__ __align__(16) int32_t ids[kLoraDirect];
-    __shared__ uint32_t leads[kLoraDirect / 32];
+    constexpr int kSlots = 2 * kLoraDirect, kChunks = kLoraDirect / 32;
+    int32_t *const slots = reinterpret_cast<int32_t *>(scratch);                                           // a hash table of the ids that occur
+    auto *const held = reinterpret_cast<uint8_t(*)[kSlots]>(scratch + kSlots * 4);                         // how many of 32 consecutive tokens have that id
+    __shared__ uint32_t leads[kChunks];
     __shared__ int32_t lead_id, lead_before;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int id[H], before[H];
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-        const int i = tid + h * kLoraThreads;
-        id[h] = i < p.m ? lora_id(p, i) : -2;
-        ids[i] = id[h];
-    }
+    for (int h = 0; h < H; ++h) id[h] = tid + h * kLoraThreads < p.m ? lora_id(p, tid + h * kLoraThreads) : -2;
     if (tid < TOKENS) toks[tid] = -1;
-    __syncthreads();
+    if (p.m > 32) {
+        for (int i = tid; i < kSlots / 4; i += kLoraThreads) reinterpret_cast<int4 *>(slots)[i] = make_int4(-3, -3, -3, -3);
+        for (int i = tid; i < kChunks * kSlots / 16; i += kLoraThreads) reinterpret_cast<uint4 *>(held)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    int slot[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-        const int i = tid + h * kLoraThreads;
-        before[h] = 0;
-        if (h * kLoraThreads >= p.m) break;
-        if (i < p.m)
-#pragma unroll 4
-            for (int j = 0; j < i; j += 4) {
-                const int4 o = *reinterpret_cast<const int4 *>(ids + j);
-                before[h] += (o.x == id[h]) + (o.y == id[h] && j + 1 < i) + (o.z == id[h] && j + 2 < i) + (o.w == id[h] && j + 3 < i);
+        const uint32_t alike = __match_any_sync(0xffffffffu, id[h]);
+        before[h] = __popc(alike & ((1u << lane) - 1));
+        if (p.m > 32 && h * kLoraThreads < p.m) {
+            slot[h] = (int)((uint32_t)id[h] * 2654435761u >> 16) % kSlots;
+            for (;;) {  // ends: there are twice as many slots as tokens
+                const int32_t o = atomicCAS(&slots[slot[h]], -3, id[h]);
+                if (o == -3 || o == id[h]) break;
+                slot[h] = (slot[h] + 1) % kSlots;
             }
+            if ((alike & ((1u << lane) - 1)) == 0) held[h * kLoraWarps + warp][slot[h]] = (uint8_t)__popc(alike);
+        }
+    }
+    if (p.m > 32) {
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            if (h * kLoraThreads < p.m)
+                for (int c = 0; c < h * kLoraWarps + warp; ++c) before[h] += held[c][slot[h]];
     }
 #pragma unroll
     for (int h = 0; h < H; ++h) {
@@ -286,16 +319,18 @@ struct LoraShape {
     // a token's ranks in bf16, padded so that a warp's fragment loads meet no bank twice
     static constexpr int kRow = kRanks * 2 + (RT >= 4 ? 64 : 0);
     static constexpr int kSplit = 3 * kTokens * kRow;
-    static constexpr int kScratch = kLoraWarps * kSums * 4 > kSplit ? kLoraWarps * kSums * 4 : kSplit;
+    static constexpr int kFind = kLoraDirect * 8 + kLoraDirect / 32 * kLoraDirect * 2;    // find_tile's tables
+    static constexpr int kWork = kLoraWarps * kSums * 4 > kSplit ? kLoraWarps * kSums * 4 : kSplit;
+    static constexpr int kScratch = kWork > kFind ? kWork : kFind;
     static constexpr int kSmem = kScratch + kLoraMaxCluster * kSums * 4;
     static constexpr int kAhead = RT * NT <= 2 ? 4 : RT * NT <= 8 ? 2 : 1;   // steps of K requested together
 };
 
 template <int RT, int NT, bool XF32, bool VEC>
-__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __launch_bounds__(kLoraThreads, RT == 1 ? 2 : 1) lora_kernel(const __grid_constant__ LoraParams p) {
     namespace cg = cooperative_groups;
     using S = LoraShape<RT, NT>;
-    extern __shared__ __align__(16) uint8_t lora_smem[];
+    extern __shared__ __align__(16) uint8_t lora_smem[];  // find_tile's tables, then the warps' sums, then the split S; the blocks' sums
     float *const warps = reinterpret_cast<float *>(lora_smem);                      // [warp][kSums], then the split S
     float *const sums = reinterpret_cast<float *>(lora_smem + S::kScratch);         // the S of the cluster's blocks, [block][kSums]
     __shared__ int32_t toks[S::kTokens];
@@ -314,7 +349,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
         const LoraTile q = p.tiles[tile];
         adapter = q.adapter;
         if (tid < S::kTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
-    } else if (!find_tile<S::kTokens>(p, tile, toks, adapter)) {
+    } else if (!find_tile<S::kTokens>(p, tile, lora_smem, toks, adapter)) {
         return;  // (the same on all threads of the cluster)
     }
     __syncthreads();
@@ -401,10 +436,16 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
 
     // ---- this warp's first 64 rows of B and its tokens' y are on their way while the blocks meet
     constexpr int KP = RT >= 2 ? RT / 2 : 1;   // steps of 32 ranks (of 16 for RT = 1)
-    const int blocks = (p.n + 63) / 64, n1 = (int)((int64_t)blocks * (part + 1) / C);
-    int nb = p.s_out ? n1 : (int)((int64_t)blocks * part / C) + warp;
+    const int blocks = (p.n + 63) / 64, nb1 = p.s_out ? 0 : (int)((int64_t)blocks * (part + 1) / C);
+    int nb = (int)((int64_t)blocks * part / C) + warp;
     uint4 bw[4][2][KP];
-    float yv[NT][4][4];
+    uint4 yv[NT][4];
+    int mytok[NT][2];                          // the tokens of this lane's results
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+        mytok[q][0] = toks[q * 8 + t4 * 2];
+        mytok[q][1] = toks[q * 8 + t4 * 2 + 1];
+    }
     auto request = [&]() {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -417,7 +458,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
 #pragma unroll
                     for (int q = 0; q < KP; ++q) bw[j][h][q] = row8<VEC>(b, q * 32 + t4 * 8, limit);
                 } else if (VEC) {
-                    const uint2 v = t4 * 4 < limit ? __ldg(reinterpret_cast<const uint2 *>(b + t4 * 4)) : make_uint2(0, 0);
+                    const uint2 v = load8_if(b + t4 * 4, t4 * 4 < limit);
                     bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
                 } else {
                     bw[j][h][0] = row8<false>(b, t4 * 4, min(limit, t4 * 4 + 4));
@@ -427,12 +468,12 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
         for (int q = 0; q < NT; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int tok = toks[q * 8 + t4 * 2 + (e & 1)];
-                if (tok >= 0) get4<VEC>(p, tok, nb * 64 + (e >> 1) * 32 + g * 4, yv[q][e]);
+                yv[q][e] = get4<VEC>(p, mytok[q][e & 1], nb * 64 + (e >> 1) * 32 + g * 4);
             }
     };
-    if (nb < n1) request();
-    if (meets) cl.sync();
+    if (meets) cl.barrier_arrive();  // (before the loads: it would wait for them)
+    if (nb < nb1) request();
+    if (meets) cl.barrier_wait();
     else __syncthreads();
 
     // ---- the whole S: the cluster's slices in order, in three bf16 parts of scale * S
@@ -463,7 +504,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
 
     // ---- out = y + B S over this block's N, 64 rows of B a warp: row h * 32 + g * 4 + j of them is row h * 8 + g of
     // product j, so that a lane ends with four consecutive outputs
-    for (; nb < n1;) {
+    while (nb < nb1) {
         float acc[NT][4][4] = {};
 #pragma unroll
         for (int q = 0; q < NT; ++q)
@@ -490,18 +531,19 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
 #pragma unroll
         for (int q = 0; q < NT; ++q)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 4; ++e) {
+                numbers4<VEC>(p, yv[q][e], sum[q][e]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum[q][e][j] = yv[q][e][j] + acc[q][j][e];
+                for (int j = 0; j < 4; ++j) sum[q][e][j] += acc[q][j][e];
+            }
         const int at = nb * 64 + g * 4;
         nb += kLoraWarps;
-        if (nb < n1) request();
+        if (nb < nb1) request();
 #pragma unroll
         for (int q = 0; q < NT; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int tok = toks[q * 8 + t4 * 2 + (e & 1)];
-                if (tok >= 0) put4<VEC>(p, tok, at + (e >> 1) * 32, sum[q][e]);
+                if (mytok[q][e & 1] >= 0) put4<VEC>(p, mytok[q][e & 1], at + (e >> 1) * 32, sum[q][e]);
             }
     }
 }

@@ -173,9 +173,10 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
               aligned(a->b, a->rank, WS_ACT_BF16, 16);
     }
     const int rt = a->rank <= 16 ? 1 : a->rank <= 32 ? 2 : a->rank <= 64 ? 4 : 8;
-    const int nt = a->m <= 32 ? 1 : 2;
-    p.cluster = a->m <= 64 ? 8 : 4;
+    const int nt = a->m <= 128 ? 1 : 2;
     unsigned tiles = (unsigned)std::min((int64_t)a->m, lora_max_tiles(a->m, a->adapters, nt * 8));
+    static const char *ec = getenv("LC");
+    p.cluster = ec ? atoi(ec) : tiles <= 148 ? 8 : 4;
     if (a->m > kLoraDirect) {
         if (a->adapters > kLoraMaxAdapters) return err(WS_ERR_CAPACITY, "%d adapters: at most %d with more than %d tokens", a->adapters, kLoraMaxAdapters, kLoraDirect);
         if (!a->workspace || a->workspace_bytes < ws_lora_workspace(a->m, a->adapters) || reinterpret_cast<uintptr_t>(a->workspace) & 15)
