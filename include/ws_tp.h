@@ -296,7 +296,7 @@ ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *args, void *stream
  * ws_lora_add is the whole; where the projection is sharded over K every rank calls ws_lora_shrink on its slice of x
  * and of a, the ranks add the shrunk rows up (ws_allreduce_f32) and each calls ws_lora_expand.
  * The adapters are bf16, the products' sums and the shrunk rows fp32.  Up to 512 tokens need no workspace; more take
- * ws_lora_workspace(m, adapters) bytes (16-byte aligned) that the call writes first, so calls on one stream may share
+ * ws_lora_workspace(m, adapters, rank) bytes (16-byte aligned) that the call writes first, so calls on one stream may share
  * it, and at most 16384 adapters (WS_ERR_CAPACITY beyond). */
 #define WS_LORA_MAX_RANK 128
 typedef struct {
@@ -315,7 +315,7 @@ typedef struct {
     int64_t workspace_bytes;
     int32_t m, k, n, rank, adapters, x_dtype, y_dtype, reserved;
 } ws_lora_args_t;
-int64_t ws_lora_workspace(int32_t m, int32_t adapters);
+int64_t ws_lora_workspace(int32_t m, int32_t adapters, int32_t rank);
 ws_status_t ws_lora_add(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
 ws_status_t ws_lora_shrink(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
 ws_status_t ws_lora_expand(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);

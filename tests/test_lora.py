@@ -320,7 +320,7 @@ def test_c_entry_refuses_a_short_workspace(dev):
              b=torch.zeros((2, 16, 8), dtype=BF16, device=dev), ids=torch.zeros(m, dtype=torch.int32, device=dev))
     a = ops._lora_args(**p)
     a.out, a.ldo = p["y"].data_ptr(), 16
-    need = L.ws_lora_workspace(m, 2)
+    need = L.ws_lora_workspace(m, 2, 8)
     work = torch.zeros(need + 16, dtype=torch.uint8, device=dev)
     for ptr, size in ((None, need), (work.data_ptr(), need - 1), (work.data_ptr() + 4, need)):
         a.workspace, a.workspace_bytes = ptr, size

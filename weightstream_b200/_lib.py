@@ -193,7 +193,7 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     L.ws_fp8_gemm_static_scratch_check.restype = st
     L.ws_fp8_gemm_static_scratch_check.argtypes = [C.c_int32, P, C.c_char_p, C.c_size_t]
     L.ws_lora_workspace.restype = C.c_int64
-    L.ws_lora_workspace.argtypes = [C.c_int32, C.c_int32]
+    L.ws_lora_workspace.argtypes = [C.c_int32, C.c_int32, C.c_int32]
     for name, args in (("ws_block_norm", BlockNormArgs), ("ws_token_logprobs", TokenLogprobsArgs), ("ws_lora_add", LoraArgs),
                        ("ws_lora_shrink", LoraArgs), ("ws_lora_expand", LoraArgs)):
         getattr(L, name).restype = st

@@ -210,8 +210,8 @@ __device__ __forceinline__ void put4(const LoraParams &p, int64_t tok, int nn, c
 // Tokens without an adapter: their y as it is, or zeros for shrunk rows.  A block's slice of all of them together, four
 // loads a thread under way.
 template <bool VEC>
-__device__ __forceinline__ void lora_none(const LoraParams &p, const int32_t *toks, int most, int part) {
-    const int n = p.s_out ? p.r : VEC ? p.n / 4 : p.n, n0 = (int)((int64_t)n * part / p.cluster), n1 = (int)((int64_t)n * (part + 1) / p.cluster);
+__device__ __forceinline__ void lora_none(const LoraParams &p, const int32_t *toks, int most, int part, int parts) {
+    const int n = p.s_out ? p.r : VEC ? p.n / 4 : p.n, n0 = (int)((int64_t)n * part / parts), n1 = (int)((int64_t)n * (part + 1) / parts);
     int count = 0;
     while (count < most && toks[count] >= 0) ++count;
     const int items = count * (n1 - n0);
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kLoraThreads, RT == 1 ? 2 : 1) lora_kernel(con
     }
     __syncthreads();
     if (adapter < 0) {  // nothing to add
-        lora_none<VEC>(p, toks, S::kTokens, part);
+        lora_none<VEC>(p, toks, S::kTokens, part, C);
         return;
     }
 
@@ -545,6 +545,251 @@ __global__ void __launch_bounds__(kLoraThreads, RT == 1 ? 2 : 1) lora_kernel(con
             for (int e = 0; e < 4; ++e) {
                 if (mytok[q][e & 1] >= 0) put4<VEC>(p, mytok[q][e & 1], at + (e >> 1) * 32, sum[q][e]);
             }
+    }
+}
+
+// ---------------------------------------------------------------- sorted batches
+// Prompts: tiles of 64 tokens of one adapter, the two products as two launches, each a stream over its large operand
+// (x; y and out), with the shrunk rows between them in the workspace.
+constexpr int kSortTokens = 64;
+constexpr int kSortK = 128;                   // values of K a stage holds
+
+template <int RT, bool XF32>
+struct ShrinkShape {
+    static constexpr int kX = kSortTokens * kSortK * (XF32 ? 4 : 2), kStage = kX + RT * 16 * kSortK * 2;
+    static constexpr int kStages = 110 * 1024 / kStage < 2 ? 2 : 110 * 1024 / kStage > 4 ? 4 : 110 * 1024 / kStage;
+    static constexpr int kSums = RT * 16 * kSortTokens;
+    static constexpr int kRing = kStages * kStage > kSums * 8 ? kStages * kStage : kSums * 8;   // at the end: half of the warps' sums
+    static constexpr int kSmem = kRing + kSums * 4;
+};
+
+__device__ __forceinline__ void lora_copy16(uint32_t dst, const void *src, bool ok) {  // zeros where not
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+// S = A x^T of a tile, K cut over the blocks of a cluster.  Eight warps: two halves of the tokens, four steps of 32 of a
+// stage's K.  Rows lie in shared memory as in global memory, 16-byte pieces swapped by the row's parity so that a
+// quarter of a warp, two rows of four pieces, reads all banks once.
+template <int RT, bool XF32>
+__global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+    namespace cg = cooperative_groups;
+    using S = ShrinkShape<RT, XF32>;
+    extern __shared__ __align__(128) uint8_t lora_smem[];
+    float *const got = reinterpret_cast<float *>(lora_smem + S::kRing);   // [block][kSums / C]: this block's share of all blocks' sums
+    __shared__ int32_t toks[kSortTokens];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3, kg = warp & 3, half = warp >> 2;
+    const int C = p.cluster, part = blockIdx.x % C, tile = blockIdx.x / C;
+    cg::cluster_group cl = cg::this_cluster();
+    if (C > 1) cl.barrier_arrive();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_predecessor();
+    if (tile >= *p.tiles_count) return;
+    const LoraTile q = p.tiles[tile];
+    if (tid < kSortTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
+    __syncthreads();
+    if (q.adapter < 0) {
+        lora_none<true>(p, toks, kSortTokens, part, C);
+        return;
+    }
+    // what this thread copies: one 16-byte column of every sixteenth row (of x in fp32: of every eighth)
+    constexpr int XP = XF32 ? 32 : 16, XR = kLoraThreads / XP, XN = kSortTokens / XR, xe = XF32 ? 4 : 8;
+    const char *xsrc[XN];
+    uint32_t xok = 0;
+    const int xc = tid % XP, ac = tid % 16;
+#pragma unroll
+    for (int i = 0; i < XN; ++i) {
+        const int tok = toks[tid / XP + i * XR];
+        xok |= (tok >= 0 ? 1u : 0u) << i;
+        xsrc[i] = static_cast<const char *>(p.x) + ((int64_t)max(tok, 0) * p.ldx + xc * xe) * (XF32 ? 4 : 2);
+    }
+    const uint16_t *const asrc = p.a + ((int64_t)q.adapter * p.r + tid / 16) * p.k + ac * 8;
+    const uint32_t ring = smem_u32(lora_smem);
+    const uint32_t xdst = ring + tid / XP * (kSortK * (XF32 ? 4 : 2)) + (XF32 ? xc ^ (tid / XP & 1) : xc ^ (tid / XP & 1) * 4) * 16;
+    const uint32_t adst = ring + S::kX + tid / 16 * (kSortK * 2) + (ac ^ (tid / 16 & 1) * 4) * 16;
+    const int steps = (p.k + kSortK - 1) / kSortK, s0 = (int)((int64_t)steps * part / C), s1 = (int)((int64_t)steps * (part + 1) / C);
+    auto request = [&](int st) {
+        if (st < s1) {
+            const int slot = (st - s0) % S::kStages * S::kStage, k0 = st * kSortK;
+#pragma unroll
+            for (int i = 0; i < XN; ++i)
+                lora_copy16(xdst + slot + i * XR * (kSortK * (XF32 ? 4 : 2)), xsrc[i] + (int64_t)k0 * (XF32 ? 4 : 2), (xok >> i & 1) && k0 + xc * xe < p.k);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                lora_copy16(adst + slot + i * 16 * (kSortK * 2), asrc + (int64_t)i * 16 * p.k + k0, tid / 16 + i * 16 < p.r && k0 + ac * 8 < p.k);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i + 1 < S::kStages; ++i) request(s0 + i);
+    float acc[RT][4][4] = {};
+    for (int st = s0; st < s1; ++st) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+        __syncthreads();  // the stage is there for all, and the one before it is read by all
+        request(st + S::kStages - 1);
+        const uint8_t *const xs = lora_smem + (st - s0) % S::kStages * S::kStage, *const as = xs + S::kX;
+        uint4 aw[RT][2];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                aw[i][h] = *reinterpret_cast<const uint4 *>(as + (i * 16 + h * 8 + g) * (kSortK * 2) + ((kg * 4 + t4) ^ (g & 1) * 4) * 16);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int row = half * 32 + n * 8 + g;
+            float f[8];
+            uint4 xv;
+            if (XF32) {
+                const uint8_t *r = xs + row * (kSortK * 4);
+                const float4 u = *reinterpret_cast<const float4 *>(r + ((kg * 8 + t4 * 2) ^ (g & 1)) * 16);
+                const float4 v = *reinterpret_cast<const float4 *>(r + ((kg * 8 + t4 * 2 + 1) ^ (g & 1)) * 16);
+                f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+                f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
+            } else {
+                xv = *reinterpret_cast<const uint4 *>(xs + row * (kSortK * 2) + ((kg * 4 + t4) ^ (g & 1) * 4) * 16);
+            }
+#pragma unroll
+            for (int w = 0; w < (XF32 ? 3 : 1); ++w) {
+                if (XF32) xv = make_uint4(cut_bf16x2(f[0], f[1]), cut_bf16x2(f[2], f[3]), cut_bf16x2(f[4], f[5]), cut_bf16x2(f[6], f[7]));
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    mma_bf16(acc[i][n], aw[i][0].x, aw[i][1].x, aw[i][0].y, aw[i][1].y, xv.x, xv.y);
+                    mma_bf16(acc[i][n], aw[i][0].z, aw[i][1].z, aw[i][0].w, aw[i][1].w, xv.z, xv.w);
+                }
+            }
+        }
+    }
+    // the four steps' sums: 2 and 3 to 0 and 1, then 1 to 0
+    float *const sums = reinterpret_cast<float *>(lora_smem);
+    constexpr int kMine = RT * 4 * 128;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int from = 2; from; from >>= 1) {
+        __syncthreads();
+        float *const at = sums + ((kg % from) * 2 + half) * kMine + lane;
+        if (kg >= from && kg < 2 * from)
+#pragma unroll
+            for (int j = 0; j < RT * 16; ++j) at[j * 32] = acc[j / 16][j / 4 % 4][j % 4];
+        __syncthreads();
+        if (kg < from)
+#pragma unroll
+            for (int j = 0; j < RT * 16; ++j) acc[j / 16][j / 4 % 4][j % 4] += at[j * 32];
+    }
+    // every block of the cluster adds one share of the sums up
+    const int share = S::kSums / C;
+    if (C > 1) cl.barrier_wait();
+    if (kg == 0)
+#pragma unroll
+        for (int j = 0; j < RT * 16; ++j) {
+            const int at = half * kMine + j * 32 + lane, c = at / share;
+            (C > 1 ? cl.map_shared_rank(got, c) : got)[part * share + at - c * share] = acc[j / 16][j / 4 % 4][j % 4];
+        }
+    if (C > 1) cl.sync();
+    else __syncthreads();
+    for (int j = tid; j < share; j += kLoraThreads) {
+        float s = 0.0f;
+        for (int c = 0; c < C; ++c) s += got[c * share + j];
+        const int at = part * share + j, l = at & 31, e = at >> 5 & 3, n = at >> 7 & 3, i = (at % kMine) >> 9, h = at / kMine;
+        const int rank = i * 16 + (l >> 2) + (e >> 1) * 8, tok = toks[h * 32 + n * 8 + (l & 3) * 2 + (e & 1)];
+        if (tok >= 0 && rank < p.r) p.s_out[(int64_t)tok * p.r + rank] = s;
+    }
+}
+
+template <int RT>
+struct ExpandShape {
+    static constexpr int kRow = LoraShape<RT, 1>::kRow, kSmem = 3 * kSortTokens * kRow;
+};
+constexpr int kExpandN = kLoraWarps * 64;     // rows of B a block takes at a time
+
+// out = y + B S of a tile and 512 rows of B, 64 a warp.  The y of eight tokens is requested two steps ahead.
+template <int RT>
+__global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+    using S = ExpandShape<RT>;
+    extern __shared__ __align__(128) uint8_t lora_smem[];
+    __shared__ int32_t toks[kSortTokens];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int slices = (p.n + kExpandN - 1) / kExpandN, slice = blockIdx.x % slices, tile = blockIdx.x / slices;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_predecessor();
+    if (tile >= *p.tiles_count) return;
+    const LoraTile q = p.tiles[tile];
+    if (tid < kSortTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
+    __syncthreads();
+    if (q.adapter < 0) {
+        lora_none<true>(p, toks, kSortTokens, slice, slices);
+        return;
+    }
+    constexpr int KP = RT >= 2 ? RT / 2 : 1;
+    const int n0 = slice * kExpandN + warp * 64;
+    uint4 bw[4][2][KP];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = n0 + h * 32 + g * 4 + j;
+            const uint16_t *b = p.b + ((int64_t)q.adapter * p.n + min(row, p.n - 1)) * p.r;
+            const int limit = row < p.n ? p.r : 0;
+            if (RT >= 2) {
+#pragma unroll
+                for (int k = 0; k < KP; ++k) bw[j][h][k] = row8<true>(b, k * 32 + t4 * 8, limit);
+            } else {
+                const uint2 v = load8_if(b + t4 * 4, t4 * 4 < limit);
+                bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
+            }
+        }
+    constexpr int kAhead = 2;
+    uint4 yv[kAhead][4];
+    auto token = [&](int u, int e) { return toks[u * 8 + t4 * 2 + (e & 1)]; };
+    auto request = [&](int u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) yv[u % kAhead][e] = get4<true>(p, token(u, e), n0 + (e >> 1) * 32 + g * 4);
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) request(u);
+    // scale * S in three bf16 parts
+    const float scale = p.scale ? p.scale[q.adapter] : 1.0f;
+    for (int j = tid; j < kSortTokens * RT * 16; j += kLoraThreads) {
+        const int place = j / (RT * 16), rank = j % (RT * 16), tok = toks[place];
+        float s = tok >= 0 && rank < p.r ? scale * p.s_in[(int64_t)tok * p.r + rank] : 0.0f;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+            *reinterpret_cast<uint16_t *>(lora_smem + (w * kSortTokens + place) * S::kRow + rank * 2) = (uint16_t)(__float_as_uint(s) >> 16);
+            s = after_bf16(s);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kSortTokens / 8; ++u) {
+        float acc[4][4] = {};
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+            const uint8_t *srow = lora_smem + (w * kSortTokens + u * 8 + g) * S::kRow;
+#pragma unroll
+            for (int k = 0; k < KP; ++k) {
+                if (RT >= 2) {
+                    const uint4 s = *reinterpret_cast<const uint4 *>(srow + k * 64 + t4 * 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        mma_bf16(acc[j], bw[j][0][k].x, bw[j][1][k].x, bw[j][0][k].y, bw[j][1][k].y, s.x, s.y);
+                        mma_bf16(acc[j], bw[j][0][k].z, bw[j][1][k].z, bw[j][0][k].w, bw[j][1][k].w, s.z, s.w);
+                    }
+                } else {
+                    const uint2 s = *reinterpret_cast<const uint2 *>(srow + t4 * 8);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][0].x, bw[j][1][0].x, bw[j][0][0].y, bw[j][1][0].y, s.x, s.y);
+                }
+            }
+        }
+        float sum[4][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            numbers4<true>(p, yv[u % kAhead][e], sum[e]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[e][j] += acc[j][e];
+        }
+        if (u + kAhead < kSortTokens / 8) request(u + kAhead);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (token(u, e) >= 0) put4<true>(p, token(u, e), n0 + (e >> 1) * 32 + g * 4, sum[e]);
     }
 }
 

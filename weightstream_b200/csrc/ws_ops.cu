@@ -136,6 +136,26 @@ ws_status_t launch_lora(const Err &err, int nt, bool xf32, bool vec, unsigned ti
     return nt == 1 ? launch_lora<RT, 1>(err, xf32, vec, tiles, stream, p) : launch_lora<RT, 2>(err, xf32, vec, tiles, stream, p);
 }
 
+template <int RT, bool XF32>
+ws_status_t launch_shrink(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
+    constexpr auto k = lora_shrink_kernel<RT, XF32>;
+    constexpr int smem = ShrinkShape<RT, XF32>::kSmem;
+    const ws_status_t st = allow_smem<k>(err, smem);
+    return st != WS_OK ? st : launch(err, k, dim3(tiles * (unsigned)p.cluster), kLoraThreads, smem, (unsigned)p.cluster, stream, p);
+}
+template <int RT>
+ws_status_t launch_shrink(const Err &err, bool xf32, unsigned tiles, void *stream, const LoraParams &p) {
+    return xf32 ? launch_shrink<RT, true>(err, tiles, stream, p) : launch_shrink<RT, false>(err, tiles, stream, p);
+}
+template <int RT>
+ws_status_t launch_expand(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
+    constexpr auto k = lora_expand_kernel<RT>;
+    constexpr int smem = ExpandShape<RT>::kSmem;
+    const ws_status_t st = allow_smem<k>(err, smem);
+    const unsigned slices = (unsigned)((p.n + kExpandN - 1) / kExpandN);
+    return st != WS_OK ? st : launch(err, k, dim3(tiles * slices), kLoraThreads, smem, 1, stream, p);
+}
+
 enum class Lora { kAdd, kShrink, kExpand };
 
 ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_text, size_t err_len) {
@@ -178,10 +198,11 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
     static const char *ec = getenv("LC");
     p.cluster = ec ? atoi(ec) : tiles <= 148 ? 8 : 4;
     if (a->m > kLoraDirect) {
+        const int64_t need = ws_lora_workspace(a->m, a->adapters, a->rank);
         if (a->adapters > kLoraMaxAdapters) return err(WS_ERR_CAPACITY, "%d adapters: at most %d with more than %d tokens", a->adapters, kLoraMaxAdapters, kLoraDirect);
-        if (!a->workspace || a->workspace_bytes < ws_lora_workspace(a->m, a->adapters) || reinterpret_cast<uintptr_t>(a->workspace) & 15)
-            return err(WS_ERR_INVALID, "%d tokens need a 16-byte aligned workspace of %lld bytes", a->m, (long long)ws_lora_workspace(a->m, a->adapters));
-        p.tile = nt * 8;
+        if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) & 15)
+            return err(WS_ERR_INVALID, "%d tokens need a 16-byte aligned workspace of %lld bytes", a->m, (long long)need);
+        p.tile = vec ? kSortTokens : nt * 8;
         p.tiles_count = static_cast<int32_t *>(a->workspace);
         p.perm = p.tiles_count + 4;
         p.tiles = reinterpret_cast<LoraTile *>(static_cast<char *>(a->workspace) + lora_perm_bytes(a->m));
@@ -191,8 +212,25 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
             const ws_status_t st = allow_smem<lora_plan_kernel>(err, (kLoraMaxAdapters + 1) * 12);
             if (st != WS_OK) return st;
         }
-        const ws_status_t st = launch(err, lora_plan_kernel, dim3(1), 1024, smem, 1, stream, p);
+        ws_status_t st = launch(err, lora_plan_kernel, dim3(1), 1024, smem, 1, stream, p);
         if (st != WS_OK) return st;
+        if (vec) {
+            if (shrinks) {
+                LoraParams q = p;
+                if (expands) q.s_out = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + need) - (int64_t)a->m * a->rank;
+                p.s_in = expands ? q.s_out : nullptr;
+                // K is cut until the blocks fill the card twice
+                q.cluster = 1;
+                while (q.cluster < 8 && (int64_t)tiles * q.cluster < 148 && a->k / (2 * q.cluster) >= 2 * kSortK) q.cluster *= 2;
+                if (ec) q.cluster = atoi(ec);
+                q.skip_none = 0;
+                st = rt == 1 ? launch_shrink<1>(err, xf32, tiles, stream, q) : rt == 2 ? launch_shrink<2>(err, xf32, tiles, stream, q)
+                     : rt == 4 ? launch_shrink<4>(err, xf32, tiles, stream, q) : launch_shrink<8>(err, xf32, tiles, stream, q);
+                if (st != WS_OK || !expands) return st;
+            }
+            return rt == 1 ? launch_expand<1>(err, tiles, stream, p) : rt == 2 ? launch_expand<2>(err, tiles, stream, p)
+                   : rt == 4 ? launch_expand<4>(err, tiles, stream, p) : launch_expand<8>(err, tiles, stream, p);
+        }
     }
     switch (rt) {
         case 1: return launch_lora<1>(err, nt, xf32, vec, tiles, stream, p);
@@ -206,9 +244,9 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
 
 extern "C" {
 
-int64_t ws_lora_workspace(int32_t m, int32_t adapters) {
-    if (m <= kLoraDirect || adapters < 1) return 0;
-    return lora_perm_bytes(m) + lora_max_tiles(m, adapters, 16) * (int64_t)sizeof(LoraTile);
+int64_t ws_lora_workspace(int32_t m, int32_t adapters, int32_t rank) {  // plan, then shrunk rows
+    if (m <= kLoraDirect || adapters < 1 || rank < 1) return 0;
+    return lora_perm_bytes(m) + lora_max_tiles(m, adapters, 16) * (int64_t)sizeof(LoraTile) + ((int64_t)m * rank * 4 + 15) / 16 * 16;
 }
 ws_status_t ws_lora_add(const ws_lora_args_t *a, void *stream, char *err, size_t err_len) { return lora(Lora::kAdd, a, stream, err, err_len); }
 ws_status_t ws_lora_shrink(const ws_lora_args_t *a, void *stream, char *err, size_t err_len) { return lora(Lora::kShrink, a, stream, err, err_len); }

@@ -477,7 +477,7 @@ PyObject *py_lora(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
         a.shrunk = made.data_ptr<float>();
     }
     at::Tensor work;
-    a.workspace_bytes = ws_lora_workspace(a.m, a.adapters);
+    a.workspace_bytes = ws_lora_workspace(a.m, a.adapters, a.rank);
     if (a.workspace_bytes > 0) {
         work = new_like(*ids, {a.workspace_bytes}, at::kByte);
         a.workspace = work.data_ptr();

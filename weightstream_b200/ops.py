@@ -221,7 +221,7 @@ def _lora_args(ids, *, x=None, a=None, y=None, b=None, scale=None, shrunk=None, 
 
 def _lora_call(name: str, args: LoraArgs, device) -> None:
     """On the current stream, whose memory the workspace is."""
-    size = _lib.load().ws_lora_workspace(args.m, args.adapters)
+    size = _lib.load().ws_lora_workspace(args.m, args.adapters, args.rank)
     work = torch.empty(size, dtype=torch.uint8, device=device)
     args.workspace, args.workspace_bytes = work.data_ptr(), size
     _call(name, args)
