@@ -65,9 +65,12 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
     for (int i = tid; i < buckets; i += 1024) count[i] = 0;
     wait_predecessor();
     __syncthreads();
-    for (int t = tid; t < p.m; t += 1024) {
-        const int id = lora_id(p, t);
-        atomicAdd(&count[id < 0 ? p.adapters : id], 1);
+    // (one atomic for all of a warp's tokens of an adapter: a prompt's tokens would queue for one word otherwise)
+    const int turns = (p.m + 1023) / 1024;
+    for (int i = 0; i < turns; ++i) {
+        const int t = tid + i * 1024, id = t < p.m ? lora_id(p, t) : -2, b = id < 0 ? p.adapters : id;
+        const uint32_t alike = __match_any_sync(0xffffffffu, id);
+        if (t < p.m && (alike & ((1u << lane) - 1)) == 0) atomicAdd(&count[b], __popc(alike));
     }
     __syncthreads();
     const int per = (buckets + 1023) / 1024, b0 = tid * per, b1 = min(buckets, b0 + per);
@@ -104,10 +107,13 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
         if (b < p.adapters || !p.skip_none) before_til += (c + p.tile - 1) / p.tile;
     }
     __syncthreads();
-    for (int t = tid; t < p.m; t += 1024) {
-        const int id = lora_id(p, t), b = id < 0 ? p.adapters : id;
-        if (b == p.adapters && p.skip_none) continue;
-        const int left = atomicSub(&count[b], 1);                      // c, c - 1, .. 1
+    for (int i = 0; i < turns; ++i) {
+        const int t = tid + i * 1024, id = t < p.m ? lora_id(p, t) : -2, b = id < 0 ? p.adapters : id;
+        const uint32_t alike = __match_any_sync(0xffffffffu, id);
+        int left = 0;
+        if (t < p.m && (alike & ((1u << lane) - 1)) == 0) left = atomicSub(&count[b], __popc(alike));   // the bucket's size, less each time
+        left = __shfl_sync(0xffffffffu, left, __ffs(alike) - 1) - __popc(alike & ((1u << lane) - 1));
+        if (t >= p.m || (b == p.adapters && p.skip_none)) continue;
         const int c = (b + 1 < buckets ? first[b + 1] : p.m) - first[b], at = c - left;
         p.perm[first[b] + at] = t;
         if (at % p.tile == 0) p.tiles[tile0[b] + at / p.tile] = LoraTile{id, first[b] + at, min(p.tile, c - at), 0};
@@ -700,96 +706,132 @@ struct ExpandShape {
 };
 constexpr int kExpandN = kLoraWarps * 64;     // rows of B a block takes at a time
 
-// out = y + B S of a tile and 512 rows of B, 64 a warp.  The y of eight tokens is requested two steps ahead.
-template <int RT>
+// out = y + B S of a tile and a slice of N, 64 rows of B a warp at a time.  The y of eight tokens is requested four steps
+// ahead of its sum.
+template <int RT, bool YF32>
 __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
     using S = ExpandShape<RT>;
+    constexpr int es = YF32 ? 4 : 2, kUnits = kSortTokens / 8, kAhead = RT <= 2 ? 2 : 4;
     extern __shared__ __align__(128) uint8_t lora_smem[];
     __shared__ int32_t toks[kSortTokens];
+    __shared__ int64_t yoff[kSortTokens], ooff[kSortTokens];    // bytes; -1: no token
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    const int slices = (p.n + kExpandN - 1) / kExpandN, slice = blockIdx.x % slices, tile = blockIdx.x / slices;
+    const int slices = p.cluster, slice = blockIdx.x % slices, tile = blockIdx.x / slices;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     wait_predecessor();
     if (tile >= *p.tiles_count) return;
     const LoraTile q = p.tiles[tile];
-    if (tid < kSortTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
+    if (tid < kSortTokens) {
+        const int tok = tid < q.count ? p.perm[q.start + tid] : -1;
+        toks[tid] = tok;
+        yoff[tid] = tok < 0 ? -1 : tok * p.ldy * es;
+        ooff[tid] = tok * p.ldo * es;
+    }
     __syncthreads();
     if (q.adapter < 0) {
         lora_none<true>(p, toks, kSortTokens, slice, slices);
         return;
     }
     constexpr int KP = RT >= 2 ? RT / 2 : 1;
-    const int n0 = slice * kExpandN + warp * 64;
+    const int rounds = (p.n + kExpandN - 1) / kExpandN, r0 = (int)((int64_t)rounds * slice / slices), r1 = (int)((int64_t)rounds * (slice + 1) / slices);
+    const uint16_t *const table = p.b + (int64_t)q.adapter * p.n * p.r;
     uint4 bw[4][2][KP];
+    auto weights = [&](int n0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = n0 + h * 32 + g * 4 + j;
-            const uint16_t *b = p.b + ((int64_t)q.adapter * p.n + min(row, p.n - 1)) * p.r;
-            const int limit = row < p.n ? p.r : 0;
-            if (RT >= 2) {
-#pragma unroll
-                for (int k = 0; k < KP; ++k) bw[j][h][k] = row8<true>(b, k * 32 + t4 * 8, limit);
-            } else {
-                const uint2 v = load8_if(b + t4 * 4, t4 * 4 < limit);
-                bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
-            }
-        }
-    constexpr int kAhead = 2;
-    uint4 yv[kAhead][4];
-    auto token = [&](int u, int e) { return toks[u * 8 + t4 * 2 + (e & 1)]; };
-    auto request = [&](int u) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) yv[u % kAhead][e] = get4<true>(p, token(u, e), n0 + (e >> 1) * 32 + g * 4);
-    };
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) request(u);
-    // scale * S in three bf16 parts
-    const float scale = p.scale ? p.scale[q.adapter] : 1.0f;
-    for (int j = tid; j < kSortTokens * RT * 16; j += kLoraThreads) {
-        const int place = j / (RT * 16), rank = j % (RT * 16), tok = toks[place];
-        float s = tok >= 0 && rank < p.r ? scale * p.s_in[(int64_t)tok * p.r + rank] : 0.0f;
-#pragma unroll
-        for (int w = 0; w < 3; ++w) {
-            *reinterpret_cast<uint16_t *>(lora_smem + (w * kSortTokens + place) * S::kRow + rank * 2) = (uint16_t)(__float_as_uint(s) >> 16);
-            s = after_bf16(s);
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kSortTokens / 8; ++u) {
-        float acc[4][4] = {};
-#pragma unroll
-        for (int w = 0; w < 3; ++w) {
-            const uint8_t *srow = lora_smem + (w * kSortTokens + u * 8 + g) * S::kRow;
-#pragma unroll
-            for (int k = 0; k < KP; ++k) {
+            for (int h = 0; h < 2; ++h) {
+                const int row = n0 + h * 32 + g * 4 + j;
+                const uint16_t *b = table + (int64_t)min(row, p.n - 1) * p.r;
+                const int limit = row < p.n ? p.r : 0;
                 if (RT >= 2) {
-                    const uint4 s = *reinterpret_cast<const uint4 *>(srow + k * 64 + t4 * 16);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        mma_bf16(acc[j], bw[j][0][k].x, bw[j][1][k].x, bw[j][0][k].y, bw[j][1][k].y, s.x, s.y);
-                        mma_bf16(acc[j], bw[j][0][k].z, bw[j][1][k].z, bw[j][0][k].w, bw[j][1][k].w, s.z, s.w);
-                    }
+                    for (int k = 0; k < KP; ++k) bw[j][h][k] = row8<true>(b, k * 32 + t4 * 8, limit);
                 } else {
-                    const uint2 s = *reinterpret_cast<const uint2 *>(srow + t4 * 8);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][0].x, bw[j][1][0].x, bw[j][0][0].y, bw[j][1][0].y, s.x, s.y);
+                    const uint2 v = load8_if(b + t4 * 4, t4 * 4 < limit);
+                    bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
                 }
             }
-        }
-        float sum[4][4];
+    };
+    uint4 yv[kAhead][4];
+    auto request = [&](int u, int n0) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            numbers4<true>(p, yv[u % kAhead][e], sum[e]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sum[e][j] += acc[j][e];
+            const int nn = n0 + (e >> 1) * 32 + g * 4;
+            const int64_t off = yoff[u * 8 + t4 * 2 + (e & 1)];
+            const char *src = static_cast<const char *>(p.y) + off + (int64_t)nn * es;
+            uint4 &r = yv[u % kAhead][e];
+            const int ok = off >= 0 && nn < p.n;
+            r = make_uint4(0, 0, 0, 0);
+            // (y may be out: not a read-only load)
+            if (YF32)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+                             : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w) : "l"(src), "r"(ok) : "memory");
+            else
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p ld.global.v2.b32 {%0, %1}, [%2];\n\t}"
+                             : "+r"(r.x), "+r"(r.y) : "l"(src), "r"(ok) : "memory");
         }
-        if (u + kAhead < kSortTokens / 8) request(u + kAhead);
+    };
+    weights(r0 * kExpandN + warp * 64);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (token(u, e) >= 0) put4<true>(p, token(u, e), n0 + (e >> 1) * 32 + g * 4, sum[e]);
+    for (int u = 0; u < kAhead; ++u) request(u, r0 * kExpandN + warp * 64);
+    // scale * S in three bf16 parts
+    const float scale = p.scale ? p.scale[q.adapter] : 1.0f;
+    for (int j = tid; j < kSortTokens * RT * 8; j += kLoraThreads) {
+        const int place = j / (RT * 8), rank = j % (RT * 8) * 2, tok = toks[place];
+        float2 s = make_float2(0.0f, 0.0f);
+        if (tok >= 0 && rank < p.r) s = *reinterpret_cast<const float2 *>(p.s_in + (int64_t)tok * p.r + rank);   // (r is even)
+        s.x *= scale;
+        s.y *= scale;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) *reinterpret_cast<uint32_t *>(lora_smem + (w * kSortTokens + place) * S::kRow + rank * 2) = cut_bf16x2(s.x, s.y);
+    }
+    __syncthreads();
+    for (int r = r0; r < r1; ++r) {
+        const int n0 = r * kExpandN + warp * 64;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            float acc[4][4] = {};
+#pragma unroll
+            for (int w = 0; w < 3; ++w) {
+                const uint8_t *srow = lora_smem + (w * kSortTokens + u * 8 + g) * S::kRow;
+#pragma unroll
+                for (int k = 0; k < KP; ++k) {
+                    if (RT >= 2) {
+                        const uint4 s = *reinterpret_cast<const uint4 *>(srow + k * 64 + t4 * 16);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][k].x, bw[j][1][k].x, bw[j][0][k].y, bw[j][1][k].y, s.x, s.y);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][k].z, bw[j][1][k].z, bw[j][0][k].w, bw[j][1][k].w, s.z, s.w);
+                    } else {
+                        const uint2 s = *reinterpret_cast<const uint2 *>(srow + t4 * 8);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][0].x, bw[j][1][0].x, bw[j][0][0].y, bw[j][1][0].y, s.x, s.y);
+                    }
+                }
+            }
+            // the next rows of B while the last sums of these are stored
+            if (u == kUnits - 1 && r + 1 < r1) weights(n0 + kExpandN);
+            float sum[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint4 &y = yv[u % kAhead][e];
+                sum[e][0] = __uint_as_float(YF32 ? y.x : y.x << 16) + acc[0][e];
+                sum[e][1] = __uint_as_float(YF32 ? y.y : y.x & 0xFFFF0000u) + acc[1][e];
+                sum[e][2] = __uint_as_float(YF32 ? y.z : y.y << 16) + acc[2][e];
+                sum[e][3] = __uint_as_float(YF32 ? y.w : y.y & 0xFFFF0000u) + acc[3][e];
+            }
+            if (u + kAhead < kUnits) request(u + kAhead, n0);
+            else if (r + 1 < r1) request(u + kAhead - kUnits, n0 + kExpandN);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int place = u * 8 + t4 * 2 + (e & 1), nn = n0 + (e >> 1) * 32 + g * 4;
+                if (yoff[place] < 0 || nn >= p.n) continue;
+                char *const dst = static_cast<char *>(p.out) + ooff[place] + (int64_t)nn * es;
+                if (YF32) *reinterpret_cast<float4 *>(dst) = make_float4(sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
+                else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(sum[e][0], sum[e][1]), pack_bf16x2(sum[e][2], sum[e][3]));
+            }
+        }
     }
 }
 

@@ -147,13 +147,16 @@ template <int RT>
 ws_status_t launch_shrink(const Err &err, bool xf32, unsigned tiles, void *stream, const LoraParams &p) {
     return xf32 ? launch_shrink<RT, true>(err, tiles, stream, p) : launch_shrink<RT, false>(err, tiles, stream, p);
 }
-template <int RT>
+template <int RT, bool YF32>
 ws_status_t launch_expand(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
-    constexpr auto k = lora_expand_kernel<RT>;
+    constexpr auto k = lora_expand_kernel<RT, YF32>;
     constexpr int smem = ExpandShape<RT>::kSmem;
     const ws_status_t st = allow_smem<k>(err, smem);
-    const unsigned slices = (unsigned)((p.n + kExpandN - 1) / kExpandN);
-    return st != WS_OK ? st : launch(err, k, dim3(tiles * slices), kLoraThreads, smem, 1, stream, p);
+    return st != WS_OK ? st : launch(err, k, dim3(tiles * (unsigned)p.cluster), kLoraThreads, smem, 1, stream, p);
+}
+template <int RT>
+ws_status_t launch_expand(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
+    return p.y_dtype == WS_ACT_F32 ? launch_expand<RT, true>(err, tiles, stream, p) : launch_expand<RT, false>(err, tiles, stream, p);
 }
 
 enum class Lora { kAdd, kShrink, kExpand };
@@ -228,6 +231,10 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
                      : rt == 4 ? launch_shrink<4>(err, xf32, tiles, stream, q) : launch_shrink<8>(err, xf32, tiles, stream, q);
                 if (st != WS_OK || !expands) return st;
             }
+            // N is cut into as many slices as fill the card once with the tiles that there may well be: one block an SM from
+            // rank 33, two below (rank 64: 113 us with 148 blocks, 122 with 296; rank 16 70 and 48)
+            const int likely = (a->m + kSortTokens - 1) / kSortTokens + std::min(a->adapters, a->m / kSortTokens) / 2;
+            p.cluster = std::max(1, std::min((a->n + kExpandN - 1) / kExpandN, (rt >= 4 ? 148 : 296) / likely));
             return rt == 1 ? launch_expand<1>(err, tiles, stream, p) : rt == 2 ? launch_expand<2>(err, tiles, stream, p)
                    : rt == 4 ? launch_expand<4>(err, tiles, stream, p) : launch_expand<8>(err, tiles, stream, p);
         }
