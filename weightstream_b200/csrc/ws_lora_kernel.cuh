@@ -213,38 +213,32 @@ __device__ __forceinline__ void put4(const LoraParams &p, int64_t tok, int nn, c
     }
 }
 
-// Tokens without an adapter: their y as it is, or zeros for shrunk rows.  A block's slice of all of them together, four
-// loads a thread under way.
+// Tokens without an adapter: their y as it is, or zeros for shrunk rows.  A block's slice of all of them, a warp a token.
 template <bool VEC>
 __device__ __forceinline__ void lora_none(const LoraParams &p, const int32_t *toks, int most, int part, int parts) {
     const int n = p.s_out ? p.r : VEC ? p.n / 4 : p.n, n0 = (int)((int64_t)n * part / parts), n1 = (int)((int64_t)n * (part + 1) / parts);
-    int count = 0;
-    while (count < most && toks[count] >= 0) ++count;
-    const int items = count * (n1 - n0);
-    if (p.s_out) {
-        for (int i = threadIdx.x; i < items; i += kLoraThreads) p.s_out[(int64_t)toks[i / (n1 - n0)] * p.r + n0 + i % (n1 - n0)] = 0.0f;
-        return;
-    }
-    if (p.out == p.y && p.ldo == p.ldy) return;
-    for (int i0 = threadIdx.x; i0 < items; i0 += 4 * kLoraThreads) {
-        uint4 v[4];
-        int64_t tok[4];
-        int at[4];
+    if (!p.s_out && p.out == p.y && p.ldo == p.ldy) return;
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < most; i += kLoraWarps) {  // a warp a token
+        const int64_t tok = toks[i];
+        if (tok < 0) break;
+        if (p.s_out) {
+            for (int j = n0 + lane; j < n1; j += 32) p.s_out[tok * p.r + j] = 0.0f;
+        } else if (VEC) {
+            for (int j0 = n0 + lane; j0 < n1; j0 += 8 * 32) {
+                uint4 v[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * kLoraThreads;
-            tok[u] = i < items ? toks[i / (n1 - n0)] : -1;
-            at[u] = i < items ? n0 + i % (n1 - n0) : 0;
-            if (VEC) v[u] = get4<true>(p, tok[u], at[u] * 4);
-            else v[u].x = tok[u] >= 0 ? __float_as_uint(load1(p.y, p.y_dtype, tok[u] * p.ldy + at[u])) : 0u;
-        }
+                for (int u = 0; u < 8; ++u) v[u] = get4<true>(p, j0 + u * 32 < n1 ? tok : -1, (j0 + u * 32) * 4);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (tok[u] < 0) continue;
-            float f[4];
-            numbers4<VEC>(p, v[u], f);
-            if (VEC) put4<true>(p, tok[u], at[u] * 4, f);
-            else store1(p.out, p.y_dtype, tok[u] * p.ldo + at[u], f[0]);
+                for (int u = 0; u < 8; ++u) {
+                    if (j0 + u * 32 >= n1) break;
+                    float f[4];
+                    numbers4<VEC>(p, v[u], f);
+                    put4<true>(p, tok, (j0 + u * 32) * 4, f);
+                }
+            }
+        } else {
+            for (int j = n0 + lane; j < n1; j += 32) store1(p.out, p.y_dtype, tok * p.ldo + j, load1(p.y, p.y_dtype, tok * p.ldy + j));
         }
     }
 }
@@ -597,32 +591,43 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_ker
         lora_none<true>(p, toks, kSortTokens, part, C);
         return;
     }
-    // what this thread copies: one 16-byte column of every sixteenth row (of x in fp32: of every eighth)
+    // What this thread copies: one 16-byte column of every sixteenth row (of x in fp32: of every eighth).  Places without a
+    // token and ranks behind the last one read the first's; nothing of them is stored.
     constexpr int XP = XF32 ? 32 : 16, XR = kLoraThreads / XP, XN = kSortTokens / XR, xe = XF32 ? 4 : 8;
-    const char *xsrc[XN];
-    uint32_t xok = 0;
+    const int steps = (p.k + kSortK - 1) / kSortK, s0 = (int)((int64_t)steps * part / C), s1 = (int)((int64_t)steps * (part + 1) / C);
     const int xc = tid % XP, ac = tid % 16;
+    const char *xsrc[XN], *asrc[RT];
 #pragma unroll
     for (int i = 0; i < XN; ++i) {
         const int tok = toks[tid / XP + i * XR];
-        xok |= (tok >= 0 ? 1u : 0u) << i;
-        xsrc[i] = static_cast<const char *>(p.x) + ((int64_t)max(tok, 0) * p.ldx + xc * xe) * (XF32 ? 4 : 2);
+        xsrc[i] = static_cast<const char *>(p.x) + ((tok < 0 ? toks[0] : tok) * p.ldx + (int64_t)s0 * kSortK + xc * xe) * (XF32 ? 4 : 2);
     }
-    const uint16_t *const asrc = p.a + ((int64_t)q.adapter * p.r + tid / 16) * p.k + ac * 8;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int rank = tid / 16 + i * 16;
+        asrc[i] = reinterpret_cast<const char *>(p.a + ((int64_t)q.adapter * p.r + (rank < p.r ? rank : 0)) * p.k + s0 * kSortK + ac * 8);
+    }
     const uint32_t ring = smem_u32(lora_smem);
     const uint32_t xdst = ring + tid / XP * (kSortK * (XF32 ? 4 : 2)) + (XF32 ? xc ^ (tid / XP & 1) : xc ^ (tid / XP & 1) * 4) * 16;
     const uint32_t adst = ring + S::kX + tid / 16 * (kSortK * 2) + (ac ^ (tid / 16 & 1) * 4) * 16;
-    const int steps = (p.k + kSortK - 1) / kSortK, s0 = (int)((int64_t)steps * part / C), s1 = (int)((int64_t)steps * (part + 1) / C);
+    int slot_in = 0, slot_out = 0;
     auto request = [&](int st) {
         if (st < s1) {
-            const int slot = (st - s0) % S::kStages * S::kStage, k0 = st * kSortK;
+            const bool whole = (st + 1) * kSortK <= p.k;
+            const bool xin = whole || st * kSortK + xc * xe < p.k, ain = whole || st * kSortK + ac * 8 < p.k;
+            const uint32_t at = slot_in * S::kStage;
 #pragma unroll
-            for (int i = 0; i < XN; ++i)
-                lora_copy16(xdst + slot + i * XR * (kSortK * (XF32 ? 4 : 2)), xsrc[i] + (int64_t)k0 * (XF32 ? 4 : 2), (xok >> i & 1) && k0 + xc * xe < p.k);
+            for (int i = 0; i < XN; ++i) {
+                lora_copy16(xdst + at + i * XR * (kSortK * (XF32 ? 4 : 2)), xsrc[i], xin);
+                xsrc[i] += kSortK * (XF32 ? 4 : 2);
+            }
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
-                lora_copy16(adst + slot + i * 16 * (kSortK * 2), asrc + (int64_t)i * 16 * p.k + k0, tid / 16 + i * 16 < p.r && k0 + ac * 8 < p.k);
+            for (int i = 0; i < RT; ++i) {
+                lora_copy16(adst + at + i * 16 * (kSortK * 2), asrc[i], ain);
+                asrc[i] += kSortK * 2;
+            }
         }
+        slot_in = slot_in + 1 == S::kStages ? 0 : slot_in + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
@@ -632,7 +637,8 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_ker
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
         __syncthreads();  // the stage is there for all, and the one before it is read by all
         request(st + S::kStages - 1);
-        const uint8_t *const xs = lora_smem + (st - s0) % S::kStages * S::kStage, *const as = xs + S::kX;
+        const uint8_t *const xs = lora_smem + slot_out * S::kStage, *const as = xs + S::kX;
+        slot_out = slot_out + 1 == S::kStages ? 0 : slot_out + 1;
         uint4 aw[RT][2];
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -714,7 +720,7 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
     constexpr int es = YF32 ? 4 : 2, kUnits = kSortTokens / 8, kAhead = RT <= 2 ? 2 : 4;
     extern __shared__ __align__(128) uint8_t lora_smem[];
     __shared__ int32_t toks[kSortTokens];
-    __shared__ int64_t yoff[kSortTokens], ooff[kSortTokens];    // bytes; -1: no token
+    __shared__ int64_t yoff[kSortTokens], ooff[kSortTokens];    // bytes; places without a token read the first one's
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int slices = p.cluster, slice = blockIdx.x % slices, tile = blockIdx.x / slices;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -722,9 +728,9 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
     if (tile >= *p.tiles_count) return;
     const LoraTile q = p.tiles[tile];
     if (tid < kSortTokens) {
-        const int tok = tid < q.count ? p.perm[q.start + tid] : -1;
-        toks[tid] = tok;
-        yoff[tid] = tok < 0 ? -1 : tok * p.ldy * es;
+        const int tok = p.perm[q.start + (tid < q.count ? tid : 0)];
+        toks[tid] = tid < q.count ? tok : -1;
+        yoff[tid] = tok * p.ldy * es;
         ooff[tid] = tok * p.ldo * es;
     }
     __syncthreads();
@@ -754,22 +760,17 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
             }
     };
     uint4 yv[kAhead][4];
-    auto request = [&](int u, int n0) {
+    const char *const ybase = static_cast<const char *>(p.y);
+    char *const obase = static_cast<char *>(p.out);
+    auto request = [&](int u, int n0) {  // (rows behind the last one's read that; nothing of them is stored)
+        const int at[2] = {min(n0 + g * 4, p.n - 4) * es, min(n0 + 32 + g * 4, p.n - 4) * es};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int nn = n0 + (e >> 1) * 32 + g * 4;
-            const int64_t off = yoff[u * 8 + t4 * 2 + (e & 1)];
-            const char *src = static_cast<const char *>(p.y) + off + (int64_t)nn * es;
+            const char *src = ybase + yoff[u * 8 + t4 * 2 + (e & 1)] + at[e >> 1];
             uint4 &r = yv[u % kAhead][e];
-            const int ok = off >= 0 && nn < p.n;
-            r = make_uint4(0, 0, 0, 0);
             // (y may be out: not a read-only load)
-            if (YF32)
-                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-                             : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w) : "l"(src), "r"(ok) : "memory");
-            else
-                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p ld.global.v2.b32 {%0, %1}, [%2];\n\t}"
-                             : "+r"(r.x), "+r"(r.y) : "l"(src), "r"(ok) : "memory");
+            if (YF32) asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(src) : "memory");
+            else asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(src) : "memory");
         }
     };
     weights(r0 * kExpandN + warp * 64);
@@ -826,8 +827,8 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int place = u * 8 + t4 * 2 + (e & 1), nn = n0 + (e >> 1) * 32 + g * 4;
-                if (yoff[place] < 0 || nn >= p.n) continue;
-                char *const dst = static_cast<char *>(p.out) + ooff[place] + (int64_t)nn * es;
+                if (place >= q.count || nn >= p.n) continue;
+                char *const dst = obase + ooff[place] + (int64_t)nn * es;
                 if (YF32) *reinterpret_cast<float4 *>(dst) = make_float4(sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
                 else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(sum[e][0], sum[e][1]), pack_bf16x2(sum[e][2], sum[e][3]));
             }

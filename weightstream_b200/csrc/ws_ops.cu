@@ -231,10 +231,18 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
                      : rt == 4 ? launch_shrink<4>(err, xf32, tiles, stream, q) : launch_shrink<8>(err, xf32, tiles, stream, q);
                 if (st != WS_OK || !expands) return st;
             }
-            // N is cut into as many slices as fill the card once with the tiles that there may well be: one block an SM from
-            // rank 33, two below (rank 64: 113 us with 148 blocks, 122 with 296; rank 16 70 and 48)
-            const int likely = (a->m + kSortTokens - 1) / kSortTokens + std::min(a->adapters, a->m / kSortTokens) / 2;
-            p.cluster = std::max(1, std::min((a->n + kExpandN - 1) / kExpandN, (rt >= 4 ? 148 : 296) / likely));
+            // N is cut so that the slices' blocks, one an SM from rank 33 and two below, end together with the tiles that there
+            // may well be (rank 64, 4000 rows: 113 us with 2 slices, 122 with 4; rank 16, 2000 rows: 70 us with 4, 48 with 8)
+            const int64_t likely = (a->m + kSortTokens - 1) / kSortTokens + std::min(a->adapters, a->m / kSortTokens) / 2, at_once = rt >= 4 ? 148 : 296;
+            const int rounds = (a->n + kExpandN - 1) / kExpandN;
+            int64_t least = INT64_MAX;
+            for (int c = 1; c <= rounds && c <= 32; ++c) {  // (a block's beginning costs about one round)
+                const int64_t cost = (likely * c + at_once - 1) / at_once * ((rounds + c - 1) / c + 1);
+                if (cost < least) {
+                    least = cost;
+                    p.cluster = c;
+                }
+            }
             return rt == 1 ? launch_expand<1>(err, tiles, stream, p) : rt == 2 ? launch_expand<2>(err, tiles, stream, p)
                    : rt == 4 ? launch_expand<4>(err, tiles, stream, p) : launch_expand<8>(err, tiles, stream, p);
         }
