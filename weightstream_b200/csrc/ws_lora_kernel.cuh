@@ -568,8 +568,8 @@ __device__ __forceinline__ void lora_copy16(uint32_t dst, const void *src, bool 
 }
 
 // S = A x^T of a tile, K cut over the blocks of a cluster.  Eight warps: two halves of the tokens, four steps of 32 of a
-// stage's K.  Rows lie in shared memory as in global memory, 16-byte pieces swapped by the row's parity so that a
-// quarter of a warp, two rows of four pieces, reads all banks once.
+// stage's K.  Rows lie in shared memory as in global memory, their 16-byte pieces swapped by the row's last three bits so
+// that the eight rows of a matrix lie in different banks.
 template <int RT, bool XF32>
 __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
     namespace cg = cooperative_groups;
@@ -608,8 +608,9 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_ker
         asrc[i] = reinterpret_cast<const char *>(p.a + ((int64_t)q.adapter * p.r + (rank < p.r ? rank : 0)) * p.k + s0 * kSortK + ac * 8);
     }
     const uint32_t ring = smem_u32(lora_smem);
-    const uint32_t xdst = ring + tid / XP * (kSortK * (XF32 ? 4 : 2)) + (XF32 ? xc ^ (tid / XP & 1) : xc ^ (tid / XP & 1) * 4) * 16;
-    const uint32_t adst = ring + S::kX + tid / 16 * (kSortK * 2) + (ac ^ (tid / 16 & 1) * 4) * 16;
+    // (a thread's rows are a multiple of eight apart: one swap for all)
+    const uint32_t xdst = ring + tid / XP * (kSortK * (XF32 ? 4 : 2)) + (xc ^ (tid / XP & 7)) * 16;
+    const uint32_t adst = ring + S::kX + tid / 16 * (kSortK * 2) + (ac ^ (tid / 16 & 7)) * 16;
     int slot_in = 0, slot_out = 0;
     auto request = [&](int st) {
         if (st < s1) {
@@ -640,32 +641,31 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_ker
         const uint8_t *const xs = lora_smem + slot_out * S::kStage, *const as = xs + S::kX;
         slot_out = slot_out + 1 == S::kStages ? 0 : slot_out + 1;
         uint4 aw[RT][2];
+        const uint32_t xa = smem_u32(xs), aa = smem_u32(as);
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                aw[i][h] = *reinterpret_cast<const uint4 *>(as + (i * 16 + h * 8 + g) * (kSortK * 2) + ((kg * 4 + t4) ^ (g & 1) * 4) * 16);
+            for (int h = 0; h < 2; ++h)  // ranks 0-7, 8-15 of K 0-7, then of K 8-15
+                ldmatrix_x4(aa + (i * 16 + (lane & 15)) * (kSortK * 2) + ((kg * 4 + h * 2 + (lane >> 4)) ^ (lane & 7)) * 16, aw[i][h].x, aw[i][h].y, aw[i][h].z, aw[i][h].w);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const int row = half * 32 + n * 8 + g;
             float f[8];
             uint4 xv;
             if (XF32) {
-                const uint8_t *r = xs + row * (kSortK * 4);
-                const float4 u = *reinterpret_cast<const float4 *>(r + ((kg * 8 + t4 * 2) ^ (g & 1)) * 16);
-                const float4 v = *reinterpret_cast<const float4 *>(r + ((kg * 8 + t4 * 2 + 1) ^ (g & 1)) * 16);
-                f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
-                f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
-            } else {
-                xv = *reinterpret_cast<const uint4 *>(xs + row * (kSortK * 2) + ((kg * 4 + t4) ^ (g & 1) * 4) * 16);
+                const uint8_t *r = xs + (half * 32 + n * 8 + g) * (kSortK * 4) + (t4 & 1) * 8;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<float2 *>(f + 2 * j) = *reinterpret_cast<const float2 *>(r + ((kg * 8 + j * 2 + (t4 >> 1)) ^ g) * 16);
+            } else {  // K 0-7, 8-15, 16-23, 24-31 of eight tokens
+                ldmatrix_x4(xa + (half * 32 + n * 8 + (lane & 7)) * (kSortK * 2) + ((kg * 4 + (lane >> 3)) ^ (lane & 7)) * 16, xv.x, xv.y, xv.z, xv.w);
             }
 #pragma unroll
             for (int w = 0; w < (XF32 ? 3 : 1); ++w) {
                 if (XF32) xv = make_uint4(cut_bf16x2(f[0], f[1]), cut_bf16x2(f[2], f[3]), cut_bf16x2(f[4], f[5]), cut_bf16x2(f[6], f[7]));
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    mma_bf16(acc[i][n], aw[i][0].x, aw[i][1].x, aw[i][0].y, aw[i][1].y, xv.x, xv.y);
-                    mma_bf16(acc[i][n], aw[i][0].z, aw[i][1].z, aw[i][0].w, aw[i][1].w, xv.z, xv.w);
+                    mma_bf16(acc[i][n], aw[i][0].x, aw[i][0].y, aw[i][0].z, aw[i][0].w, xv.x, xv.y);
+                    mma_bf16(acc[i][n], aw[i][1].x, aw[i][1].y, aw[i][1].z, aw[i][1].w, xv.z, xv.w);
                 }
             }
         }
@@ -706,18 +706,23 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_ker
     }
 }
 
+// out = y + B S of a tile and a slice of N, 64 rows of B a warp at a time.  Here the tokens are the rows of the product
+// and B's rows its columns: a fragment of B is two neighbouring registers of a 16-byte load, and S lies in shared memory
+// in fragments, so nothing is moved between registers (with the operands the other way round, four moves a product,
+// 73 us for the 4000 rows of rank 64).  Row 16 q + 4 (c / 2) + 2 i + c % 2 of the 64 is column c of product 2 q + i,
+// which leaves a lane four consecutive outputs of a token.  The y of a step, 16 tokens and 32 rows of B, is requested
+// kAhead steps ahead of its sum.
 template <int RT>
 struct ExpandShape {
-    static constexpr int kRow = LoraShape<RT, 1>::kRow, kSmem = 3 * kSortTokens * kRow;
+    static constexpr int kFragments = 4 * RT;                     // (tokens of 16, ranks of 16)
+    static constexpr int kSmem = 3 * kFragments * 512;
 };
 constexpr int kExpandN = kLoraWarps * 64;     // rows of B a block takes at a time
 
-// out = y + B S of a tile and a slice of N, 64 rows of B a warp at a time.  The y of eight tokens is requested four steps
-// ahead of its sum.
 template <int RT, bool YF32>
 __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
     using S = ExpandShape<RT>;
-    constexpr int es = YF32 ? 4 : 2, kUnits = kSortTokens / 8, kAhead = RT <= 2 ? 2 : 4;
+    constexpr int es = YF32 ? 4 : 2, kStepsN = kSortTokens / 16 * 2, kAhead = RT <= 2 ? 2 : 4;
     extern __shared__ __align__(128) uint8_t lora_smem[];
     __shared__ int32_t toks[kSortTokens];
     __shared__ int64_t yoff[kSortTokens], ooff[kSortTokens];    // bytes; places without a token read the first one's
@@ -741,33 +746,30 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
     constexpr int KP = RT >= 2 ? RT / 2 : 1;
     const int rounds = (p.n + kExpandN - 1) / kExpandN, r0 = (int)((int64_t)rounds * slice / slices), r1 = (int)((int64_t)rounds * (slice + 1) / slices);
     const uint16_t *const table = p.b + (int64_t)q.adapter * p.n * p.r;
-    uint4 bw[4][2][KP];
+    uint4 bw[8][KP];
     auto weights = [&](int n0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 8; ++j) {
+            const int row = n0 + (j >> 1) * 16 + (g >> 1) * 4 + (j & 1) * 2 + (g & 1);
+            const uint16_t *b = table + (int64_t)min(row, p.n - 1) * p.r;
+            if (RT >= 2) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = n0 + h * 32 + g * 4 + j;
-                const uint16_t *b = table + (int64_t)min(row, p.n - 1) * p.r;
-                const int limit = row < p.n ? p.r : 0;
-                if (RT >= 2) {
-#pragma unroll
-                    for (int k = 0; k < KP; ++k) bw[j][h][k] = row8<true>(b, k * 32 + t4 * 8, limit);
-                } else {
-                    const uint2 v = load8_if(b + t4 * 4, t4 * 4 < limit);
-                    bw[j][h][0] = make_uint4(v.x, v.y, 0, 0);
-                }
+                for (int k = 0; k < KP; ++k) bw[j][k] = row8<true>(b, k * 32 + t4 * 8, p.r);
+            } else {
+                const uint2 v = load8_if(b + t4 * 4, t4 * 4 < p.r);
+                bw[j][0] = make_uint4(v.x, v.y, 0, 0);
             }
+        }
     };
-    uint4 yv[kAhead][4];
     const char *const ybase = static_cast<const char *>(p.y);
     char *const obase = static_cast<char *>(p.out);
-    auto request = [&](int u, int n0) {  // (rows behind the last one's read that; nothing of them is stored)
-        const int at[2] = {min(n0 + g * 4, p.n - 4) * es, min(n0 + 32 + g * 4, p.n - 4) * es};
+    uint4 yv[kAhead][4];
+    auto request = [&](int s, int n0) {  // (rows behind the last one's read that; nothing of them is stored)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const char *src = ybase + yoff[u * 8 + t4 * 2 + (e & 1)] + at[e >> 1];
-            uint4 &r = yv[u % kAhead][e];
+            const int at = min(n0 + ((s & 1) * 2 + (e & 1)) * 16 + t4 * 4, p.n - 4) * es;
+            const char *src = ybase + yoff[(s >> 1) * 16 + (e >> 1) * 8 + g] + at;
+            uint4 &r = yv[s % kAhead][e];
             // (y may be out: not a read-only load)
             if (YF32) asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(src) : "memory");
             else asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(src) : "memory");
@@ -775,8 +777,8 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
     };
     weights(r0 * kExpandN + warp * 64);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) request(u, r0 * kExpandN + warp * 64);
-    // scale * S in three bf16 parts
+    for (int s = 0; s < kAhead; ++s) request(s, r0 * kExpandN + warp * 64);
+    // scale * S in three bf16 parts, as fragments: ranks of a lane as B's 16-byte loads have them
     const float scale = p.scale ? p.scale[q.adapter] : 1.0f;
     for (int j = tid; j < kSortTokens * RT * 8; j += kLoraThreads) {
         const int place = j / (RT * 8), rank = j % (RT * 8) * 2, tok = toks[place];
@@ -784,49 +786,45 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
         if (tok >= 0 && rank < p.r) s = *reinterpret_cast<const float2 *>(p.s_in + (int64_t)tok * p.r + rank);   // (r is even)
         s.x *= scale;
         s.y *= scale;
+        const int step = RT >= 2 ? rank / 32 * 2 + rank % 8 / 4 : 0, col = RT >= 2 ? rank % 32 / 8 : rank / 4;
+        const int at = (place / 16 * RT + step) * 512 + (place % 8 * 4 + col) * 16 + (rank % 4 / 2 * 2 + place % 16 / 8) * 4;
 #pragma unroll
-        for (int w = 0; w < 3; ++w) *reinterpret_cast<uint32_t *>(lora_smem + (w * kSortTokens + place) * S::kRow + rank * 2) = cut_bf16x2(s.x, s.y);
+        for (int w = 0; w < 3; ++w) *reinterpret_cast<uint32_t *>(lora_smem + w * S::kFragments * 512 + at) = cut_bf16x2(s.x, s.y);
     }
     __syncthreads();
     for (int r = r0; r < r1; ++r) {
         const int n0 = r * kExpandN + warp * 64;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
+        for (int s = 0; s < kStepsN; ++s) {
             float acc[4][4] = {};
 #pragma unroll
-            for (int w = 0; w < 3; ++w) {
-                const uint8_t *srow = lora_smem + (w * kSortTokens + u * 8 + g) * S::kRow;
+            for (int w = 0; w < 3; ++w)
 #pragma unroll
-                for (int k = 0; k < KP; ++k) {
-                    if (RT >= 2) {
-                        const uint4 s = *reinterpret_cast<const uint4 *>(srow + k * 64 + t4 * 16);
+                for (int k = 0; k < RT; ++k) {
+                    const uint4 f = *reinterpret_cast<const uint4 *>(lora_smem + ((w * 4 + (s >> 1)) * RT + k) * 512 + lane * 16);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][k].x, bw[j][1][k].x, bw[j][0][k].y, bw[j][1][k].y, s.x, s.y);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][k].z, bw[j][1][k].z, bw[j][0][k].w, bw[j][1][k].w, s.z, s.w);
-                    } else {
-                        const uint2 s = *reinterpret_cast<const uint2 *>(srow + t4 * 8);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_bf16(acc[j], bw[j][0][0].x, bw[j][1][0].x, bw[j][0][0].y, bw[j][1][0].y, s.x, s.y);
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 &b = bw[(s & 1) * 4 + j][k / 2];
+                        mma_bf16(acc[j], f.x, f.y, f.z, f.w, k & 1 ? b.z : b.x, k & 1 ? b.w : b.y);
                     }
                 }
-            }
             // the next rows of B while the last sums of these are stored
-            if (u == kUnits - 1 && r + 1 < r1) weights(n0 + kExpandN);
+            if (s == kStepsN - 1 && r + 1 < r1) weights(n0 + kExpandN);
             float sum[4][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint4 &y = yv[u % kAhead][e];
-                sum[e][0] = __uint_as_float(YF32 ? y.x : y.x << 16) + acc[0][e];
-                sum[e][1] = __uint_as_float(YF32 ? y.y : y.x & 0xFFFF0000u) + acc[1][e];
-                sum[e][2] = __uint_as_float(YF32 ? y.z : y.y << 16) + acc[2][e];
-                sum[e][3] = __uint_as_float(YF32 ? y.w : y.y & 0xFFFF0000u) + acc[3][e];
+                const uint4 &y = yv[s % kAhead][e];
+                const int j = (e & 1) * 2, h = (e >> 1) * 2;
+                sum[e][0] = __uint_as_float(YF32 ? y.x : y.x << 16) + acc[j][h];
+                sum[e][1] = __uint_as_float(YF32 ? y.y : y.x & 0xFFFF0000u) + acc[j][h + 1];
+                sum[e][2] = __uint_as_float(YF32 ? y.z : y.y << 16) + acc[j + 1][h];
+                sum[e][3] = __uint_as_float(YF32 ? y.w : y.y & 0xFFFF0000u) + acc[j + 1][h + 1];
             }
-            if (u + kAhead < kUnits) request(u + kAhead, n0);
-            else if (r + 1 < r1) request(u + kAhead - kUnits, n0 + kExpandN);
+            if (s + kAhead < kStepsN) request(s + kAhead, n0);
+            else if (r + 1 < r1) request(s + kAhead - kStepsN, n0 + kExpandN);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int place = u * 8 + t4 * 2 + (e & 1), nn = n0 + (e >> 1) * 32 + g * 4;
+                const int place = (s >> 1) * 16 + (e >> 1) * 8 + g, nn = n0 + ((s & 1) * 2 + (e & 1)) * 16 + t4 * 4;
                 if (place >= q.count || nn >= p.n) continue;
                 char *const dst = obase + ooff[place] + (int64_t)nn * es;
                 if (YF32) *reinterpret_cast<float4 *>(dst) = make_float4(sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
