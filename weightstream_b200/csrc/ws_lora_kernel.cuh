@@ -66,11 +66,19 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
     wait_predecessor();
     __syncthreads();
     // (one atomic for all of a warp's tokens of an adapter: a prompt's tokens would queue for one word otherwise)
-    const int turns = (p.m + 1023) / 1024;
-    for (int i = 0; i < turns; ++i) {
-        const int t = tid + i * 1024, id = t < p.m ? lora_id(p, t) : -2, b = id < 0 ? p.adapters : id;
-        const uint32_t alike = __match_any_sync(0xffffffffu, id);
-        if (t < p.m && (alike & ((1u << lane) - 1)) == 0) atomicAdd(&count[b], __popc(alike));
+    constexpr int kBatch = 4;  // ids a thread requests together
+    int id[kBatch];
+    auto request = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) id[i] = t0 + i * 1024 + tid < p.m ? lora_id(p, t0 + i * 1024 + tid) : -2;
+    };
+    for (int t0 = 0; t0 < p.m; t0 += kBatch * 1024) {
+        request(t0);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const uint32_t alike = __match_any_sync(0xffffffffu, id[i]);
+            if (id[i] != -2 && (alike & ((1u << lane) - 1)) == 0) atomicAdd(&count[id[i] < 0 ? p.adapters : id[i]], __popc(alike));
+        }
     }
     __syncthreads();
     const int per = (buckets + 1023) / 1024, b0 = tid * per, b1 = min(buckets, b0 + per);
@@ -107,16 +115,20 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
         if (b < p.adapters || !p.skip_none) before_til += (c + p.tile - 1) / p.tile;
     }
     __syncthreads();
-    for (int i = 0; i < turns; ++i) {
-        const int t = tid + i * 1024, id = t < p.m ? lora_id(p, t) : -2, b = id < 0 ? p.adapters : id;
-        const uint32_t alike = __match_any_sync(0xffffffffu, id);
-        int left = 0;
-        if (t < p.m && (alike & ((1u << lane) - 1)) == 0) left = atomicSub(&count[b], __popc(alike));   // the bucket's size, less each time
-        left = __shfl_sync(0xffffffffu, left, __ffs(alike) - 1) - __popc(alike & ((1u << lane) - 1));
-        if (t >= p.m || (b == p.adapters && p.skip_none)) continue;
-        const int c = (b + 1 < buckets ? first[b + 1] : p.m) - first[b], at = c - left;
-        p.perm[first[b] + at] = t;
-        if (at % p.tile == 0) p.tiles[tile0[b] + at / p.tile] = LoraTile{id, first[b] + at, min(p.tile, c - at), 0};
+    for (int t0 = 0; t0 < p.m; t0 += kBatch * 1024) {
+        if (p.m > kBatch * 1024) request(t0);  // (else they are still there)
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int b = id[i] < 0 ? p.adapters : id[i];
+            const uint32_t alike = __match_any_sync(0xffffffffu, id[i]);
+            int left = 0;
+            if (id[i] != -2 && (alike & ((1u << lane) - 1)) == 0) left = atomicSub(&count[b], __popc(alike));   // the bucket's size, less each time
+            left = __shfl_sync(0xffffffffu, left, __ffs(alike) - 1) - __popc(alike & ((1u << lane) - 1));
+            if (id[i] == -2 || (b == p.adapters && p.skip_none)) continue;
+            const int c = (b + 1 < buckets ? first[b + 1] : p.m) - first[b], at = c - left;
+            p.perm[first[b] + at] = t0 + i * 1024 + tid;
+            if (at % p.tile == 0) p.tiles[tile0[b] + at / p.tile] = LoraTile{id[i], first[b] + at, min(p.tile, c - at), 0};
+        }
     }
 }
 
@@ -571,7 +583,7 @@ __device__ __forceinline__ void lora_copy16(uint32_t dst, const void *src, bool 
 // stage's K.  Rows lie in shared memory as in global memory, their 16-byte pieces swapped by the row's last three bits so
 // that the eight rows of a matrix lie in different banks.
 template <int RT, bool XF32>
-__global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __launch_bounds__(kLoraThreads, RT <= 2 || (RT == 4 && !XF32) ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
     namespace cg = cooperative_groups;
     using S = ShrinkShape<RT, XF32>;
     extern __shared__ __align__(128) uint8_t lora_smem[];
@@ -722,7 +734,7 @@ constexpr int kExpandN = kLoraWarps * 64;     // rows of B a block takes at a ti
 template <int RT, bool YF32>
 __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
     using S = ExpandShape<RT>;
-    constexpr int es = YF32 ? 4 : 2, kStepsN = kSortTokens / 16 * 2, kAhead = RT <= 2 ? 2 : 4;
+    constexpr int es = YF32 ? 4 : 2, kStepsN = kSortTokens / 16 * 2, kAhead = RT == 4 ? 4 : 2;
     extern __shared__ __align__(128) uint8_t lora_smem[];
     __shared__ int32_t toks[kSortTokens];
     __shared__ int64_t yoff[kSortTokens], ooff[kSortTokens];    // bytes; places without a token read the first one's

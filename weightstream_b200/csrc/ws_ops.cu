@@ -4,7 +4,6 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
-#include <cstdlib>
 
 #include "ws_lora_kernel.cuh"
 #include "ws_norm_kernel.cuh"
@@ -70,33 +69,34 @@ ws_status_t launch(const Err &err, void (*kernel)(P), dim3 grid, unsigned thread
 }
 
 // ---- norms
-template <int NV, bool VEC>
-auto norm_kernel(const NormParams &p) {
-    constexpr int F = WS_ACT_F32;
-    if constexpr (!VEC) return block_norm_rows_kernel<NV, false, true, true, true>;  // (types are looked at as it runs)
-    else if (p.y_dtype == F)
-        return p.r_dtype == F ? (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, true, true, true> : block_norm_rows_kernel<NV, VEC, true, true, false>)
-                              : (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, true, false, true> : block_norm_rows_kernel<NV, VEC, true, false, false>);
-    else
-        return p.r_dtype == F ? (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, false, true, true> : block_norm_rows_kernel<NV, VEC, false, true, false>)
-                          : (p.w_dtype == F ? block_norm_rows_kernel<NV, VEC, false, false, true> : block_norm_rows_kernel<NV, VEC, false, false, false>);
-}
-template <int NV>
-ws_status_t launch_norm(const Err &err, bool vec, const NormParams &p, void *stream) {
+template <int NV, bool VEC, bool YF32, int RK>
+ws_status_t launch_norm(const Err &err, const NormParams &p, void *stream) {
     const unsigned threads = (unsigned)((p.n + NV * 8 * 32 - 1) / (NV * 8 * 32)) * 32;
-    return launch(err, vec ? norm_kernel<NV, true>(p) : norm_kernel<NV, false>(p), dim3((unsigned)p.m), threads, 0, 1, stream, p);
+    const int gk = !p.gate || !p.gate_inc ? 0 : p.g_dtype == WS_ACT_F32 ? 2 : 1;
+    auto *k = gk == 0 ? block_norm_rows_kernel<NV, VEC, YF32, RK, 0> : gk == 1 ? block_norm_rows_kernel<NV, VEC, YF32, RK, 1>
+                                                                              : block_norm_rows_kernel<NV, VEC, YF32, RK, 2>;
+    return launch(err, k, dim3((unsigned)p.m), threads, 0, 1, stream, p);
+}
+template <int NV, bool VEC, bool YF32>
+ws_status_t launch_norm(const Err &err, const NormParams &p, void *stream) {
+    if (!p.residual) return launch_norm<NV, VEC, YF32, 0>(err, p, stream);
+    return p.r_dtype == WS_ACT_F32 ? launch_norm<NV, VEC, YF32, 2>(err, p, stream) : launch_norm<NV, VEC, YF32, 1>(err, p, stream);
+}
+template <int NV, bool VEC>
+ws_status_t launch_norm(const Err &err, const NormParams &p, void *stream) {
+    return p.y_dtype == WS_ACT_F32 ? launch_norm<NV, VEC, true>(err, p, stream) : launch_norm<NV, VEC, false>(err, p, stream);
 }
 ws_status_t norm(const Err &err, const NormParams &p, void *stream) {
     auto wide = [](const void *q, int64_t ld, int32_t type) { return !q || aligned(q, ld, type, 8 * type_bytes(type)); };
     const bool vec = p.n % 8 == 0 && wide(p.y, p.ldy, p.y_dtype) && wide(p.residual, p.ldr, p.r_dtype) && (!p.gate_inc || wide(p.gate, p.ldg, p.g_dtype)) &&
                      wide(p.post_weight, 0, p.w_dtype) && wide(p.next_weight, 0, p.w_dtype) && wide(p.hidden, p.ldh, p.h_dtype) && wide(p.normed, p.ldn, p.n_dtype);
-    static const char *ev = getenv("NV");
-    int nv = ev ? atoi(ev) : p.m <= 296 ? 1 : 2;
-    if (nv < 4 && p.n > 8192) nv = 4;
-    if (p.n > 16384) {
-        return launch(err, block_norm_any_kernel, dim3((unsigned)p.m), 512, 0, 1, stream, p);
-    }
-    return nv == 1 ? launch_norm<1>(err, vec, p, stream) : nv == 2 ? launch_norm<2>(err, vec, p, stream) : launch_norm<4>(err, vec, p, stream);
+    // Eight values a thread where rows are few or short (one row 2.7 us against 3.1 with sixteen, 1503 rows of 2307 11.0 us
+    // against 11.4); sixteen keep more blocks an SM loading while others sum (8192 rows of 7168 124 us against 186, with 32
+    // 155); wider rows need more registers a thread, up to 32 values.
+    const int nv = p.n > 8192 ? 4 : p.m <= 296 || p.n <= 2560 ? 1 : 2;
+    if (p.n > 16384) return launch(err, block_norm_any_kernel, dim3((unsigned)p.m), 512, 0, 1, stream, p);
+    if (vec) return nv == 1 ? launch_norm<1, true>(err, p, stream) : nv == 2 ? launch_norm<2, true>(err, p, stream) : launch_norm<4, true>(err, p, stream);
+    return nv == 1 ? launch_norm<1, false>(err, p, stream) : nv == 2 ? launch_norm<2, false>(err, p, stream) : launch_norm<4, false>(err, p, stream);
 }
 
 // ---- scores
@@ -198,8 +198,7 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
     const int rt = a->rank <= 16 ? 1 : a->rank <= 32 ? 2 : a->rank <= 64 ? 4 : 8;
     const int nt = a->m <= 128 ? 1 : 2;
     unsigned tiles = (unsigned)std::min((int64_t)a->m, lora_max_tiles(a->m, a->adapters, nt * 8));
-    static const char *ec = getenv("LC");
-    p.cluster = ec ? atoi(ec) : tiles <= 148 ? 8 : 4;
+    p.cluster = tiles <= 148 ? 8 : 4;  // (333 rows of up to 54 tiles 14.8 us with 8 blocks a tile, 17.4 with 4)
     if (a->m > kLoraDirect) {
         const int64_t need = ws_lora_workspace(a->m, a->adapters, a->rank);
         if (a->adapters > kLoraMaxAdapters) return err(WS_ERR_CAPACITY, "%d adapters: at most %d with more than %d tokens", a->adapters, kLoraMaxAdapters, kLoraDirect);
@@ -225,7 +224,6 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
                 // K is cut until the blocks fill the card twice
                 q.cluster = 1;
                 while (q.cluster < 8 && (int64_t)tiles * q.cluster < 148 && a->k / (2 * q.cluster) >= 2 * kSortK) q.cluster *= 2;
-                if (ec) q.cluster = atoi(ec);
                 q.skip_none = 0;
                 st = rt == 1 ? launch_shrink<1>(err, xf32, tiles, stream, q) : rt == 2 ? launch_shrink<2>(err, xf32, tiles, stream, q)
                      : rt == 4 ? launch_shrink<4>(err, xf32, tiles, stream, q) : launch_shrink<8>(err, xf32, tiles, stream, q);
