@@ -99,6 +99,14 @@ def test_sizes(dev, k, n, m, adapters):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k,n", [(1025, 516), (1030, 516), (1024, 517), (1025, 517), (129, 3), (1, 65)])
+@pytest.mark.parametrize("rank", [8, 32, 64, 128])
+@pytest.mark.parametrize("xt,yt", [(BF16, F32), (F32, BF16)])
+def test_sorted_odd_sizes(dev, k, n, rank, xt, yt):
+    check(dev, 600, k, n, rank, 3, xt=xt, yt=yt)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("xt", [F32, BF16])
 @pytest.mark.parametrize("yt", [F32, BF16])
 @pytest.mark.parametrize("rank", [16, 32, 64, 128])

@@ -61,7 +61,7 @@ def _run(cmd, verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if force or _older(LIB, [os.path.join(CSRC, f) for f in SOURCES + HEADERS]):
-        _run([nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
+        _run([nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "--threads", "0",
               "-shared", "-Xcompiler", "-fPIC", "-Xptxas", "-v" if verbose else "-O3",
               "-o", LIB] + [os.path.join(CSRC, s) for s in SOURCES] + ["-lcudart"], verbose)
     if force or _torch_ext_is_stale():

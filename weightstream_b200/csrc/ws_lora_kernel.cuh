@@ -579,11 +579,27 @@ __device__ __forceinline__ void lora_copy16(uint32_t dst, const void *src, bool 
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
+__device__ __forceinline__ void lora_copy4x4(uint32_t dst, const char *src, int left) {  // four words, those from `left` on as zeros
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + j * 4), "l"(src + j * 4), "r"(j < left ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void lora_take8(uint32_t dst, const char *src, int left) {    // eight bf16, those from `left` on as zeros
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b16 l, h;\n\tmov.b16 l, 0;\n\tmov.b16 h, 0;\n\tsetp.gt.s32 p, %2, 0;\n\tsetp.gt.s32 q, %2, 1;\n\t"
+                     "@p ld.global.nc.b16 l, [%1];\n\t@q ld.global.nc.b16 h, [%1+2];\n\tmov.b32 %0, {l, h};\n\t}"
+                     : "=r"(w[j]) : "l"(src + j * 4), "r"(left - 2 * j) : "memory");
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
 // S = A x^T of a tile, K cut over the blocks of a cluster.  Eight warps: two halves of the tokens, four steps of 32 of a
 // stage's K.  Rows lie in shared memory as in global memory, their 16-byte pieces swapped by the row's last three bits so
 // that the eight rows of a matrix lie in different banks.
-template <int RT, bool XF32>
-__global__ void __launch_bounds__(kLoraThreads, RT <= 2 || (RT == 4 && !XF32) ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+// VEC: rows of x and A are 16-byte aligned.  Else their values are copied one by one, bf16 ones through registers.
+template <int RT, bool XF32, bool VEC>
+__global__ void __launch_bounds__(kLoraThreads, VEC && (RT <= 2 || (RT == 4 && !XF32)) ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
     namespace cg = cooperative_groups;
     using S = ShrinkShape<RT, XF32>;
     extern __shared__ __align__(128) uint8_t lora_smem[];
@@ -631,12 +647,16 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 || (RT == 4 && !XF32) ? 
             const uint32_t at = slot_in * S::kStage;
 #pragma unroll
             for (int i = 0; i < XN; ++i) {
-                lora_copy16(xdst + at + i * XR * (kSortK * (XF32 ? 4 : 2)), xsrc[i], xin);
+                const uint32_t dst = xdst + at + i * XR * (kSortK * (XF32 ? 4 : 2));
+                if (VEC) lora_copy16(dst, xsrc[i], xin);
+                else if (XF32) lora_copy4x4(dst, xsrc[i], p.k - st * kSortK - xc * xe);
+                else lora_take8(dst, xsrc[i], p.k - st * kSortK - xc * xe);
                 xsrc[i] += kSortK * (XF32 ? 4 : 2);
             }
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                lora_copy16(adst + at + i * 16 * (kSortK * 2), asrc[i], ain);
+                if (VEC) lora_copy16(adst + at + i * 16 * (kSortK * 2), asrc[i], ain);
+                else lora_take8(adst + at + i * 16 * (kSortK * 2), asrc[i], p.k - st * kSortK - ac * 8);
                 asrc[i] += kSortK * 2;
             }
         }
@@ -731,7 +751,8 @@ struct ExpandShape {
 };
 constexpr int kExpandN = kLoraWarps * 64;     // rows of B a block takes at a time
 
-template <int RT, bool YF32>
+// VEC: four consecutive values of y and of out are one access.
+template <int RT, bool YF32, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_kernel(const __grid_constant__ LoraParams p) {
     using S = ExpandShape<RT>;
     constexpr int es = YF32 ? 4 : 2, kStepsN = kSortTokens / 16 * 2, kAhead = RT == 4 ? 4 : 2;
@@ -752,7 +773,7 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
     }
     __syncthreads();
     if (q.adapter < 0) {
-        lora_none<true>(p, toks, kSortTokens, slice, slices);
+        lora_none<VEC>(p, toks, kSortTokens, slice, slices);
         return;
     }
     constexpr int KP = RT >= 2 ? RT / 2 : 1;
@@ -779,12 +800,24 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
     auto request = [&](int s, int n0) {  // (rows behind the last one's read that; nothing of them is stored)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int at = min(n0 + ((s & 1) * 2 + (e & 1)) * 16 + t4 * 4, p.n - 4) * es;
-            const char *src = ybase + yoff[(s >> 1) * 16 + (e >> 1) * 8 + g] + at;
+            const int nn = n0 + ((s & 1) * 2 + (e & 1)) * 16 + t4 * 4;
+            const char *row = ybase + yoff[(s >> 1) * 16 + (e >> 1) * 8 + g];
             uint4 &r = yv[s % kAhead][e];
             // (y may be out: not a read-only load)
-            if (YF32) asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(src) : "memory");
-            else asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(src) : "memory");
+            if (VEC) {
+                const char *src = row + min(nn, p.n - 4) * es;
+                if (YF32) asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(src) : "memory");
+                else asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(src) : "memory");
+            } else {
+                uint32_t v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const char *src = row + min(nn + j, p.n - 1) * es;
+                    if (YF32) asm volatile("ld.global.b32 %0, [%1];" : "=r"(v[j]) : "l"(src) : "memory");
+                    else asm volatile("{\n\t.reg .b16 h, z;\n\tmov.b16 z, 0;\n\tld.global.b16 h, [%1];\n\tmov.b32 %0, {z, h};\n\t}" : "=r"(v[j]) : "l"(src) : "memory");
+                }
+                r = make_uint4(v[0], v[1], v[2], v[3]);
+            }
         }
     };
     weights(r0 * kExpandN + warp * 64);
@@ -827,10 +860,11 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
             for (int e = 0; e < 4; ++e) {
                 const uint4 &y = yv[s % kAhead][e];
                 const int j = (e & 1) * 2, h = (e >> 1) * 2;
-                sum[e][0] = __uint_as_float(YF32 ? y.x : y.x << 16) + acc[j][h];
-                sum[e][1] = __uint_as_float(YF32 ? y.y : y.x & 0xFFFF0000u) + acc[j][h + 1];
-                sum[e][2] = __uint_as_float(YF32 ? y.z : y.y << 16) + acc[j + 1][h];
-                sum[e][3] = __uint_as_float(YF32 ? y.w : y.y & 0xFFFF0000u) + acc[j + 1][h + 1];
+                constexpr bool packed = VEC && !YF32;
+                sum[e][0] = __uint_as_float(packed ? y.x << 16 : y.x) + acc[j][h];
+                sum[e][1] = __uint_as_float(packed ? y.x & 0xFFFF0000u : y.y) + acc[j][h + 1];
+                sum[e][2] = __uint_as_float(packed ? y.y << 16 : y.z) + acc[j + 1][h];
+                sum[e][3] = __uint_as_float(packed ? y.y & 0xFFFF0000u : y.w) + acc[j + 1][h + 1];
             }
             if (s + kAhead < kStepsN) request(s + kAhead, n0);
             else if (r + 1 < r1) request(s + kAhead - kStepsN, n0 + kExpandN);
@@ -839,7 +873,11 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
                 const int place = (s >> 1) * 16 + (e >> 1) * 8 + g, nn = n0 + ((s & 1) * 2 + (e & 1)) * 16 + t4 * 4;
                 if (place >= q.count || nn >= p.n) continue;
                 char *const dst = obase + ooff[place] + (int64_t)nn * es;
-                if (YF32) *reinterpret_cast<float4 *>(dst) = make_float4(sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
+                if (!VEC) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (nn + i < p.n) store1(dst, YF32 ? WS_ACT_F32 : WS_ACT_BF16, i, sum[e][i]);
+                } else if (YF32) *reinterpret_cast<float4 *>(dst) = make_float4(sum[e][0], sum[e][1], sum[e][2], sum[e][3]);
                 else *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(sum[e][0], sum[e][1]), pack_bf16x2(sum[e][2], sum[e][3]));
             }
         }

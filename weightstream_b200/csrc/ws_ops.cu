@@ -136,27 +136,30 @@ ws_status_t launch_lora(const Err &err, int nt, bool xf32, bool vec, unsigned ti
     return nt == 1 ? launch_lora<RT, 1>(err, xf32, vec, tiles, stream, p) : launch_lora<RT, 2>(err, xf32, vec, tiles, stream, p);
 }
 
-template <int RT, bool XF32>
+template <int RT, bool XF32, bool VEC>
 ws_status_t launch_shrink(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
-    constexpr auto k = lora_shrink_kernel<RT, XF32>;
+    constexpr auto k = lora_shrink_kernel<RT, XF32, VEC>;
     constexpr int smem = ShrinkShape<RT, XF32>::kSmem;
     const ws_status_t st = allow_smem<k>(err, smem);
     return st != WS_OK ? st : launch(err, k, dim3(tiles * (unsigned)p.cluster), kLoraThreads, smem, (unsigned)p.cluster, stream, p);
 }
 template <int RT>
-ws_status_t launch_shrink(const Err &err, bool xf32, unsigned tiles, void *stream, const LoraParams &p) {
-    return xf32 ? launch_shrink<RT, true>(err, tiles, stream, p) : launch_shrink<RT, false>(err, tiles, stream, p);
+ws_status_t launch_shrink(const Err &err, bool xf32, bool vec, unsigned tiles, void *stream, const LoraParams &p) {
+    if (vec) return xf32 ? launch_shrink<RT, true, true>(err, tiles, stream, p) : launch_shrink<RT, false, true>(err, tiles, stream, p);
+    return xf32 ? launch_shrink<RT, true, false>(err, tiles, stream, p) : launch_shrink<RT, false, false>(err, tiles, stream, p);
 }
-template <int RT, bool YF32>
+template <int RT, bool YF32, bool VEC>
 ws_status_t launch_expand(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
-    constexpr auto k = lora_expand_kernel<RT, YF32>;
+    constexpr auto k = lora_expand_kernel<RT, YF32, VEC>;
     constexpr int smem = ExpandShape<RT>::kSmem;
     const ws_status_t st = allow_smem<k>(err, smem);
     return st != WS_OK ? st : launch(err, k, dim3(tiles * (unsigned)p.cluster), kLoraThreads, smem, 1, stream, p);
 }
 template <int RT>
-ws_status_t launch_expand(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
-    return p.y_dtype == WS_ACT_F32 ? launch_expand<RT, true>(err, tiles, stream, p) : launch_expand<RT, false>(err, tiles, stream, p);
+ws_status_t launch_expand(const Err &err, bool vec, unsigned tiles, void *stream, const LoraParams &p) {
+    const bool yf32 = p.y_dtype == WS_ACT_F32;
+    if (vec) return yf32 ? launch_expand<RT, true, true>(err, tiles, stream, p) : launch_expand<RT, false, true>(err, tiles, stream, p);
+    return yf32 ? launch_expand<RT, true, false>(err, tiles, stream, p) : launch_expand<RT, false, false>(err, tiles, stream, p);
 }
 
 enum class Lora { kAdd, kShrink, kExpand };
@@ -188,13 +191,15 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
     p.ids = a->ids; p.m = a->m; p.r = a->rank; p.adapters = a->adapters;
     p.skip_none = expands && a->y == a->out && a->ldy == a->ldo;
     const bool xf32 = shrinks && a->x_dtype == WS_ACT_F32;
-    bool vec = a->rank % 8 == 0;
-    if (shrinks) vec = vec && a->k % 8 == 0 && aligned(a->x, a->ldx, a->x_dtype, 16) && aligned(a->a, a->k, WS_ACT_BF16, 16);
+    // whole vectors of ranks; of K; of N
+    const bool vec_r = a->rank % 8 == 0 && (!expands || aligned(a->b, a->rank, WS_ACT_BF16, 16));
+    bool vec_k = true, vec_n = true;
+    if (shrinks) vec_k = a->k % 8 == 0 && aligned(a->x, a->ldx, a->x_dtype, 16) && aligned(a->a, a->k, WS_ACT_BF16, 16);
     if (expands) {
         const int64_t four = 4 * type_bytes(a->y_dtype);
-        vec = vec && a->n % 4 == 0 && aligned(a->y, a->ldy, a->y_dtype, four) && aligned(a->out, a->ldo, a->y_dtype, four) &&
-              aligned(a->b, a->rank, WS_ACT_BF16, 16);
+        vec_n = a->n % 4 == 0 && aligned(a->y, a->ldy, a->y_dtype, four) && aligned(a->out, a->ldo, a->y_dtype, four);
     }
+    const bool vec = vec_r && vec_k && vec_n;
     const int rt = a->rank <= 16 ? 1 : a->rank <= 32 ? 2 : a->rank <= 64 ? 4 : 8;
     const int nt = a->m <= 128 ? 1 : 2;
     unsigned tiles = (unsigned)std::min((int64_t)a->m, lora_max_tiles(a->m, a->adapters, nt * 8));
@@ -204,7 +209,7 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
         if (a->adapters > kLoraMaxAdapters) return err(WS_ERR_CAPACITY, "%d adapters: at most %d with more than %d tokens", a->adapters, kLoraMaxAdapters, kLoraDirect);
         if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) & 15)
             return err(WS_ERR_INVALID, "%d tokens need a 16-byte aligned workspace of %lld bytes", a->m, (long long)need);
-        p.tile = vec ? kSortTokens : nt * 8;
+        p.tile = vec_r ? kSortTokens : nt * 8;
         p.tiles_count = static_cast<int32_t *>(a->workspace);
         p.perm = p.tiles_count + 4;
         p.tiles = reinterpret_cast<LoraTile *>(static_cast<char *>(a->workspace) + lora_perm_bytes(a->m));
@@ -216,7 +221,7 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
         }
         ws_status_t st = launch(err, lora_plan_kernel, dim3(1), 1024, smem, 1, stream, p);
         if (st != WS_OK) return st;
-        if (vec) {
+        if (vec_r) {
             if (shrinks) {
                 LoraParams q = p;
                 if (expands) q.s_out = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + need) - (int64_t)a->m * a->rank;
@@ -225,8 +230,8 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
                 q.cluster = 1;
                 while (q.cluster < 8 && (int64_t)tiles * q.cluster < 148 && a->k / (2 * q.cluster) >= 2 * kSortK) q.cluster *= 2;
                 q.skip_none = 0;
-                st = rt == 1 ? launch_shrink<1>(err, xf32, tiles, stream, q) : rt == 2 ? launch_shrink<2>(err, xf32, tiles, stream, q)
-                     : rt == 4 ? launch_shrink<4>(err, xf32, tiles, stream, q) : launch_shrink<8>(err, xf32, tiles, stream, q);
+                st = rt == 1 ? launch_shrink<1>(err, xf32, vec_k, tiles, stream, q) : rt == 2 ? launch_shrink<2>(err, xf32, vec_k, tiles, stream, q)
+                     : rt == 4 ? launch_shrink<4>(err, xf32, vec_k, tiles, stream, q) : launch_shrink<8>(err, xf32, vec_k, tiles, stream, q);
                 if (st != WS_OK || !expands) return st;
             }
             // N is cut so that the slices' blocks, one an SM from rank 33 and two below, end together with the tiles that there
@@ -241,8 +246,8 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
                     p.cluster = c;
                 }
             }
-            return rt == 1 ? launch_expand<1>(err, tiles, stream, p) : rt == 2 ? launch_expand<2>(err, tiles, stream, p)
-                   : rt == 4 ? launch_expand<4>(err, tiles, stream, p) : launch_expand<8>(err, tiles, stream, p);
+            return rt == 1 ? launch_expand<1>(err, vec_n, tiles, stream, p) : rt == 2 ? launch_expand<2>(err, vec_n, tiles, stream, p)
+                   : rt == 4 ? launch_expand<4>(err, vec_n, tiles, stream, p) : launch_expand<8>(err, vec_n, tiles, stream, p);
         }
     }
     switch (rt) {
