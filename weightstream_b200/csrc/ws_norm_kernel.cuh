@@ -6,6 +6,11 @@
 //
 // All of it is held in 32 bits between the loads and the one rounding of h and of z to their types; z is taken from the
 // unrounded h.
+//
+// Bound: HBM for many rows (8192 rows of 7168 with a gate a value: 124 us, 5.7 TB/s; a row's two sums are the time in
+// which its block loads nothing, so that several blocks share an SM), the launch for few (one row 2.7 us on the device).
+// Widths that no vector divides load value by value and are bound by those instructions (1503 rows of 2307: 11.0 us,
+// 3.2 TB/s).
 #pragma once
 
 #include <type_traits>

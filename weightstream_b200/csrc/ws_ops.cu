@@ -103,8 +103,8 @@ ws_status_t norm(const Err &err, const NormParams &p, void *stream) {
 template <int T, bool F32, bool TOP>
 ws_status_t launch_scores(const Err &err, const ScoreParams &p, void *stream) {
     constexpr auto k = token_scores_kernel<T, F32, TOP>;
-    const ws_status_t st = allow_smem<k>(err, kScoreSmem<T>);
-    return st != WS_OK ? st : launch(err, k, dim3((unsigned)p.m * p.cluster), T, kScoreSmem<T>, (unsigned)p.cluster, stream, p);
+    const ws_status_t st = allow_smem<k>(err, kScoreSmem<T, F32>);
+    return st != WS_OK ? st : launch(err, k, dim3((unsigned)p.m * p.cluster), T, kScoreSmem<T, F32>, (unsigned)p.cluster, stream, p);
 }
 template <int T>
 ws_status_t launch_scores(const Err &err, bool f32, const ScoreParams &p, void *stream) {
@@ -322,8 +322,8 @@ ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *a, void *stream, c
     p.logprob = a->logprob; p.entropy = a->entropy; p.top_logprob = a->top_logprob; p.rank = a->rank; p.top_id = a->top_id;
     // Few rows: a row is cut over a cluster, as long as two blocks an SM take them all (64 rows: 17 us with four blocks a
     // row, 23 with two, 29 with eight) and a thread of each has a vector.  Blocks of 512 threads then have the shorter way
-    // (one row 9 us against 12, 64 rows 17 against 21); three blocks of 256 an SM stream faster when there are more (2000
-    // rows 157 us against 161, with 20 alternatives 193 against 217).
+    // (one row 9 us against 12, 64 rows 17 against 21); smaller blocks, three or four an SM, lose less while one of them
+    // ranks its alternatives (2000 rows with 20 of them 190 us against 217, without them 160 against 161).
     const int vector = a->dtype == WS_ACT_F32 ? 4 : 8;
     int c = 1;
     while (c < 8 && (int64_t)a->m * c * 2 <= 320 && a->vocab / (2 * c) >= vector * 256) c *= 2;
