@@ -10,8 +10,8 @@
 // memory: the order of a contraction's terms is free, so a lane takes 8 consecutive values of a row, 16 bytes, as the
 // terms that the instruction's fragment layout gives it (4 lanes x 16 bytes are two whole sectors of a row), and no
 // shared memory or shuffles lie between.  mma.sync's rate is enough at the ranks in use: 2 m r (k + n) operations, three
-// times that where an operand is split, against m (2 k + 8 n) bytes; 4000 rows of rank 64 need 27 us of it and 47 us of
-// HBM.
+// times that where an operand is split, against m (2 k + 8 n) bytes; 4000 rows of rank 64 keep it busy for 30 us and
+// HBM for 47.
 //
 // Bound: latency for few tokens (one row of 8192 x 7168 at rank 16 5.4 us, 64 rows of 24 adapters 10.8 us, of which HBM
 // needs 2.5: finding the tile, two waits for HBM and the blocks' meeting follow one another).  For prompts HBM would be
