@@ -29,7 +29,6 @@ namespace ws {
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
-constexpr int kLoraMaxRank = 128;
 constexpr int kLoraMaxCluster = 8;
 constexpr int kLoraDirect = 512;             // up to this many tokens a block finds its tile by itself
 constexpr int kLoraMaxAdapters = 16384;      // of a sorted batch: two words of shared memory each

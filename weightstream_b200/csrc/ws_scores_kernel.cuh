@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(T, T == 512 ? 2 : F32 ? 4 : 3) token_scores_ke
     if (TOP && tid == 0) sh.listed = sh.found = sh.kept = 0;
     float m = kLowest, best = kNegInf;   // m: what s and t refer to; best: maximum of this thread's values
     int32_t best_b = 0, before = 0;      // the first batch that holds it
-    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2, many = s2;  // many: counts, whole numbers far below 2^24 (checked: a thread's share of a row)
+    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2, many = s2;  // many: counts of at most 2^23, a thread's share of a row
     float note = __uint_as_float(0x7FC00000u);  // values from here on are noted; NaN: none
     uint4 raw[kBatch];
     for (int b = 0; b < batches; ++b) {
