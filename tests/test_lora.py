@@ -333,3 +333,22 @@ def test_c_entry_refuses_a_short_workspace(dev):
     for ptr, size in ((None, need), (work.data_ptr(), need - 1), (work.data_ptr() + 4, need)):
         a.workspace, a.workspace_bytes = ptr, size
         assert L.ws_lora_add(C.byref(a), None, err, len(err)) == _lib.WS_ERR_INVALID and b"workspace" in err.value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", [8, 16, 32, 64, 128, 7])
+@pytest.mark.parametrize("m", [20, 513, 600])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_shrunk_rows_at_any_float(dev, rank, m, offset):
+    """Shrunk rows that begin anywhere in a buffer, as a view into what one all-reduce returned for several projections."""
+    from weightstream_b200 import ops
+    rng = np.random.default_rng(17 * rank + m + offset)
+    y, b = make(rng, (m, 136), F32, dev), make(rng, (5, 136, rank), BF16, dev, 0.3)
+    ids, scale = batch(rng, m, 5, dev), make(rng, (5,), F32, dev)
+    many = make(rng, (offset + m * rank,), F32, dev)
+    t = many[offset:].view(m, rank)
+    assert t.is_contiguous() and t.data_ptr() % 16 == 4 * offset
+    _, _, out, err = ref(y, None, None, b, ids, scale, shrunk=t)
+    got = ops.lora_expand(y, t, b, ids, scale)
+    close(got, out, err)
+    assert torch.equal(got, ops.lora_expand(y, t.clone(), b, ids, scale))

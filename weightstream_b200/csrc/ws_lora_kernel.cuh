@@ -833,7 +833,10 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 2 ? 2 : 1) lora_expand_ker
     for (int j = tid; j < kSortTokens * RT * 8; j += kLoraThreads) {
         const int place = j / (RT * 8), rank = j % (RT * 8) * 2, tok = toks[place];
         float2 s = make_float2(0.0f, 0.0f);
-        if (tok >= 0 && rank < p.r) s = *reinterpret_cast<const float2 *>(p.s_in + (int64_t)tok * p.r + rank);   // (r is even)
+        if (tok >= 0 && rank < p.r) {  // (r is even; the shrunk rows may be a caller's, aligned to 4 bytes: no vector)
+            const float *const src = p.s_in + (int64_t)tok * p.r + rank;
+            s = make_float2(src[0], src[1]);
+        }
         s.x *= scale;
         s.y *= scale;
         const int step = RT >= 2 ? rank / 32 * 2 + rank % 8 / 4 : 0, col = RT >= 2 ? rank % 32 / 8 : rank / 4;
