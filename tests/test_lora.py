@@ -352,3 +352,22 @@ def test_shrunk_rows_at_any_float(dev, rank, m, offset):
     got = ops.lora_expand(y, t, b, ids, scale)
     close(got, out, err)
     assert torch.equal(got, ops.lora_expand(y, t.clone(), b, ids, scale))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", [1, 7, 8, 16, 24, 40, 72, 100])
+@pytest.mark.parametrize("m", [1, 5, 200, 512, 600])
+@pytest.mark.parametrize("xt", [F32, BF16])
+def test_an_infinite_activation_is_infinite_at_any_rank(dev, rank, m, xt):
+    """Positive weights and one infinite activation of a sign: the definition gives that infinity and no NaN, however many
+    ranks a tile is filled up to."""
+    from weightstream_b200 import ops
+    rng = np.random.default_rng(rank + m)
+    x, y = make(rng, (m, 72), xt, dev), make(rng, (m, 68), F32, dev)
+    a, b = make(rng, (3, rank, 72), BF16, dev).abs() + 0.01, make(rng, (3, 68, rank), BF16, dev).abs() + 0.01
+    ids = torch.arange(m, dtype=torch.int32, device=dev) % 3
+    x[m // 2, 5], x[m - 1, 71] = float("inf"), -float("inf")
+    for got in (ops.lora_add(y, x, a, b, ids), ops.lora_expand(y, ops.lora_shrink(x, a, ids), b, ids)):
+        if m > 1:
+            assert (got[m // 2] == float("inf")).all() and (got[m - 1] == -float("inf")).all()
+        assert (~torch.isfinite(got).all(1)).nonzero().squeeze(1).tolist() == ([m // 2, m - 1] if m > 1 else [0])

@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kLoraThreads, RT == 1 ? 2 : 1) lora_kernel(con
             if (tok >= 0 && rank < p.r) p.s_out[(int64_t)tok * p.r + rank] = s;
             continue;
         }
-        s *= scale;
+        s = rank < p.r ? s * scale : 0.0f;  // (A's missing rows are zeros, which an infinite activation makes NaN)
 #pragma unroll
         for (int w = 0; w < 3; ++w) {
             *reinterpret_cast<uint16_t *>(split + (w * S::kTokens + place) * S::kRow + rank * 2) = (uint16_t)(__float_as_uint(s) >> 16);
