@@ -218,3 +218,15 @@ def test_calls_refuse(dev):
         ops.block_norm(**plain())  # tensors of the host
     with pytest.raises(ValueError):
         ops.block_norm(**{**move(plain()), "residual": plain()["residual"]})
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 4096, 0, -1])
+def test_c_entry_refuses_widths_that_its_counters_do_not_hold(n):
+    """A row is counted in 32 bits, up to a block's step past its end.  (No rows, so that nothing could be launched.)"""
+    import ctypes as C
+    from weightstream_b200 import _lib
+    L, err = _lib.load(), C.create_string_buffer(256)
+    a = _lib.BlockNormArgs(m=0, n=n, eps=1e-6)
+    assert L.ws_block_norm(C.byref(a), None, err, len(err)) == _lib.WS_ERR_INVALID and b"out of range" in err.value
+    a.n = 2 ** 31 - 4097
+    assert L.ws_block_norm(C.byref(a), None, err, len(err)) == _lib.WS_OK

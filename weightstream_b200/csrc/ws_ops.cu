@@ -275,7 +275,8 @@ ws_status_t ws_block_norm(const ws_block_norm_args_t *a, void *stream, char *err
     const Err err{err_text, err_len};
     if (err_text && err_len) err_text[0] = 0;
     if (!a) return err(WS_ERR_INVALID, "null args");
-    if (a->m < 0 || a->n < 1) return err(WS_ERR_INVALID, "m=%d n=%d: m must not be negative, n at least 1", a->m, a->n);
+    // (the kernels count a row's values in 32 bits, up to a step past its end)
+    if (a->m < 0 || a->n < 1 || a->n > INT32_MAX - 4096) return err(WS_ERR_INVALID, "m=%d n=%d out of range", a->m, a->n);
     if (!is_type(a->y_dtype) || !is_type(a->residual_dtype) || !is_type(a->gate_dtype) || !is_type(a->weight_dtype) ||
         !is_type(a->hidden_dtype) || !is_type(a->normed_dtype))
         return err(WS_ERR_INVALID, "unknown type of a tensor");
