@@ -260,3 +260,16 @@ def test_calls_refuse(dev):
         ops.token_logprobs(**plain())
     with pytest.raises(ValueError):
         ops.token_logprobs(**{**move(plain()), "tokens": plain()["tokens"]})
+
+
+@pytest.mark.parametrize("name", ["logits", "tokens", "logprob", "entropy", "rank", "top_id", "top_logprob"])
+def test_c_entry_refuses_what_is_not_aligned(name):
+    """Results as well as inputs, before anything is launched."""
+    import ctypes as C
+    from weightstream_b200 import _lib
+    L, err = _lib.load(), C.create_string_buffer(256)
+    a = _lib.TokenLogprobsArgs(m=1, vocab=64, ld=64, top=2, dtype=_lib.WS_ACT_F32, token_bytes=4)
+    room = torch.zeros(7, 128)
+    for i, n in enumerate(["logits", "tokens", "logprob", "entropy", "rank", "top_id", "top_logprob"]):
+        setattr(a, n, room[i].data_ptr() + (2 if n == name else 0))
+    assert L.ws_token_logprobs(C.byref(a), None, err, len(err)) == _lib.WS_ERR_INVALID and b"aligned" in err.value

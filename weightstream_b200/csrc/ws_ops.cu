@@ -316,7 +316,9 @@ ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *a, void *stream, c
     if (!a->logits || !a->tokens || !a->logprob || !a->entropy || !a->rank || (a->top && (!a->top_id || !a->top_logprob)))
         return err(WS_ERR_INVALID, "a tensor is missing");
     if (a->ld < a->vocab) return err(WS_ERR_INVALID, "the row stride %lld is shorter than the row of %d values", (long long)a->ld, a->vocab);
-    if (!natural(a->logits, a->dtype) || reinterpret_cast<uintptr_t>(a->tokens) % a->token_bytes)
+    if (!natural(a->logits, a->dtype) || reinterpret_cast<uintptr_t>(a->tokens) % a->token_bytes || !natural(a->logprob, WS_ACT_F32) ||
+        !natural(a->entropy, WS_ACT_F32) || !natural(a->rank, WS_ACT_F32) ||
+        (a->top && (!natural(a->top_id, WS_ACT_F32) || !natural(a->top_logprob, WS_ACT_F32))))
         return err(WS_ERR_INVALID, "a tensor is not aligned to its type");
     ScoreParams p{};
     p.logits = a->logits; p.tokens = a->tokens; p.ld = a->ld; p.m = a->m; p.vocab = a->vocab; p.top = a->top; p.token_bytes = a->token_bytes;
