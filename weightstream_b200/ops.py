@@ -67,6 +67,17 @@ def _on(device: torch.device, stream):
     return both
 
 
+def _handle(stream, t) -> Optional[int]:
+    """A stream's handle, None for the current one.  Entering a stream of another device would make that device the
+    current one, which then reads this one's memory.  (A stream that is only a handle cannot be told from its own.)"""
+    if stream is None:
+        return None
+    device = getattr(stream, "device", None)
+    if device is not None and isinstance(t, torch.Tensor) and device != t.device:
+        raise ValueError(f"a stream of {device} for tensors on {t.device}")
+    return stream.cuda_stream
+
+
 def _call(name: str, args) -> None:
     L, err = _lib.load(), C.create_string_buffer(256)
     st = getattr(L, name)(C.byref(args), int(torch.cuda.current_stream().cuda_stream), err, len(err))
@@ -157,7 +168,7 @@ def block_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post
     ``out_dtype``; ``out`` takes it and may be ``residual`` itself.
     """
     r = (_native or _load()).block_norm(y, residual, post_weight, next_weight, gate, _GATES.get(gate_act, -1), eps, weight_offset,
-                                      residual_scale, block_scale, out, out_dtype, normed_dtype, None if stream is None else stream.cuda_stream)
+                                      residual_scale, block_scale, out, out_dtype, normed_dtype, _handle(stream, y))
     if r is not None:
         return r
     a, hidden_dtype, normed_dtype = _block_norm_args(y, residual, post_weight, next_weight, gate, gate_act, eps, weight_offset,
@@ -237,7 +248,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     outside [0, adapters), such as -1, has no adapter.  Ranks of 1 to 128; sums are fp32 and no activation is rounded on
     the way.  Returns ``out``, of ``y``'s type, which may be ``y`` itself.
     """
-    r = (_native or _load()).lora(0, y, x, a, b, ids, scale, None, out, None if stream is None else stream.cuda_stream)
+    r = (_native or _load()).lora(0, y, x, a, b, ids, scale, None, out, _handle(stream, ids))
     if r is not None:
         return r
     args = _lora_args(ids, x=x, a=a, y=y, b=b, scale=scale, out=out)
@@ -252,7 +263,7 @@ def lora_shrink(x: torch.Tensor, a: torch.Tensor, ids: torch.Tensor, *, stream=N
     """The first half of :func:`lora_add`, ``a[ids[t]] @ x[t]`` as fp32 [m, rank], for a projection whose K is sharded: each
     rank shrinks its slice of ``x`` with its slice of ``a``, ``Endpoint.allreduce_`` adds the ranks' rows up, and
     :func:`lora_expand` follows.  Rows of tokens without an adapter are zeros."""
-    r = (_native or _load()).lora(1, None, x, a, None, ids, None, None, None, None if stream is None else stream.cuda_stream)
+    r = (_native or _load()).lora(1, None, x, a, None, ids, None, None, None, _handle(stream, ids))
     if r is not None:
         return r
     args = _lora_args(ids, x=x, a=a)
@@ -266,7 +277,7 @@ def lora_shrink(x: torch.Tensor, a: torch.Tensor, ids: torch.Tensor, *, stream=N
 def lora_expand(y: torch.Tensor, shrunk: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, scale: Optional[torch.Tensor] = None, *,
                 out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """The second half of :func:`lora_add`: ``out[t] = y[t] + scale[i] * b[i] @ shrunk[t]`` with ``i = ids[t]``."""
-    r = (_native or _load()).lora(2, y, None, None, b, ids, scale, shrunk, out, None if stream is None else stream.cuda_stream)
+    r = (_native or _load()).lora(2, y, None, None, b, ids, scale, shrunk, out, _handle(stream, ids))
     if r is not None:
         return r
     args = _lora_args(ids, y=y, b=b, scale=scale, shrunk=shrunk, out=out)
@@ -315,7 +326,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     [0, vocab), such as -1 for padding, is none: log probability 0, rank -1.  A row that is masked whole has log
     probability -inf and entropy 0; NaN or +inf in a row make its log probabilities and entropy NaN.
     """
-    r = (_native or _load()).token_logprobs(logits, tokens, top, None if stream is None else stream.cuda_stream)
+    r = (_native or _load()).token_logprobs(logits, tokens, top, _handle(stream, logits))
     if r is not None:
         return tuple.__new__(TokenLogprobs, r)
     a = _token_logprobs_args(logits, tokens, top)
