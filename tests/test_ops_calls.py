@@ -41,3 +41,16 @@ def test_a_stream_of_another_device_is_refused(name):
     with pytest.raises(ValueError, match="stream of cuda:1"):
         f(**args, stream=s)
     assert not s.used
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_what_is_no_tensor_is_a_type_error(name):
+    f, args = next((f, a) for n, f, a in calls() if n == name)
+    for missing in args:
+        for value in (None, [1.0, 2.0]):
+            with pytest.raises(TypeError, match=missing):
+                f(**{**args, missing: value})
+    for more in {"block_norm": ("residual", "post_weight", "next_weight", "gate", "out"), "lora_add": ("scale", "out"),
+                 "lora_expand": ("scale", "out")}.get(name, ()):
+        with pytest.raises(TypeError, match=more):
+            f(**{**args, more: [1.0, 2.0]})

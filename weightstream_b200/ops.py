@@ -50,6 +50,12 @@ def _vector(t: torch.Tensor, name: str, n: int, dtype=None) -> None:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
 
 
+def _tensors(optional: bool = False, **given) -> None:
+    for name, t in given.items():
+        if not isinstance(t, torch.Tensor) and not (optional and t is None):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+
+
 def _same_device(first: torch.Tensor, *others) -> None:
     for t in others:
         if t is not None and t.device != first.device:
@@ -171,6 +177,8 @@ def block_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post
                                       residual_scale, block_scale, out, out_dtype, normed_dtype, _handle(stream, y))
     if r is not None:
         return r
+    _tensors(y=y)
+    _tensors(True, residual=residual, post_weight=post_weight, next_weight=next_weight, gate=gate, out=out)
     a, hidden_dtype, normed_dtype = _block_norm_args(y, residual, post_weight, next_weight, gate, gate_act, eps, weight_offset,
                                                      residual_scale, block_scale, out, out_dtype, normed_dtype)
     with _on(y.device, stream):
@@ -251,6 +259,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     r = (_native or _load()).lora(0, y, x, a, b, ids, scale, None, out, _handle(stream, ids))
     if r is not None:
         return r
+    _tensors(y=y, x=x, a=a, b=b, ids=ids)
+    _tensors(True, scale=scale, out=out)
     args = _lora_args(ids, x=x, a=a, y=y, b=b, scale=scale, out=out)
     with _on(y.device, stream):
         out = out if out is not None else torch.empty((args.m, args.n), dtype=y.dtype, device=y.device)
@@ -266,6 +276,7 @@ def lora_shrink(x: torch.Tensor, a: torch.Tensor, ids: torch.Tensor, *, stream=N
     r = (_native or _load()).lora(1, None, x, a, None, ids, None, None, None, _handle(stream, ids))
     if r is not None:
         return r
+    _tensors(x=x, a=a, ids=ids)
     args = _lora_args(ids, x=x, a=a)
     with _on(x.device, stream):
         shrunk = torch.empty((args.m, args.rank), dtype=torch.float32, device=x.device)
@@ -280,6 +291,8 @@ def lora_expand(y: torch.Tensor, shrunk: torch.Tensor, b: torch.Tensor, ids: tor
     r = (_native or _load()).lora(2, y, None, None, b, ids, scale, shrunk, out, _handle(stream, ids))
     if r is not None:
         return r
+    _tensors(y=y, shrunk=shrunk, b=b, ids=ids)
+    _tensors(True, scale=scale, out=out)
     args = _lora_args(ids, y=y, b=b, scale=scale, shrunk=shrunk, out=out)
     with _on(y.device, stream):
         out = out if out is not None else torch.empty((args.m, args.n), dtype=y.dtype, device=y.device)
@@ -329,6 +342,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     r = (_native or _load()).token_logprobs(logits, tokens, top, _handle(stream, logits))
     if r is not None:
         return tuple.__new__(TokenLogprobs, r)
+    _tensors(logits=logits, tokens=tokens)
     a = _token_logprobs_args(logits, tokens, top)
     with _on(logits.device, stream):
         new = lambda *shape, dtype: torch.empty(shape, dtype=dtype, device=logits.device)
