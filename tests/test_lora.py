@@ -371,3 +371,39 @@ def test_an_infinite_activation_is_infinite_at_any_rank(dev, rank, m, xt):
         if m > 1:
             assert (got[m // 2] == float("inf")).all() and (got[m - 1] == -float("inf")).all()
         assert (~torch.isfinite(got).all(1)).nonzero().squeeze(1).tolist() == ([m // 2, m - 1] if m > 1 else [0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", [8, 32, 64, 128])
+@pytest.mark.parametrize("xt", [F32, BF16])
+def test_a_table_that_is_hardly_used(dev, rank, xt):
+    """A sorted batch is worked on by the tiles that it has, not by those that its table has adapters for: the same bits
+    with a few adapters and with many more that no token names."""
+    from weightstream_b200 import ops
+    rng = np.random.default_rng(rank)
+    m, k, n = 600, 2304, 72
+    x, y = make(rng, (m, k), xt, dev), make(rng, (m, n), F32, dev)
+    a, b = make(rng, (16, rank, k), BF16, dev, k ** -0.5), make(rng, (16, n, rank), BF16, dev, 0.3)
+    few = torch.from_numpy(rng.integers(0, 16, m).astype(np.int32)).to(dev)
+    many_a, many_b = torch.zeros((900, rank, k), dtype=BF16, device=dev), torch.zeros((900, n, rank), dtype=BF16, device=dev)
+    many_a[::60][:15], many_b[::60][:15] = a[:15], b[:15]
+    many_a[899], many_b[899] = a[15], b[15]
+    many = torch.where(few == 15, 899, few * 60).to(torch.int32)
+    for ids, far in ((few, many), (torch.full_like(few, 15), torch.full_like(few, 899))):
+        s, se, out, err = ref(y, x, a, b, ids, None)
+        t = ops.lora_shrink(x, many_a, far)
+        close(t, s, se)
+        close(ops.lora_add(y, x, many_a, many_b, far), out, err)
+        assert torch.equal(t, ops.lora_shrink(x, a, ids))
+        assert torch.equal(ops.lora_add(y, x, many_a, many_b, far), ops.lora_add(y, x, a, b, ids))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank,k,xt", [(16, 2305, BF16), (32, 2304, F32), (64, 2304, BF16), (128, 1000, F32)])
+@pytest.mark.parametrize("used", [1, 18, 19, 37, 38, 74, 75, 148, 149, 600])
+def test_sorted_batches_of_any_number_of_tiles(dev, rank, k, xt, used):
+    """Both sides of every number of tiles at which the work is split in another way: a tile an adapter here."""
+    m = 601
+    order = torch.from_numpy(np.random.default_rng(used).permutation(m).astype(np.int32)).to(dev)
+    check(dev, m, k, 8, rank, 640, xt=xt, ids=order % used * (640 // used))
+    check(dev, m, k, 8, rank, used, xt=xt, ids=torch.where(order < 40, -1, order % used).to(torch.int32))

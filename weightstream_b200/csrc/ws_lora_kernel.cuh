@@ -50,7 +50,7 @@ struct LoraParams {
     // sorted batches
     int32_t *tiles_count, *perm;
     LoraTile *tiles;
-    int32_t tile, skip_none;
+    int32_t tile, skip_none, most;   // most: the first product's largest cut, as a power of two
 };
 
 __device__ __forceinline__ int lora_id(const LoraParams &p, int t) {
@@ -599,35 +599,51 @@ __device__ __forceinline__ void lora_take8(uint32_t dst, const char *src, int le
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-// S = A x^T of a tile, K cut over the blocks of a cluster.  Eight warps: two halves of the tokens, four steps of 32 of a
-// stage's K.  Rows lie in shared memory as in global memory, their 16-byte pieces swapped by the row's last three bits so
-// that the eight rows of a matrix lie in different banks.
+// Into how many parts K of a tile is cut, as a power of two: as many as let all blocks run at once.  The tiles are known on
+// the device alone: with the cut of all tiles that a table of 200 adapters can give, one request's 600 tokens at rank 64
+// and K 8192 took 45 us, with that of its own 10 tiles 14; 600 tokens of 200 adapters 71 and 70 us.
+__host__ __device__ __forceinline__ int lora_shrink_cut(int tiles, int most, int at_once) {
+    int cut = 0;
+    while (cut < most && tiles <= at_once >> (cut + 1)) ++cut;
+    return cut;
+}
+template <int RT, bool XF32, bool VEC>
+constexpr int kShrinkBlocks = RT == 1 || (VEC && (RT == 2 || (RT == 4 && !XF32))) ? 2 : 1;   // an SM (registers)
+
+// S = A x^T of a tile, K cut over blocks of a cluster, which holds as many tiles as the cut leaves room for.  Eight warps:
+// two halves of the tokens, four steps of 32 of a stage's K.  Rows lie in shared memory as in global memory, their 16-byte
+// pieces swapped by the row's last three bits so that the eight rows of a matrix lie in different banks.
 // VEC: rows of x and A are 16-byte aligned.  Else their values are copied one by one, bf16 ones through registers.
 template <int RT, bool XF32, bool VEC>
-__global__ void __launch_bounds__(kLoraThreads, VEC && (RT <= 2 || (RT == 4 && !XF32)) ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
+__global__ void __launch_bounds__(kLoraThreads, kShrinkBlocks<RT, XF32, VEC>) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
     namespace cg = cooperative_groups;
     using S = ShrinkShape<RT, XF32>;
     extern __shared__ __align__(128) uint8_t lora_smem[];
     float *const got = reinterpret_cast<float *>(lora_smem + S::kRing);   // [block][kSums / C]: this block's share of all blocks' sums
     __shared__ int32_t toks[kSortTokens];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3, kg = warp & 3, half = warp >> 2;
-    const int C = p.cluster, part = blockIdx.x % C, tile = blockIdx.x / C;
     cg::cluster_group cl = cg::this_cluster();
-    if (C > 1) cl.barrier_arrive();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     wait_predecessor();
-    if (tile >= *p.tiles_count) return;
-    const LoraTile q = p.tiles[tile];
+    const int own = 31 - __clz(p.cluster);
+    LoraTile q = p.tiles[blockIdx.x >> own];            // (the tile if the cut is the cluster's, asked for beside the count)
+    const int count = *p.tiles_count, cut = lora_shrink_cut(count, p.most, 148 * kShrinkBlocks<RT, XF32, VEC>), C = 1 << cut;
+    if ((cut == 0) != (own == 0)) return;               // the other launch's batch
+    const int tile = blockIdx.x >> cut, part = blockIdx.x & (C - 1), rank0 = blockIdx.x & (p.cluster - 1) & -C;   // rank0: the tile's first block in the cluster
+    // (a tile's blocks leave here together; a cluster's meetings do not wait for blocks that have left)
+    if (tile >= count) return;
+    if (cut != own) q = p.tiles[tile];
     if (tid < kSortTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
     __syncthreads();
     if (q.adapter < 0) {
         lora_none<true>(p, toks, kSortTokens, part, C);
         return;
     }
+    if (C > 1) cl.barrier_arrive();  // waited for before another block's shared memory is written
     // What this thread copies: one 16-byte column of every sixteenth row (of x in fp32: of every eighth).  Places without a
     // token and ranks behind the last one read the first's; nothing of them is stored.
     constexpr int XP = XF32 ? 32 : 16, XR = kLoraThreads / XP, XN = kSortTokens / XR, xe = XF32 ? 4 : 8;
-    const int steps = (p.k + kSortK - 1) / kSortK, s0 = (int)((int64_t)steps * part / C), s1 = (int)((int64_t)steps * (part + 1) / C);
+    const int steps = (p.k + kSortK - 1) / kSortK, s0 = steps * part >> cut, s1 = steps * (part + 1) >> cut;
     const int xc = tid % XP, ac = tid % 16;
     const char *xsrc[XN], *asrc[RT];
 #pragma unroll
@@ -724,13 +740,13 @@ __global__ void __launch_bounds__(kLoraThreads, VEC && (RT <= 2 || (RT == 4 && !
             for (int j = 0; j < RT * 16; ++j) acc[j / 16][j / 4 % 4][j % 4] += at[j * 32];
     }
     // every block of the cluster adds one share of the sums up
-    const int share = S::kSums / C;
+    const int share = S::kSums >> cut;
     if (C > 1) cl.barrier_wait();
     if (kg == 0)
 #pragma unroll
         for (int j = 0; j < RT * 16; ++j) {
             const int at = half * kMine + j * 32 + lane, c = at / share;
-            (C > 1 ? cl.map_shared_rank(got, c) : got)[part * share + at - c * share] = acc[j / 16][j / 4 % 4][j % 4];
+            (C > 1 ? cl.map_shared_rank(got, rank0 + c) : got)[part * share + at - c * share] = acc[j / 16][j / 4 % 4][j % 4];
         }
     if (C > 1) cl.sync();
     else __syncthreads();

@@ -137,14 +137,30 @@ ws_status_t launch_lora(const Err &err, int nt, bool xf32, bool vec, unsigned ti
 }
 
 template <int RT, bool XF32, bool VEC>
-ws_status_t launch_shrink(const Err &err, unsigned tiles, void *stream, const LoraParams &p) {
+ws_status_t launch_shrink(const Err &err, unsigned tiles, void *stream, LoraParams &p) {
     constexpr auto k = lora_shrink_kernel<RT, XF32, VEC>;
-    constexpr int smem = ShrinkShape<RT, XF32>::kSmem;
-    const ws_status_t st = allow_smem<k>(err, smem);
-    return st != WS_OK ? st : launch(err, k, dim3(tiles * (unsigned)p.cluster), kLoraThreads, smem, (unsigned)p.cluster, stream, p);
+    constexpr int smem = ShrinkShape<RT, XF32>::kSmem, at_once = 148 * kShrinkBlocks<RT, XF32, VEC>;
+    // The device cuts K by the tiles that there are (lora_shrink_cut).  A cluster has the blocks of the largest cut, which is
+    // that of all tiles that there can be, or of twice the fewest where a table has adapters for more.  A batch that may
+    // have too many tiles for a cut gets a launch without clusters beside, and one of the two finds its work: blocks of
+    // clusters of eight that each take a tile are placed worse (1000 tokens of 500 adapters, rank 128, 314 us; alone 242).
+    const int fewest = (p.m + kSortTokens - 1) / kSortTokens, usual = std::min((int)tiles, 2 * fewest);
+    p.most = 0;
+    while (p.most < 3 && usual << p.most < 148 && p.k >> (p.most + 1) >= 2 * kSortK) ++p.most;
+    ws_status_t st = allow_smem<k>(err, smem);
+    if (st == WS_OK && p.most > 0) {
+        p.cluster = 1 << p.most;
+        const unsigned blocks = std::min(tiles << p.most, (unsigned)at_once), clusters = (blocks + p.cluster - 1) / p.cluster;
+        st = launch(err, k, dim3(clusters * p.cluster), kLoraThreads, smem, (unsigned)p.cluster, stream, p);
+    }
+    if (st == WS_OK && (p.most == 0 || (int)tiles > at_once / 2)) {
+        p.cluster = 1;
+        st = launch(err, k, dim3(tiles), kLoraThreads, smem, 1, stream, p);
+    }
+    return st;
 }
 template <int RT>
-ws_status_t launch_shrink(const Err &err, bool xf32, bool vec, unsigned tiles, void *stream, const LoraParams &p) {
+ws_status_t launch_shrink(const Err &err, bool xf32, bool vec, unsigned tiles, void *stream, LoraParams &p) {
     if (vec) return xf32 ? launch_shrink<RT, true, true>(err, tiles, stream, p) : launch_shrink<RT, false, true>(err, tiles, stream, p);
     return xf32 ? launch_shrink<RT, true, false>(err, tiles, stream, p) : launch_shrink<RT, false, false>(err, tiles, stream, p);
 }
@@ -226,9 +242,6 @@ ws_status_t lora(Lora what, const ws_lora_args_t *a, void *stream, char *err_tex
                 LoraParams q = p;
                 if (expands) q.s_out = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + need) - (int64_t)a->m * a->rank;
                 p.s_in = expands ? q.s_out : nullptr;
-                // K is cut until the blocks fill the card twice
-                q.cluster = 1;
-                while (q.cluster < 8 && (int64_t)tiles * q.cluster < 148 && a->k / (2 * q.cluster) >= 2 * kSortK) q.cluster *= 2;
                 q.skip_none = 0;
                 st = rt == 1 ? launch_shrink<1>(err, xf32, vec_k, tiles, stream, q) : rt == 2 ? launch_shrink<2>(err, xf32, vec_k, tiles, stream, q)
                      : rt == 4 ? launch_shrink<4>(err, xf32, vec_k, tiles, stream, q) : launch_shrink<8>(err, xf32, vec_k, tiles, stream, q);
