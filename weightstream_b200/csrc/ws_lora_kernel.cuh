@@ -48,7 +48,7 @@ struct LoraParams {
     int32_t m, k, n, r, adapters;
     int32_t y_dtype, cluster;
     // sorted batches
-    int32_t *tiles_count, *perm;
+    int32_t *tiles_count, *perm;   // tiles_count: of all tiles, of those of an adapter
     LoraTile *tiles;
     int32_t tile, skip_none, most;   // most: the first product's largest cut, as a power of two
 };
@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(const __grid_constant__
         const int c = count[b];
         first[b] = before_tok;
         tile0[b] = before_til;
+        if (b == p.adapters) p.tiles_count[1] = before_til;
         before_tok += c;
         if (b < p.adapters || !p.skip_none) before_til += (c + p.tile - 1) / p.tile;
     }
@@ -626,13 +627,16 @@ __global__ void __launch_bounds__(kLoraThreads, kShrinkBlocks<RT, XF32, VEC>) lo
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     wait_predecessor();
     const int own = 31 - __clz(p.cluster);
-    LoraTile q = p.tiles[blockIdx.x >> own];            // (the tile if the cut is the cluster's, asked for beside the count)
-    const int count = *p.tiles_count, cut = lora_shrink_cut(count, p.most, 148 * kShrinkBlocks<RT, XF32, VEC>), C = 1 << cut;
+    LoraTile q = p.tiles[blockIdx.x >> own];            // (the tile if the cut is the cluster's, asked for beside the counts)
+    const int count = p.tiles_count[0], served = p.tiles_count[1], cut = lora_shrink_cut(served, p.most, 148 * kShrinkBlocks<RT, XF32, VEC>);
     if ((cut == 0) != (own == 0)) return;               // the other launch's batch
-    const int tile = blockIdx.x >> cut, part = blockIdx.x & (C - 1), rank0 = blockIdx.x & (p.cluster - 1) & -C;   // rank0: the tile's first block in the cluster
+    // tiles of an adapter first, C blocks each; then, a block each, those of tokens without one
+    const int behind = (int)blockIdx.x - (served << cut), C = behind < 0 ? 1 << cut : 1;
+    const int tile = behind < 0 ? (int)blockIdx.x >> cut : served + behind, part = blockIdx.x & (C - 1);
+    const int rank0 = (blockIdx.x & (p.cluster - 1)) - part;   // the tile's first block in the cluster
     // (a tile's blocks leave here together; a cluster's meetings do not wait for blocks that have left)
     if (tile >= count) return;
-    if (cut != own) q = p.tiles[tile];
+    if (tile != (int)(blockIdx.x >> own)) q = p.tiles[tile];
     if (tid < kSortTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
     __syncthreads();
     if (q.adapter < 0) {

@@ -150,7 +150,7 @@ ws_status_t launch_shrink(const Err &err, unsigned tiles, void *stream, LoraPara
     ws_status_t st = allow_smem<k>(err, smem);
     if (st == WS_OK && p.most > 0) {
         p.cluster = 1 << p.most;
-        const unsigned blocks = std::min(tiles << p.most, (unsigned)at_once), clusters = (blocks + p.cluster - 1) / p.cluster;
+        const unsigned blocks = std::min(tiles << p.most, (unsigned)(at_once + fewest)), clusters = (blocks + p.cluster - 1) / p.cluster;
         st = launch(err, k, dim3(clusters * p.cluster), kLoraThreads, smem, (unsigned)p.cluster, stream, p);
     }
     if (st == WS_OK && (p.most == 0 || (int)tiles > at_once / 2)) {
