@@ -630,19 +630,19 @@ __global__ void __launch_bounds__(kLoraThreads, kShrinkBlocks<RT, XF32, VEC>) lo
     LoraTile q = p.tiles[blockIdx.x >> own];            // (the tile if the cut is the cluster's, asked for beside the counts)
     const int count = p.tiles_count[0], served = p.tiles_count[1], cut = lora_shrink_cut(served, p.most, 148 * kShrinkBlocks<RT, XF32, VEC>);
     if ((cut == 0) != (own == 0)) return;               // the other launch's batch
-    // tiles of an adapter first, C blocks each; then, a block each, those of tokens without one
-    const int behind = (int)blockIdx.x - (served << cut), C = behind < 0 ? 1 << cut : 1;
-    const int tile = behind < 0 ? (int)blockIdx.x >> cut : served + behind, part = blockIdx.x & (C - 1);
-    const int rank0 = (blockIdx.x & (p.cluster - 1)) - part;   // the tile's first block in the cluster
-    // (a tile's blocks leave here together; a cluster's meetings do not wait for blocks that have left)
-    if (tile >= count) return;
-    if (tile != (int)(blockIdx.x >> own)) q = p.tiles[tile];
+    const int behind = (int)blockIdx.x - (served << cut);
+    if (behind >= 0) {  // behind the tiles of an adapter, a block each, those of tokens without one
+        if (served + behind >= count) return;
+        q = p.tiles[served + behind];
+        if (tid < kSortTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
+        __syncthreads();
+        lora_none<true>(p, toks, kSortTokens, 0, 1);
+        return;             // (a cluster's meetings do not wait for blocks that have left)
+    }
+    const int C = 1 << cut, part = blockIdx.x & (C - 1), rank0 = blockIdx.x & (p.cluster - 1) & -C;   // rank0: the tile's first block in the cluster
+    if (cut != own) q = p.tiles[blockIdx.x >> cut];
     if (tid < kSortTokens) toks[tid] = tid < q.count ? p.perm[q.start + tid] : -1;
     __syncthreads();
-    if (q.adapter < 0) {
-        lora_none<true>(p, toks, kSortTokens, part, C);
-        return;
-    }
     if (C > 1) cl.barrier_arrive();  // waited for before another block's shared memory is written
     // What this thread copies: one 16-byte column of every sixteenth row (of x in fp32: of every eighth).  Places without a
     // token and ranks behind the last one read the first's; nothing of them is stored.
