@@ -230,3 +230,27 @@ def test_c_entry_refuses_widths_that_its_counters_do_not_hold(n):
     assert L.ws_block_norm(C.byref(a), None, err, len(err)) == _lib.WS_ERR_INVALID and b"out of range" in err.value
     a.n = 2 ** 31 - 4097
     assert L.ws_block_norm(C.byref(a), None, err, len(err)) == _lib.WS_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,pad", [(400, 5121, 0), (400, 5120, 1), (297, 2561, 0), (300, 8191, 0), (3, 8193, 0), (3, 9001, 0), (3, 16383, 0),
+                                     (3, 16384, 1), (2, 16385, 0), (3, 16640, 8)])
+def test_values_one_by_one_at_every_width(dev, m, n, pad):
+    """Rows that no vector fits, with eight, sixteen and thirty-two values a thread and with any number of them."""
+    check(dev, m, n, gate="full", act="sigmoid", rt=F32, pad=pad)
+    check(dev, m, n, yt=BF16, rt=BF16, gt=F32, wt=F32, ht=F32, zt=F32, gate="channel", pad=pad)
+    check(dev, m, n, gate="token", post=False, pad=pad)
+    check(dev, m, n, res=False, nxt=False, gate="full", pad=pad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(400, 5121), (3, 9001), (3, 16383), (2, 20001)])
+def test_values_one_by_one_in_place(dev, m, n):
+    from weightstream_b200 import ops
+    rng = np.random.default_rng(m + n)
+    for t in (F32, BF16):
+        y, r, g = make(rng, (m, n), F32, dev), make(rng, (m, n), t, dev), make(rng, (m, n), BF16, dev)
+        w = make(rng, (n,), BF16, dev)
+        h, z = ops.block_norm(y, r, post_weight=w, next_weight=w, gate=g)
+        h2, z2 = ops.block_norm(y, r, post_weight=w, next_weight=w, gate=g, out=r)
+        assert h2 is r and torch.equal(h2, h) and torch.equal(z2, z)

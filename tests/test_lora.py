@@ -407,3 +407,52 @@ def test_sorted_batches_of_any_number_of_tiles(dev, rank, k, xt, used):
     order = torch.from_numpy(np.random.default_rng(used).permutation(m).astype(np.int32)).to(dev)
     check(dev, m, k, 8, rank, 640, xt=xt, ids=order % used * (640 // used))
     check(dev, m, k, 8, rank, used, xt=xt, ids=torch.where(order < 40, -1, order % used).to(torch.int32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,adapters", [(700, 4), (700, 400)])
+def test_a_sorted_batch_on_another_stream_and_in_a_graph(dev, m, adapters):
+    """More than 512 tokens: several launches that overlap, and a workspace that belongs to the call's stream."""
+    from weightstream_b200 import ops
+    rng = np.random.default_rng(30 + adapters)
+    a, b = make(rng, (adapters, 16, 2048), BF16, dev, 0.1), make(rng, (adapters, 128, 16), BF16, dev, 0.1)
+    x, y, ids = make(rng, (m, 2048), BF16, dev), make(rng, (m, 128), F32, dev), batch(rng, m, adapters, dev)
+    want, rows = ops.lora_add(y, x, a, b, ids), ops.lora_shrink(x, a, ids)
+    _, _, out, err = ref(y, x, a, b, ids, None)
+    close(want, out, err)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for _ in range(4):  # (each call's workspace is the one before's, freed on that stream)
+        outs += [ops.lora_add(y, x, a, b, ids, stream=s)]
+        t = ops.lora_shrink(x, a, ids, stream=s)
+        outs += [ops.lora_expand(y, t, b, ids, stream=s)]
+    s.synchronize()
+    assert torch.equal(t, rows) and all(torch.equal(o, want) for o in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.lora_add(y, x, a, b, ids)
+        t = ops.lora_shrink(x, a, ids)
+        halves = ops.lora_expand(y, t, b, ids)
+    for _ in range(2):
+        x.mul_(2.0)
+        ids.copy_(ids.flip(0).clamp(max=adapters // 2))  # other tiles, and fewer
+        g.replay()
+        want = ops.lora_add(y, x, a, b, ids)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(halves, want)
+
+
+@pytest.mark.gpu
+def test_a_sorted_batch_with_the_largest_table(dev):
+    check(dev, 600, 64, 32, 8, 16384)
+    check(dev, 600, 64, 32, 7, 16384, xt=F32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4096, 4097, 4500, 9000])
+@pytest.mark.parametrize("rank", [16, 12])
+def test_more_tokens_than_the_plan_asks_for_at_once(dev, m, rank):
+    check(dev, m, 72, 24, rank, 37)
+    check(dev, m, 72, 24, rank, 3, xt=F32, yt=BF16)
+    check(dev, m, 72, 24, rank, 2, ids=(torch.arange(m, dtype=torch.int32, device=dev) > 4094).to(torch.int32))
