@@ -240,8 +240,9 @@ ws_status_t ws_fp8_gemm_static_scratch_check(int32_t device, void *stream, char 
 /* ---- operators between the steps --------------------------------------------------------------
  * What an engine does between two reduction points, on the tensors that the steps above take and
  * return.  They need no endpoint and run on the calling thread's current device.  Types are
- * WS_ACT_BF16 or WS_ACT_F32, sums and statistics are held in 32 bits.  `err` (optional, err_len bytes)
- * gets the text of an error.  m = 0 launches nothing. */
+ * WS_ACT_BF16 or WS_ACT_F32, sums and statistics are held in 32 bits.  Every tensor, results among them,
+ * is aligned to its type, and widths stay below 2^31 - 4096 (the vocabulary below 2^31 - 65536); else
+ * WS_ERR_INVALID.  `err` (optional, err_len bytes) gets the text of an error.  m = 0 launches nothing. */
 
 /* Norms before and after a block with its gate, residual scale and the residual stream:
  *   u = y, or with post_weight  y * rsqrt(mean(y^2) + eps) * (weight_offset + post_weight)
@@ -295,7 +296,8 @@ ws_status_t ws_token_logprobs(const ws_token_logprobs_args_t *args, void *stream
  * Tokens with an id outside [0, adapters), such as -1, have no adapter: out = y, shrunk rows are zeros.
  * ws_lora_add is the whole; where the projection is sharded over K every rank calls ws_lora_shrink on its slice of x
  * and of a, the ranks add the shrunk rows up (ws_allreduce_f32) and each calls ws_lora_expand.
- * The adapters are bf16, the products' sums and the shrunk rows fp32.  Up to 512 tokens need no workspace; more take
+ * The adapters are bf16 (an infinite weight makes its results infinite or NaN), the products' sums and
+ * the shrunk rows fp32.  Up to 512 tokens need no workspace; more take
  * ws_lora_workspace(m, adapters, rank) bytes (16-byte aligned) that the call writes first, so calls on one stream may share
  * it, and at most 16384 adapters (WS_ERR_CAPACITY beyond). */
 #define WS_LORA_MAX_RANK 128

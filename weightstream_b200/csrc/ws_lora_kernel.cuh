@@ -13,12 +13,15 @@
 // times that where an operand is split, against m (2 k + 8 n) bytes; 4000 rows of rank 64 keep it busy for 30 us and
 // HBM for 47.
 //
-// Bound: latency for few tokens (one row of 8192 x 7168 at rank 16 5.4 us, 64 rows of 24 adapters 10.8 us, of which HBM
+// Bound: latency for few tokens (one row of 8192 x 7168 at rank 16 5.7 us, 64 rows of 24 adapters 9.7 us, of which HBM
 // needs 2.5: finding the tile, two waits for HBM and the blocks' meeting follow one another).  For prompts HBM would be
-// (4000 rows of rank 64: 97 us, 3.2 TB/s, of which the plan takes 9, the first product 29 and the second 60).
+// (4000 rows of rank 64: 96 us, 3.2 TB/s; each by itself on cold caches, the plan takes 9, the first product 29 and the
+// second 63).
 //
 // fp32 operands (x, and S between the products) are split into three bf16 parts that add up to all 24 bits, and each
-// part is multiplied: nothing is rounded to 16 bits but the weights that are stored so.
+// part is multiplied: nothing is rounded to 16 bits but the weights that are stored so.  An infinite activation has no
+// second and third part.  A weight that is not finite makes its results NaN where a part is zero, also those that the
+// definition makes infinite.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -30,8 +33,12 @@ namespace ws {
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
 constexpr int kLoraMaxCluster = 8;
-constexpr int kLoraDirect = 512;             // up to this many tokens a block finds its tile by itself
-constexpr int kLoraMaxAdapters = 16384;      // of a sorted batch: two words of shared memory each
+// Up to this many tokens a block finds its tile by itself.  This form and the sorted one, K 8192, N 7168, us: rank 16, 256
+// tokens of one request 14 and 20, 512 of one 18 and 24, of 24 adapters 27 and 27, of 200 54 and 83; 1024 tokens of one 39
+// and 27, of 24 47 and 35.  At rank 64, 512 tokens of 200 adapters 157 and 196, but 256 of one 32 and 26, 512 of one 54 and
+// 34: few adapters of high rank would be sorted earlier, which a limit on tokens alone does not do.
+constexpr int kLoraDirect = 512;
+constexpr int kLoraMaxAdapters = 16384;      // of a sorted batch: three words of shared memory each, of 227 KB
 
 struct LoraTile {
     int32_t adapter, start, count, pad;      // adapter -1: tokens without one
@@ -602,7 +609,7 @@ __device__ __forceinline__ void lora_take8(uint32_t dst, const char *src, int le
 
 // Into how many parts K of a tile is cut, as a power of two: as many as let all blocks run at once.  The tiles are known on
 // the device alone: with the cut of all tiles that a table of 200 adapters can give, one request's 600 tokens at rank 64
-// and K 8192 took 45 us, with that of its own 10 tiles 14; 600 tokens of 200 adapters 71 and 70 us.
+// and K 8192 took 45 us, with that of its own 10 tiles 17; 600 tokens of 200 adapters 71 with either.
 __host__ __device__ __forceinline__ int lora_shrink_cut(int tiles, int most, int at_once) {
     int cut = 0;
     while (cut < most && tiles <= at_once >> (cut + 1)) ++cut;
@@ -768,7 +775,8 @@ __global__ void __launch_bounds__(kLoraThreads, kShrinkBlocks<RT, XF32, VEC>) lo
 // in fragments, so nothing is moved between registers (with the operands the other way round, four moves a product,
 // 73 us for the 4000 rows of rank 64).  Row 16 q + 4 (c / 2) + 2 i + c % 2 of the 64 is column c of product 2 q + i,
 // which leaves a lane four consecutive outputs of a token.  The y of a step, 16 tokens and 32 rows of B, is requested
-// kAhead steps ahead of its sum.
+// kAhead steps ahead of its sum: four where registers allow it (rank 64, 4000 rows of 7168 66.6 us, with two 67.4), else two
+// (the others spill more with four: rank 16 53 us against 70, rank 32 74 against 87, rank 128 144 against 171).
 template <int RT>
 struct ExpandShape {
     static constexpr int kFragments = 4 * RT;                     // (tokens of 16, ranks of 16)

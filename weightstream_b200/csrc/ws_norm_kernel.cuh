@@ -7,10 +7,11 @@
 // All of it is held in 32 bits between the loads and the one rounding of h and of z to their types; z is taken from the
 // unrounded h.
 //
-// Bound: HBM for many rows (8192 rows of 7168 with a gate a value: 124 us, 5.7 TB/s; a row's two sums are the time in
-// which its block loads nothing, so that several blocks share an SM), the launch for few (one row 2.7 us on the device).
-// Widths that no vector divides load value by value and are bound by those instructions (1503 rows of 2307: 11.0 us,
-// 3.2 TB/s).
+// Bound: HBM for many rows (8192 rows of 7168 with a gate a value: 131 us, 5.4 TB/s, in a graph of such calls 124 us; a
+// row's two sums are the time in which its block loads nothing, so that several blocks share an SM), the launch for few
+// (one row 2.7 us on the device).  Widths that no vector divides load value by value and are bound by those instructions
+// (1503 rows of 2307: 10.3 us, 3.4 TB/s), and so are those beyond 16384, which besides read three times (2048 rows of 18432
+// 256 us, of which HBM would need 58).
 #pragma once
 
 #include <type_traits>

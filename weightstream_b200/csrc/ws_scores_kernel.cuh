@@ -10,9 +10,10 @@
 // the threads whose maximum reaches it (about k threads) are read once more (a row that is one batch still has them in
 // registers), and what is left is ranked in shared memory.
 //
-// Bound: HBM for fp32 rows (2000 rows of 129280: 160 us, 6.46 TB/s), instructions for bf16 ones (117 us, 4.4 TB/s: about
-// ten a value, of which one is the exponential and two keep masked values from giving NaN) and for alternatives (twenty
-// of them: 190 us and 187 us), latency for few rows (one row 9 us, 64 rows 18 us).
+// Bound: HBM for fp32 rows (2000 rows of 129280: 167 us, 6.2 TB/s, in a graph of such calls 163 us), instructions for bf16
+// ones (117 us, 4.4 TB/s: about ten a value, of which one is the exponential and two keep masked values from giving NaN) and
+// for alternatives (twenty of them: 190 us and 187 us; five under a mask of 40 % of the vocabulary 204 us), latency for few
+// rows (one row with twenty alternatives 10 us and without 6, 64 rows with twenty 18 us and without 10).
 //
 // Order of values: larger first, equal ones by index, as argmax has it (crates/weightstream-ref/src/sample.rs:13-23).
 // -inf (masked) and NaN are never alternatives.

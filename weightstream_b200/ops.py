@@ -7,7 +7,8 @@ vocabulary head's logits (:func:`token_logprobs`).
 
 Every function runs on the GPU that holds its tensors, on ``stream`` or the current stream, and does not synchronise.
 Results are allocated on that stream.  A tensor that a call reads has to live until the stream has passed the call, as
-with torch's own operators.  Wrong arguments raise ``TypeError`` or ``ValueError`` before anything is launched.
+with torch's own operators.  Wrong arguments raise ``TypeError`` or ``ValueError``, sizes beyond what a kernel counts
+``WsError``, before anything is launched.  The operators are for serving: a result has no gradient, whatever its inputs ask.
 """
 from __future__ import annotations
 
@@ -170,7 +171,7 @@ def block_norm(y: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post
     ``"sigmoid"``.  ``weight_offset`` is 1 for models that keep their norm weights as a difference from one.  Everything
     between the loads and the results is held in 32 bits; ``normed`` is taken from ``hidden`` before it is rounded.
 
-    Returns ``(hidden, normed)``; ``normed`` is None without ``next_weight``.  ``hidden`` has the residual's type, or
+    Returns ``(hidden, normed)``; ``hidden`` is always written, ``normed`` is None without ``next_weight``.  ``hidden`` has the residual's type, or
     ``out_dtype``; ``out`` takes it and may be ``residual`` itself.
     """
     r = (_native or _load()).block_norm(y, residual, post_weight, next_weight, gate, _GATES.get(gate_act, -1), eps, weight_offset,
@@ -254,7 +255,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     ``x`` [m, k] is what the projection read, ``y`` [m, n] what it returned (bf16 or fp32 each); ``a`` [adapters, rank, k]
     and ``b`` [adapters, n, rank] are bf16, ``scale`` [adapters] fp32, ``ids`` [m] int32 in any order.  A token whose id is
     outside [0, adapters), such as -1, has no adapter.  Ranks of 1 to 128; sums are fp32 and no activation is rounded on
-    the way.  Returns ``out``, of ``y``'s type, which may be ``y`` itself.
+    the way.  With more than 512 tokens a table has at most 16384 adapters; more raise ``WsError`` (the halves alike).
+    Returns ``out``, of ``y``'s type, which may be ``y`` itself.
     """
     r = (_native or _load()).lora(0, y, x, a, b, ids, scale, None, out, _handle(stream, ids))
     if r is not None:
