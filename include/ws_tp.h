@@ -322,6 +322,104 @@ ws_status_t ws_lora_add(const ws_lora_args_t *args, void *stream, char *err, siz
 ws_status_t ws_lora_shrink(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
 ws_status_t ws_lora_expand(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
 
+/* Norms of queries and keys, head by head, and the rotation of positions:
+ *   u = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight)      over a head's d values (norm = 0: u = x * weight)
+ *   a' = scale (a cos - b sin), b' = scale (a sin + b cos)         angle = position * inv_freq[i], for the pairs
+ *   (a, b) = (u[start + i], u[start + pairs + i]), or with interleaved (u[start + 2 i], u[start + 2 i + 1]);
+ * the other values of u stay.  The angle is a product of 64 bits.  pairs = 0: no rotation (positions and inv_freq unused).
+ * q_out and k_out may be q and k themselves.  (Takes the place of the reference's `rmsnorm` and `rope` launches in front of its
+ * attention.) */
+#define WS_MAX_PAIRS 1024
+typedef struct {
+    const void *q, *k;        /* [m, heads, d]; k NULL: queries alone                                       */
+    int64_t ldqt, ldqh, ldkt, ldkh;       /* strides from token to token and head to head (elements)          */
+    void *q_out, *k_out;
+    int64_t ldqt_out, ldqh_out, ldkt_out, ldkh_out;
+    const void *q_weight, *k_weight;      /* [d] or NULL: 1 (without weight_offset)                           */
+    const void *positions;    /* [m] int32 or int64 (position_bytes 4 or 8)                                  */
+    const float *inv_freq;    /* [pairs]                                                                     */
+    int32_t m, q_heads, k_heads, d, pairs, start, interleaved, norm, dtype, weight_dtype, position_bytes;
+    float eps, weight_offset, scale;
+} ws_head_norm_rope_args_t;
+ws_status_t ws_head_norm_rope(const ws_head_norm_rope_args_t *args, void *stream, char *err, size_t err_len);
+
+/* Experts of every token from the gate's logits, in the form that the routed steps read:
+ *   score = softmax(logits), sigmoid(logits) or sqrt(ln(1 + exp(logits)));  key = score + bias (score without one)
+ *   ids = the top_k experts by key, larger first and equal ones by index
+ *   weights = scale * score, with renormalize divided by the sum of the chosen scores
+ * Experts whose logit is -inf or NaN, or whose key is NaN, are never chosen; places that stay empty hold id -1 and weight 0.
+ * The order is that of the definition: near ones are compared in 64 bits.  (Takes the place of the reference's `moe_select`.) */
+enum { WS_SCORE_SOFTMAX = 0, WS_SCORE_SIGMOID = 1, WS_SCORE_SQRTSOFTPLUS = 2 };
+#define WS_ROUTE_MAX_EXPERTS 1024
+#define WS_ROUTE_MAX_TOP_K 32
+typedef struct {
+    const void *logits;       /* [m, experts], row stride ld (elements) */
+    int64_t ld;
+    const float *bias;        /* [experts] or NULL                       */
+    int32_t *ids;             /* [m, top_k]                              */
+    float *weights;           /* [m, top_k]                              */
+    int32_t m, experts, top_k, score, dtype, renormalize;
+    float scale;
+} ws_moe_route_args_t;
+ws_status_t ws_moe_route(const ws_moe_route_args_t *args, void *stream, char *err, size_t err_len);
+
+/* A whole mixture-of-experts layer of a few tokens over MXFP4 experts, in two kernels:
+ *   g = w1[e] x[t], u = w3[e] x[t];  with limit > 0: g = min(g, limit), u = min(max(u, -limit), limit)
+ *   out[t] = sum over t's routes (in the order of their slots) of w2[e] (weight * silu(g) * u)
+ * Weights are packed E2M1 (low nibble = even K) with a UE8M0 byte per 32 values of K, as in ws_moe_down_combine_allreduce,
+ * every expert's rows one after the other; experts lie w1_stride .. s2_stride bytes apart, so W1 and W3 may be halves of one
+ * tensor.  Scale byte 0 counts as 0, 255 gives infinities or NaN.  Routes to experts outside [e_start, e_start + e_len), such as
+ * -1, are other ranks': out then is this rank's part of the sum (ws_allreduce_f32).
+ * Activations are not rounded (act_quant 0), or x and the weighted hidden are rounded as the fused steps do (1).
+ * hidden and inter are multiples of 32; weights, scales and strides are multiples of 16 bytes.
+ * At most 512 routes (m * top_k), 512 local experts, top_k 8 and widths of 24576 (WS_ERR_CAPACITY beyond).  The workspace
+ * (ws_moe_layer_workspace bytes, 16-byte aligned) is written first, so calls on one stream may share it. */
+typedef struct {
+    const void *x;            /* [m, hidden] activations, row stride ldx (elements)  */
+    int64_t ldx;
+    const int32_t *route_ids; /* [m, top_k] global expert ids                        */
+    const float *route_w;     /* [m, top_k]                                          */
+    const uint8_t *w1, *s1;   /* [e_len][inter][hidden/2], [e_len][inter][hidden/32] */
+    const uint8_t *w3, *s3;   /* as w1 and s1                                        */
+    const uint8_t *w2, *s2;   /* [e_len][hidden][inter/2], [e_len][hidden][inter/32] */
+    int64_t w1_stride, s1_stride, w3_stride, s3_stride, w2_stride, s2_stride;
+    void *out;                /* [m, hidden], row stride ldo                         */
+    int64_t ldo;
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t m, hidden, inter, top_k, e_start, e_len, x_dtype, out_dtype, act_quant;
+    float limit;              /* <= 0: none                                          */
+} ws_moe_layer_args_t;
+int64_t ws_moe_layer_workspace(int32_t m, int32_t top_k, int32_t hidden, int32_t inter);
+ws_status_t ws_moe_layer(const ws_moe_layer_args_t *args, void *stream, char *err, size_t err_len);
+
+/* Bias, penalties for repeated tokens and grammar masks on logits, in this order:
+ *   z = logits + bias                              (the row's listed tokens; of a token listed twice the last entry counts)
+ *   z = z > 0 ? z / repetition : z * repetition    where the token occurs in the row's history
+ *   z = z - frequency * count - presence           where count, its occurrences behind the first prompt_lens tokens, is not 0
+ *   z = -inf                                       where the row's mask has no bit for the token
+ * Row t's history is tokens[offsets[t] .. offsets[t + 1]), its biases likewise; offsets outside [0, n_tokens] are taken to its
+ * ends, and tokens outside [0, vocab) ignored.  Bit v % 32 of word v / 32 of a mask allows token v; row t uses mask row
+ * mask_rows[t] (NULL: t), and none if that is outside [0, mask_count).  out may be logits itself. */
+typedef struct {
+    const void *logits;       /* [m, vocab], row stride ld (elements)               */
+    int64_t ld;
+    void *out;                /* [m, vocab] of the logits' type, row stride ldo      */
+    int64_t ldo;
+    const int32_t *tokens;    /* [n_tokens] or NULL: no penalties                    */
+    const void *offsets;      /* [m + 1] int32 or int64 (offset_bytes 4 or 8)        */
+    const int32_t *prompt_lens;                       /* [m] or NULL: 0              */
+    const float *repetition, *frequency, *presence;   /* [m] or NULL: 1, 0, 0        */
+    const int32_t *bias_ids;  /* [n_bias] or NULL: no biases                         */
+    const float *bias;        /* [n_bias]                                            */
+    const void *bias_offsets; /* [m + 1] as offsets                                  */
+    const uint32_t *mask;     /* [mask_count, ld_mask] words or NULL                 */
+    const int32_t *mask_rows; /* [m] or NULL                                         */
+    int64_t n_tokens, n_bias, ld_mask;
+    int32_t m, vocab, mask_count, offset_bytes, bias_offset_bytes, dtype;
+} ws_adjust_logits_args_t;
+ws_status_t ws_adjust_logits(const ws_adjust_logits_args_t *args, void *stream, char *err, size_t err_len);
+
 const char *ws_version(void);
 
 #ifdef __cplusplus

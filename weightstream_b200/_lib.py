@@ -19,6 +19,9 @@ WS_ACT_BF16, WS_ACT_F32 = 0, 1
 WS_GATE_LINEAR, WS_GATE_SIGMOID = 0, 1
 WS_MAX_TOP = 32
 WS_LORA_MAX_RANK = 128
+WS_MAX_PAIRS = 1024
+WS_SCORE_SOFTMAX, WS_SCORE_SIGMOID, WS_SCORE_SQRTSOFTPLUS = 0, 1, 2
+WS_ROUTE_MAX_EXPERTS, WS_ROUTE_MAX_TOP_K = 1024, 32
 
 STATUS_NAMES = {0: "WS_OK", -1: "WS_ERR_INVALID", -2: "WS_ERR_CUDA", -3: "WS_ERR_TIMEOUT",
                 -4: "WS_ERR_SEQUENCE", -5: "WS_ERR_CAPACITY", -6: "WS_ERR_UNSUPPORTED"}
@@ -34,7 +37,8 @@ EXPORTS = [
     "ws_allreduce_f32", "ws_allgather_f32", "ws_allreduce_f32_group", "ws_allgather_f32_group",
     "ws_allreduce_f32_host", "ws_allgather_f32_host", "ws_fp8_rowpar_gemm_allreduce_host",
     "ws_act_quant_fp8", "ws_tp_set_split", "ws_tp_set_kernel", "ws_fp8_gemm_static_scratch", "ws_fp8_gemm_static_scratch_check",
-    "ws_block_norm", "ws_token_logprobs", "ws_lora_workspace", "ws_lora_add", "ws_lora_shrink", "ws_lora_expand", "ws_version",
+    "ws_block_norm", "ws_token_logprobs", "ws_lora_workspace", "ws_lora_add", "ws_lora_shrink", "ws_lora_expand",
+    "ws_head_norm_rope", "ws_moe_route", "ws_moe_layer_workspace", "ws_moe_layer", "ws_adjust_logits", "ws_version",
 ]
 
 
@@ -99,6 +103,44 @@ class LoraArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
                 ("m", C.c_int32), ("k", C.c_int32), ("n", C.c_int32), ("rank", C.c_int32), ("adapters", C.c_int32),
                 ("x_dtype", C.c_int32), ("y_dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class HeadNormRopeArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p),
+                ("ldqt", C.c_int64), ("ldqh", C.c_int64), ("ldkt", C.c_int64), ("ldkh", C.c_int64),
+                ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+                ("ldqt_out", C.c_int64), ("ldqh_out", C.c_int64), ("ldkt_out", C.c_int64), ("ldkh_out", C.c_int64),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("positions", C.c_void_p), ("inv_freq", C.c_void_p),
+                ("m", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("d", C.c_int32), ("pairs", C.c_int32),
+                ("start", C.c_int32), ("interleaved", C.c_int32), ("norm", C.c_int32), ("dtype", C.c_int32),
+                ("weight_dtype", C.c_int32), ("position_bytes", C.c_int32),
+                ("eps", C.c_float), ("weight_offset", C.c_float), ("scale", C.c_float)]
+
+
+class MoeRouteArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("bias", C.c_void_p), ("ids", C.c_void_p), ("weights", C.c_void_p),
+                ("m", C.c_int32), ("experts", C.c_int32), ("top_k", C.c_int32), ("score", C.c_int32), ("dtype", C.c_int32),
+                ("renormalize", C.c_int32), ("scale", C.c_float)]
+
+
+class MoeLayerArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("ldx", C.c_int64), ("route_ids", C.c_void_p), ("route_w", C.c_void_p),
+                ("w1", C.c_void_p), ("s1", C.c_void_p), ("w3", C.c_void_p), ("s3", C.c_void_p), ("w2", C.c_void_p), ("s2", C.c_void_p),
+                ("w1_stride", C.c_int64), ("s1_stride", C.c_int64), ("w3_stride", C.c_int64), ("s3_stride", C.c_int64),
+                ("w2_stride", C.c_int64), ("s2_stride", C.c_int64), ("out", C.c_void_p), ("ldo", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+                ("m", C.c_int32), ("hidden", C.c_int32), ("inter", C.c_int32), ("top_k", C.c_int32), ("e_start", C.c_int32),
+                ("e_len", C.c_int32), ("x_dtype", C.c_int32), ("out_dtype", C.c_int32), ("act_quant", C.c_int32), ("limit", C.c_float)]
+
+
+class AdjustLogitsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("out", C.c_void_p), ("ldo", C.c_int64), ("tokens", C.c_void_p),
+                ("offsets", C.c_void_p), ("prompt_lens", C.c_void_p), ("repetition", C.c_void_p), ("frequency", C.c_void_p),
+                ("presence", C.c_void_p), ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_offsets", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_rows", C.c_void_p),
+                ("n_tokens", C.c_int64), ("n_bias", C.c_int64), ("ld_mask", C.c_int64),
+                ("m", C.c_int32), ("vocab", C.c_int32), ("mask_count", C.c_int32), ("offset_bytes", C.c_int32),
+                ("bias_offset_bytes", C.c_int32), ("dtype", C.c_int32)]
 
 
 _lib = None
@@ -194,8 +236,11 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     L.ws_fp8_gemm_static_scratch_check.argtypes = [C.c_int32, P, C.c_char_p, C.c_size_t]
     L.ws_lora_workspace.restype = C.c_int64
     L.ws_lora_workspace.argtypes = [C.c_int32, C.c_int32, C.c_int32]
+    L.ws_moe_layer_workspace.restype = C.c_int64
+    L.ws_moe_layer_workspace.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32]
     for name, args in (("ws_block_norm", BlockNormArgs), ("ws_token_logprobs", TokenLogprobsArgs), ("ws_lora_add", LoraArgs),
-                       ("ws_lora_shrink", LoraArgs), ("ws_lora_expand", LoraArgs)):
+                       ("ws_lora_shrink", LoraArgs), ("ws_lora_expand", LoraArgs), ("ws_head_norm_rope", HeadNormRopeArgs),
+                       ("ws_moe_route", MoeRouteArgs), ("ws_moe_layer", MoeLayerArgs), ("ws_adjust_logits", AdjustLogitsArgs)):
         getattr(L, name).restype = st
         getattr(L, name).argtypes = [C.POINTER(args), P, C.c_char_p, C.c_size_t]
     _lib = L

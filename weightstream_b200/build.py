@@ -11,9 +11,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libws_tp.so")
 TORCH_EXT = os.path.join(HERE, "_ws_torch.so")
-SOURCES = ["ws_api.cu", "ws_bootstrap.cu", "ws_ops.cu"]
+SOURCES = ["ws_api.cu", "ws_bootstrap.cu", "ws_ops.cu", "ws_step_ops.cu"]
 HEADERS = ["ws_device.cuh", "ws_fp8_kernel.cuh", "ws_fp8_gemv_kernel.cuh", "ws_fp8_bs_kernel.cuh", "ws_fp8_tile_kernel.cuh", "ws_moe_kernel.cuh", "ws_moe_gemv_kernel.cuh", "ws_moe_bs_kernel.cuh", "ws_misc_kernels.cuh",
-           "ws_norm_kernel.cuh", "ws_scores_kernel.cuh", "ws_lora_kernel.cuh",
+           "ws_norm_kernel.cuh", "ws_scores_kernel.cuh", "ws_lora_kernel.cuh", "ws_ops_host.cuh", "ws_values.cuh",
+           "ws_heads_kernel.cuh", "ws_route_kernel.cuh", "ws_layer_kernel.cuh", "ws_adjust_kernel.cuh",
            os.path.join("..", "..", "include", "ws_tp.h")]
 
 

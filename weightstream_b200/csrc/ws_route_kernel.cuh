@@ -1,0 +1,198 @@
+// Experts of every token from the gate's logits: the top_k by  key = score + bias  (score alone without one), larger
+// first and equal ones by index, and their weights  scale * score  or  scale * score / sum of the chosen scores.
+//
+//   score = softmax(l), sigmoid(l) or sqrt(ln(1 + e^l))
+//
+// A warp takes a token, its logits in registers.  Without a bias the order is that of the logits themselves.  With one,
+// keys are compared in 32 bits first; where two neighbours of the order lie as close as their errors, the candidates'
+// keys are taken again in 64 bits, so that the choice is the definition's and not that of a rounding.
+// Experts whose logit is -inf or NaN are never chosen; places that stay empty hold id -1 and weight 0.
+#pragma once
+
+#include "ws_values.cuh"
+
+namespace ws {
+
+constexpr int kRouteThreads = 128;
+static_assert(WS_ROUTE_MAX_TOP_K == 32 && WS_ROUTE_MAX_EXPERTS <= 32 * 32, "a lane keeps one result, and 32 logits");
+constexpr float kRouteNear = 4e-6f;     // keys whose difference is below this share of theirs: compared in 64 bits
+
+struct RouteParams {
+    const void *logits;
+    const float *bias;                  // [experts] or null
+    int64_t ld;
+    int32_t *ids;
+    float *weights;
+    int32_t m, experts, top_k, score, dtype, renormalize;
+    float scale;
+};
+
+// Larger floats have larger keys; 0 stands for what is never chosen.
+__device__ __forceinline__ uint32_t route_order(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float route_unorder(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+
+__device__ __forceinline__ float route_score(float l, int kind) {
+    if (kind == WS_SCORE_SIGMOID) return l >= 0.0f ? 1.0f / (1.0f + expf(-l)) : expf(l) / (1.0f + expf(l));
+    return sqrtf(l > 0.0f ? l + log1pf(expf(-l)) : log1pf(expf(l)));
+}
+__device__ __forceinline__ double route_score64(double l, int kind) {
+    if (kind == WS_SCORE_SIGMOID) return l >= 0.0 ? 1.0 / (1.0 + exp(-l)) : exp(l) / (1.0 + exp(l));
+    return sqrt(l > 0.0 ? l + log1p(exp(-l)) : log1p(exp(l)));
+}
+
+template <int N>  // logits a lane
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteParams p) {
+    const int t = blockIdx.x * (kRouteThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_predecessor();
+    if (t >= p.m) return;
+    const int64_t row = (int64_t)t * p.ld;
+    const bool soft = p.score == WS_SCORE_SOFTMAX;
+    float l[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) l[i] = i * 32 + lane < p.experts ? load1(p.logits, p.dtype, row + i * 32 + lane) : -__builtin_huge_valf();
+    // softmax over all experts, where its values themselves count
+    float top = -__builtin_huge_valf(), total = 1.0f;
+    if (soft && (p.bias || !p.renormalize)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = fmaxf(top, l[i]);     // (a NaN counts as nothing)
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) total += l[i] > -__builtin_huge_valf() ? expf(l[i] - top) : 0.0f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    uint32_t key[N];
+    bool fine = true;                   // no two neighbours of the order are too close
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = i * 32 + lane;
+        float k = l[i];
+        if (p.bias && e < p.experts) k = (soft ? expf(l[i] - top) / total : route_score(l[i], p.score)) + p.bias[e];
+        key[i] = l[i] > -__builtin_huge_valf() && k == k ? route_order(k + 0.0f) : 0u;     // (+ 0: -0 and 0 are one)
+    }
+    // ---- rounds: the largest key left, of the lowest index
+    int mine = -1;                      // lane j: the j-th expert
+    float mine_l = 0.0f;
+    float before = __builtin_huge_valf(), last = 0.0f;
+    const int rounds = p.top_k + (p.bias ? 1 : 0);      // one more: how close the first that is left out comes
+    uint32_t best = 0u;
+    int best_i = 0;
+    uint32_t gone = 0u;                 // of this lane's logits
+    auto look = [&]() {
+        best = 0u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool better = !(gone >> i & 1u) && key[i] > best;
+            best = better ? key[i] : best;
+            best_i = better ? i : best_i;
+        }
+    };
+    look();
+    for (int j = 0; j < rounds; ++j) {
+        const uint32_t k = __reduce_max_sync(0xffffffffu, best);
+        if (!k) break;
+        const int e = __reduce_min_sync(0xffffffffu, best == k ? best_i * 32 + lane : 0x7fffffff);
+        if (p.bias) {
+            const float v = route_unorder(k);
+            if (j && before - v <= kRouteNear * fmaxf(1.0f, fabsf(v))) fine = false;
+            before = v;
+        }
+        if (j == p.top_k) break;
+        last = before;
+        float chosen = 0.0f;
+        if ((e & 31) == lane) {
+            gone |= 1u << (e >> 5);
+#pragma unroll
+            for (int i = 0; i < N; ++i) chosen = i == e >> 5 ? l[i] : chosen;
+            look();
+        }
+        chosen = __shfl_sync(0xffffffffu, chosen, e & 31);
+        if (lane == j) {
+            mine = e;
+            mine_l = chosen;
+        }
+    }
+    if (p.bias && !fine) {              // (all lanes alike; rare, so the logits are read again)
+        const float bound = last - kRouteNear * fmaxf(1.0f, fabsf(last));
+        auto logit = [&](int i) { return i * 32 + lane < p.experts ? load1(p.logits, p.dtype, row + i * 32 + lane) : -__builtin_huge_valf(); };
+        double total64 = 1.0;
+        if (soft) {
+            total64 = 0.0;
+#pragma unroll 1
+            for (int i = 0; i < N; ++i) {
+                const float v = logit(i);
+                total64 += v > -__builtin_huge_valf() ? exp((double)v - (double)top) : 0.0;
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) total64 += __shfl_xor_sync(0xffffffffu, total64, o);
+        }
+        uint32_t close = 0u;            // this lane's candidates
+#pragma unroll
+        for (int i = 0; i < N; ++i) close |= key[i] && route_unorder(key[i]) >= bound ? 1u << i : 0u;
+#pragma unroll 1
+        for (int j = 0; j < p.top_k; ++j) {
+            double bk = -__builtin_huge_val();
+            int bi = -1;
+            float bl = 0.0f;
+            for (uint32_t left = close; left; left &= left - 1) {
+                const int i = __ffs(left) - 1;
+                const float v = logit(i);
+                const double k = (soft ? exp((double)v - (double)top) / total64 : route_score64(v, p.score)) + (double)p.bias[i * 32 + lane];
+                if (bi < 0 || k > bk) { bk = k; bi = i * 32 + lane; bl = v; }
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const double ok = __shfl_xor_sync(0xffffffffu, bk, o);
+                const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+                const float ol = __shfl_xor_sync(0xffffffffu, bl, o);
+                if (oi >= 0 && (bi < 0 || ok > bk || (ok == bk && oi < bi))) { bk = ok; bi = oi; bl = ol; }
+            }
+            if (bi < 0) break;
+            if ((bi & 31) == lane) close &= ~(1u << (bi >> 5));
+            if (lane == j) {
+                mine = bi;
+                mine_l = bl;
+            }
+        }
+    }
+    // ---- weights
+    const bool have = mine >= 0;
+    float w = 0.0f, sum = 1.0f;
+    if (soft) {
+        float of = top;
+        if (p.renormalize) {            // a ratio of the chosen: their own maximum will do
+            of = have ? mine_l : -__builtin_huge_valf();
+#pragma unroll
+            for (int o = 16; o; o >>= 1) of = fmaxf(of, __shfl_xor_sync(0xffffffffu, of, o));
+        } else {
+            sum = total;
+        }
+        w = have ? expf(mine_l - of) : 0.0f;
+    } else {
+        w = have ? route_score(mine_l, p.score) : 0.0f;
+    }
+    if (p.renormalize) {
+        sum = w;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (!soft && sum < 1e-30f) {    // scores at the type's end: their ratios in 64 bits
+            double w64 = have ? route_score64(mine_l, p.score) : 0.0, sum64 = w64;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum64 += __shfl_xor_sync(0xffffffffu, sum64, o);
+            w = sum64 > 0.0 ? (float)(w64 / sum64) : 0.0f;
+            sum = 1.0f;
+        }
+    }
+    if (lane < p.top_k) {
+        p.ids[(int64_t)t * p.top_k + lane] = mine;
+        p.weights[(int64_t)t * p.top_k + lane] = have ? p.scale * (w / sum) : 0.0f;
+    }
+}
+
+}  // namespace ws

@@ -491,8 +491,254 @@ PyObject *py_lora(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// A [m, heads, d] tensor with heads' values one after the other; strides from token to token and head to head.
+bool heads(const at::Tensor *t, const at::Tensor &like, int64_t m, int64_t d, int64_t *ldt, int64_t *ldh) {
+    if (!t || t->dim() != 3 || t->size(0) != m || t->size(2) != d || t->device() != like.device() || t->scalar_type() != like.scalar_type()) return false;
+    if ((d > 1 && t->stride(2) != 1) || t->size(1) < 1 || t->size(1) > INT32_MAX) return false;
+    *ldt = m > 1 ? t->stride(0) : t->size(1) * d;
+    *ldh = t->size(1) > 1 ? t->stride(1) : d;
+    return true;
+}
+// A result like it: given, if none of its values is written twice, or made here.
+bool heads_out(PyObject *o, const at::Tensor &like, at::Tensor *made, void **data, int64_t *ldt, int64_t *ldh) {
+    const int64_t m = like.size(0), n = like.size(1), d = like.size(2);
+    if (o == Py_None) {
+        *made = new_like(like, like.sizes(), like.scalar_type());
+        *data = made->data_ptr();
+        *ldt = n * d;
+        *ldh = d;
+        return true;
+    }
+    const at::Tensor *t = tensor(o);
+    if (!heads(t, like, m, d, ldt, ldh) || t->size(1) != n) return false;
+    *data = t->data_ptr();
+    return (*ldh >= d && *ldt >= (n - 1) * *ldh + d) || (*ldt >= d && *ldh >= (m - 1) * *ldt + d);
+}
+
+// head_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, norm, eps, weight_offset, rotary_start, interleaved, rope_scale,
+//                q_out, k_out, stream) -> (q', k' | None)
+PyObject *py_head_norm_rope(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 15) { PyErr_SetString(PyExc_TypeError, "head_norm_rope takes 15 arguments"); return nullptr; }
+    const at::Tensor *q = tensor(v[0]), *k = v[1] == Py_None ? nullptr : tensor(v[1]);
+    if (!q || q->dim() != 3 || (v[1] != Py_None && !k) || (!k && (v[5] != Py_None || v[13] != Py_None))) Py_RETURN_NONE;
+    ws_head_norm_rope_args_t a{};
+    const int64_t m = q->size(0), d = q->size(2);
+    if (m > INT32_MAX || d < 1 || d > INT32_MAX || !act_dtype(*q, &a.dtype) || !heads(q, *q, m, d, &a.ldqt, &a.ldqh)) Py_RETURN_NONE;
+    a.m = (int32_t)m; a.d = (int32_t)d; a.q_heads = (int32_t)q->size(1); a.q = q->data_ptr();
+    if (k) {
+        if (!heads(k, *q, m, d, &a.ldkt, &a.ldkh)) Py_RETURN_NONE;
+        a.k = k->data_ptr();
+        a.k_heads = (int32_t)k->size(1);
+    }
+    const void **weights[2] = {&a.q_weight, &a.k_weight};
+    int32_t seen = -1;
+    for (int i = 0; i < 2; ++i) {
+        if (v[4 + i] == Py_None) continue;
+        const at::Tensor *w = tensor(v[4 + i]);
+        if (!vec(w, *q, d) || !act_dtype(*w, &a.weight_dtype) || (seen >= 0 && seen != a.weight_dtype)) Py_RETURN_NONE;
+        seen = a.weight_dtype;
+        *weights[i] = w->data_ptr();
+    }
+    a.position_bytes = 8;
+    if ((v[2] == Py_None) != (v[3] == Py_None)) Py_RETURN_NONE;
+    a.start = (int32_t)PyLong_AsLong(v[9]);
+    if (v[2] != Py_None) {
+        const at::Tensor *pos = tensor(v[2]), *inv = tensor(v[3]);
+        if (!vec(pos, *q, m) || (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong)) Py_RETURN_NONE;
+        if (!inv || inv->dim() != 1 || inv->size(0) < 1 || inv->size(0) > WS_MAX_PAIRS || !vec(inv, *q, inv->size(0)) || inv->scalar_type() != at::kFloat) Py_RETURN_NONE;
+        a.positions = pos->data_ptr(); a.position_bytes = (int32_t)pos->element_size();
+        a.inv_freq = inv->data_ptr<float>(); a.pairs = (int32_t)inv->size(0);
+    } else {
+        a.start = 0;
+    }
+    a.norm = PyObject_IsTrue(v[6]); a.interleaved = PyObject_IsTrue(v[10]);
+    a.eps = (float)PyFloat_AsDouble(v[7]); a.weight_offset = (float)PyFloat_AsDouble(v[8]); a.scale = (float)PyFloat_AsDouble(v[11]);
+    if (PyErr_Occurred()) return nullptr;
+    CallOn on(*q, v[14]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor made[2];
+    if (!heads_out(v[12], *q, &made[0], &a.q_out, &a.ldqt_out, &a.ldqh_out)) Py_RETURN_NONE;
+    if (k && !heads_out(v[13], *k, &made[1], &a.k_out, &a.ldkt_out, &a.ldkh_out)) Py_RETURN_NONE;
+    WS_CALL(st, ws_head_norm_rope(&a, on.stream, nullptr, 0))
+    if (st != WS_OK) Py_RETURN_NONE;
+    PyObject *pair = PyTuple_New(2);
+    for (int i = 0; pair && i < 2; ++i) {
+        PyObject *o = v[12 + i];
+        if (made[i].defined()) o = THPVariable_Wrap(std::move(made[i]));
+        else Py_INCREF(o);
+        PyTuple_SET_ITEM(pair, i, o);
+    }
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_route(logits, top_k, score, bias, renormalize, scale, stream) -> (ids, weights)
+PyObject *py_moe_route(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 7) { PyErr_SetString(PyExc_TypeError, "moe_route takes 7 arguments"); return nullptr; }
+    const at::Tensor *x = tensor(v[0]);
+    const long top = PyLong_AsLong(v[1]), score = PyLong_AsLong(v[2]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!x || x->dim() != 2) Py_RETURN_NONE;
+    ws_moe_route_args_t a{};
+    const int64_t m = x->size(0), n = x->size(1);
+    if (m > INT32_MAX || n > INT32_MAX || !rows(x, *x, m, n, &a.ld) || !act_dtype(*x, &a.dtype) || top < 1 || top > n || top > WS_ROUTE_MAX_TOP_K) Py_RETURN_NONE;
+    a.logits = x->data_ptr(); a.m = (int32_t)m; a.experts = (int32_t)n; a.top_k = (int32_t)top; a.score = (int32_t)score;
+    if (v[3] != Py_None) {
+        const at::Tensor *b = tensor(v[3]);
+        if (!vec(b, *x, n) || b->scalar_type() != at::kFloat) Py_RETURN_NONE;
+        a.bias = b->data_ptr<float>();
+    }
+    a.renormalize = PyObject_IsTrue(v[4]);
+    a.scale = (float)PyFloat_AsDouble(v[5]);
+    if (PyErr_Occurred()) return nullptr;
+    CallOn on(*x, v[6]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor ids = new_like(*x, {m, top}, at::kInt), w = new_like(*x, {m, top}, at::kFloat);
+    a.ids = ids.data_ptr<int32_t>(); a.weights = w.data_ptr<float>();
+    WS_CALL(st, ws_moe_route(&a, on.stream, nullptr, 0))
+    if (st != WS_OK) Py_RETURN_NONE;
+    PyObject *first = THPVariable_Wrap(std::move(ids)), *second = THPVariable_Wrap(std::move(w));
+    PyObject *pair = PyTuple_Pack(2, first, second);
+    Py_DECREF(first);
+    Py_DECREF(second);
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// Packed weights or scales [experts, rows, width] whose experts lie `stride` bytes apart.
+bool experts(const at::Tensor *t, const at::Tensor &like, int64_t n, int64_t rows, int64_t width, const uint8_t **data, int64_t *stride) {
+    if (!t || t->dim() != 3 || t->element_size() != 1 || t->size(0) != n || t->size(1) != rows || t->size(2) != width || t->device() != like.device()) return false;
+    if ((width > 1 && t->stride(2) != 1) || t->stride(1) != width) return false;
+    *data = static_cast<const uint8_t *>(t->data_ptr());
+    *stride = n > 1 ? t->stride(0) : rows * width;
+    return true;
+}
+
+// moe_layer(x, route_ids, route_w, w1, s1, w3, s3, w2, s2, e_start, limit, act_quant, out, out_dtype, stream) -> out;
+// limit 0: none
+PyObject *py_moe_layer(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 15) { PyErr_SetString(PyExc_TypeError, "moe_layer takes 15 arguments"); return nullptr; }
+    const at::Tensor *x = tensor(v[0]), *ids = tensor(v[1]), *w = tensor(v[2]), *w1 = tensor(v[3]);
+    if (!x || !ids || !w || !w1 || x->dim() != 2 || ids->dim() != 2 || w1->dim() != 3) Py_RETURN_NONE;
+    ws_moe_layer_args_t a{};
+    const int64_t m = x->size(0), h = x->size(1), k = ids->size(1), n = w1->size(0), f = w1->size(1);
+    if (m > INT32_MAX || h > INT32_MAX || k > INT32_MAX || n > INT32_MAX || f > INT32_MAX || h % 32 || f % 32) Py_RETURN_NONE;
+    if (!rows(x, *x, m, h, &a.ldx) || !act_dtype(*x, &a.x_dtype) || ids->size(0) != m || !ids->is_contiguous() || !w->is_contiguous() || ids->sizes() != w->sizes()) Py_RETURN_NONE;
+    if (ids->scalar_type() != at::kInt || w->scalar_type() != at::kFloat || ids->device() != x->device() || w->device() != x->device()) Py_RETURN_NONE;
+    if (!experts(w1, *x, n, f, h / 2, &a.w1, &a.w1_stride) || !experts(tensor(v[4]), *x, n, f, h / 32, &a.s1, &a.s1_stride) ||
+        !experts(tensor(v[5]), *x, n, f, h / 2, &a.w3, &a.w3_stride) || !experts(tensor(v[6]), *x, n, f, h / 32, &a.s3, &a.s3_stride) ||
+        !experts(tensor(v[7]), *x, n, h, f / 2, &a.w2, &a.w2_stride) || !experts(tensor(v[8]), *x, n, h, f / 32, &a.s2, &a.s2_stride))
+        Py_RETURN_NONE;
+    const long start = PyLong_AsLong(v[9]);
+    a.limit = (float)PyFloat_AsDouble(v[10]);
+    a.act_quant = PyObject_IsTrue(v[11]);
+    if (PyErr_Occurred()) return nullptr;
+    at::ScalarType type = at::kFloat;
+    if (start < 0 || start > INT32_MAX || !(a.limit >= 0.0f) || (v[12] == Py_None && !result_dtype(v[13], at::kFloat, &type, &a.out_dtype))) Py_RETURN_NONE;
+    a.x = x->data_ptr(); a.route_ids = ids->data_ptr<int32_t>(); a.route_w = w->data_ptr<float>();
+    a.m = (int32_t)m; a.hidden = (int32_t)h; a.inter = (int32_t)f; a.top_k = (int32_t)k; a.e_start = (int32_t)start; a.e_len = (int32_t)n;
+    CallOn on(*x, v[14]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor made, work;
+    if (v[12] != Py_None) {
+        const at::Tensor *out = tensor(v[12]);
+        if (!rows(out, *x, m, h, &a.ldo) || !act_dtype(*out, &a.out_dtype)) Py_RETURN_NONE;
+        a.out = out->data_ptr();
+    } else {
+        made = new_like(*x, {m, h}, type);
+        a.out = made.data_ptr();
+        a.ldo = h;
+    }
+    a.workspace_bytes = ws_moe_layer_workspace(a.m, a.top_k, a.hidden, a.inter);
+    if (a.workspace_bytes > 0) {
+        work = new_like(*x, {a.workspace_bytes}, at::kByte);
+        a.workspace = work.data_ptr();
+    }
+    WS_CALL(st, ws_moe_layer(&a, on.stream, nullptr, 0))
+    if (st != WS_OK) Py_RETURN_NONE;
+    if (made.defined()) return THPVariable_Wrap(std::move(made));
+    Py_INCREF(v[12]);
+    return v[12];
+    END_HANDLE_TH_ERRORS
+}
+
+// adjust_logits(logits, tokens, offsets, prompt_lens, repetition, frequency, presence, bias_ids, bias, bias_offsets, mask, mask_rows, out,
+//               stream) -> out
+PyObject *py_adjust_logits(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 14) { PyErr_SetString(PyExc_TypeError, "adjust_logits takes 14 arguments"); return nullptr; }
+    const at::Tensor *x = tensor(v[0]);
+    if (!x || x->dim() != 2) Py_RETURN_NONE;
+    ws_adjust_logits_args_t a{};
+    const int64_t m = x->size(0), n = x->size(1);
+    if (m > INT32_MAX || n > INT32_MAX || !rows(x, *x, m, n, &a.ld) || !act_dtype(*x, &a.dtype)) Py_RETURN_NONE;
+    a.logits = x->data_ptr(); a.m = (int32_t)m; a.vocab = (int32_t)n;
+    auto entries = [&](PyObject *o, PyObject *at, const int32_t **data, int64_t *count, const void **offsets, int32_t *bytes) {
+        if ((o == Py_None) != (at == Py_None)) return false;
+        if (o == Py_None) return true;
+        const at::Tensor *t = tensor(o), *w = tensor(at);
+        if (!t || t->dim() != 1 || !vec(t, *x, t->size(0)) || t->scalar_type() != at::kInt || !vec(w, *x, m + 1)) return false;
+        if (w->scalar_type() != at::kInt && w->scalar_type() != at::kLong) return false;
+        *data = t->data_ptr<int32_t>();
+        *count = t->size(0);
+        *offsets = w->data_ptr();
+        *bytes = (int32_t)w->element_size();
+        return true;
+    };
+    if (!entries(v[1], v[2], &a.tokens, &a.n_tokens, &a.offsets, &a.offset_bytes)) Py_RETURN_NONE;
+    if (!entries(v[7], v[9], &a.bias_ids, &a.n_bias, &a.bias_offsets, &a.bias_offset_bytes)) Py_RETURN_NONE;
+    const void **per_row[4] = {reinterpret_cast<const void **>(&a.prompt_lens), reinterpret_cast<const void **>(&a.repetition),
+                               reinterpret_cast<const void **>(&a.frequency), reinterpret_cast<const void **>(&a.presence)};
+    for (int i = 0; i < 4; ++i) {
+        if (v[3 + i] == Py_None) continue;
+        const at::Tensor *t = tensor(v[3 + i]);
+        if (v[1] == Py_None || !vec(t, *x, m) || t->scalar_type() != (i ? at::kFloat : at::kInt)) Py_RETURN_NONE;
+        *per_row[i] = t->data_ptr();
+    }
+    if ((v[7] == Py_None) != (v[8] == Py_None)) Py_RETURN_NONE;
+    if (v[8] != Py_None) {
+        const at::Tensor *b = tensor(v[8]);
+        if (!vec(b, *x, a.n_bias) || b->scalar_type() != at::kFloat || a.n_bias > INT32_MAX) Py_RETURN_NONE;
+        a.bias = b->data_ptr<float>();
+    }
+    if (v[10] != Py_None) {
+        const at::Tensor *k = tensor(v[10]);
+        if (!k || k->dim() != 2 || k->scalar_type() != at::kInt || k->size(1) < (n + 31) / 32 || k->size(0) < 1 || k->size(0) > INT32_MAX) Py_RETURN_NONE;
+        if (!rows(k, *x, k->size(0), k->size(1), &a.ld_mask) || (v[11] == Py_None && k->size(0) != m)) Py_RETURN_NONE;
+        a.mask = reinterpret_cast<const uint32_t *>(k->data_ptr<int32_t>());
+        a.mask_count = (int32_t)k->size(0);
+    }
+    if (v[11] != Py_None) {
+        const at::Tensor *t = tensor(v[11]);
+        if (v[10] == Py_None || !vec(t, *x, m) || t->scalar_type() != at::kInt) Py_RETURN_NONE;
+        a.mask_rows = t->data_ptr<int32_t>();
+    }
+    CallOn on(*x, v[13]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor made;
+    if (v[12] != Py_None) {
+        const at::Tensor *out = tensor(v[12]);
+        if (!rows(out, *x, m, n, &a.ldo) || out->scalar_type() != x->scalar_type()) Py_RETURN_NONE;
+        a.out = out->data_ptr();
+    } else {
+        made = new_like(*x, {m, n}, x->scalar_type());
+        a.out = made.data_ptr();
+        a.ldo = n;
+    }
+    WS_CALL(st, ws_adjust_logits(&a, on.stream, nullptr, 0))
+    if (st != WS_OK) Py_RETURN_NONE;
+    if (made.defined()) return THPVariable_Wrap(std::move(made));
+    Py_INCREF(v[12]);
+    return v[12];
+    END_HANDLE_TH_ERRORS
+}
+
 #define WS_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {WS_METHOD(fp8), WS_METHOD(fp8_host), WS_METHOD(moe), WS_METHOD(head), WS_METHOD(fp8_group), WS_METHOD(block_norm), WS_METHOD(lora), WS_METHOD(token_logprobs),
+                         WS_METHOD(head_norm_rope), WS_METHOD(moe_route), WS_METHOD(moe_layer), WS_METHOD(adjust_logits),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_ws_torch", "torch tensors -> libws_tp.so", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
