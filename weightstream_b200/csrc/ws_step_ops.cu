@@ -45,7 +45,7 @@ ws_status_t launch_adjust(const Err &err, AdjustParams &p, void *stream) {
 }
 
 // ---- layer
-constexpr int kLayerSmem = 232448 - (int)sizeof(LayerPlan) - 1024;
+constexpr int kLayerSmem = 232448 - (int)sizeof(LayerPlan) - kLayerWarps * 16 * 8 * 4 - 1024;
 
 template <bool FIRST, bool PAIR, bool FULL, int NT, int D>
 ws_status_t launch_layer(const Err &err, const LayerParams &p, int smem, void *stream) {
@@ -55,17 +55,20 @@ ws_status_t launch_layer(const Err &err, const LayerParams &p, int smem, void *s
 }
 template <bool FIRST, bool PAIR, bool FULL, int NT>
 ws_status_t launch_layer(const Err &err, LayerParams &p, void *stream) {
-    const int column = layer_column_pitch(p.k) * (PAIR ? 2 : 1);
-    auto smem = [&](int d) { return kLayerWarps * d * kLayerStage + p.per * column; };
-    // routes a pass: as many as columns hold and the batch can have, less where wide rows leave no room for three stages
-    p.per = std::min(p.m, PAIR ? NT * 4 : 8);
-    while (p.per > 1 && smem(3) > kLayerSmem) p.per = (p.per + 1) / 2;
-    if (smem(6) <= kLayerSmem) return launch_layer<FIRST, PAIR, FULL, NT, 6>(err, p, smem(6), stream);
-    if (smem(4) <= kLayerSmem) return launch_layer<FIRST, PAIR, FULL, NT, 4>(err, p, smem(4), stream);
-    if (smem(3) <= kLayerSmem) return launch_layer<FIRST, PAIR, FULL, NT, 3>(err, p, smem(3), stream);
-    return err(WS_ERR_CAPACITY, "rows of %d activations do not fit", p.k);
+    const int row = layer_column_pitch(p.k) * (PAIR ? 2 : 1), rest = 2 * kLayerWarps * NT * 4 * 32 * 4;
+    auto room = [&](int d) { return (kLayerSmem - rest - kLayerWarps * d * kLayerStage<FULL>) / row; };
+    // Routes a pass: as many as the columns hold and the batch can have, less where wide rows leave no room for three stages.
+    // Then as many stages as leave room for the rows of a block's passes, of which there are mostly two.
+    p.per = std::max(1, std::min({p.m, PAIR ? NT * 4 : 8, room(3)}));
+    const int wanted = std::min(p.m * p.top_k, 2 * p.per);
+    const int d = room(6) >= wanted ? 6 : room(4) >= wanted ? 4 : 3;
+    p.room = std::min(room(d), kLayerMaxPasses * 8);
+    const int smem = kLayerWarps * d * kLayerStage<FULL> + p.room * row + rest;
+    if (p.room < p.per) return err(WS_ERR_CAPACITY, "rows of %d activations do not fit", p.k);
+    return d == 6 ? launch_layer<FIRST, PAIR, FULL, NT, 6>(err, p, smem, stream) : d == 4 ? launch_layer<FIRST, PAIR, FULL, NT, 4>(err, p, smem, stream)
+                                                                                          : launch_layer<FIRST, PAIR, FULL, NT, 3>(err, p, smem, stream);
 }
-static_assert(kLayerWarps * 3 * kLayerStage + 2 * layer_column_pitch(kLayerMaxWidth) <= kLayerSmem, "the widest rows");
+static_assert(kLayerWarps * 3 * kLayerStage<false> + 2 * layer_column_pitch(kLayerMaxWidth) + 2 * kLayerWarps * 2 * 4 * 32 * 4 <= kLayerSmem, "the widest rows");
 
 int64_t layer_bytes(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -138,9 +141,9 @@ ws_status_t ws_moe_route(const ws_moe_route_args_t *a, void *stream, char *err_t
                   grid, kRouteThreads, 0, 1, stream, p);
 }
 
-int64_t ws_moe_layer_workspace(int32_t m, int32_t top_k, int32_t hidden, int32_t inter) {   // hidden of the routes, their results, counts
+int64_t ws_moe_layer_workspace(int32_t m, int32_t top_k, int32_t hidden, int32_t inter) {   // hidden of the routes, their results
     if (m < 1 || top_k < 1 || hidden < 1 || inter < 1) return 0;
-    return layer_bytes((int64_t)m * top_k * inter * 4) + layer_bytes((int64_t)m * top_k * hidden * 4) + layer_bytes((int64_t)(hidden / 16) * m * 4);
+    return layer_bytes((int64_t)m * top_k * inter * 4) + layer_bytes((int64_t)m * top_k * hidden * 4);
 }
 
 ws_status_t ws_moe_layer(const ws_moe_layer_args_t *a, void *stream, char *err_text, size_t err_len) {
@@ -168,8 +171,7 @@ ws_status_t ws_moe_layer(const ws_moe_layer_args_t *a, void *stream, char *err_t
     LayerParams p{};
     char *work = static_cast<char *>(a->workspace);
     p.h = reinterpret_cast<float *>(work); work += layer_bytes((int64_t)a->m * a->top_k * a->inter * 4);
-    p.part = reinterpret_cast<float *>(work); work += layer_bytes((int64_t)a->m * a->top_k * a->hidden * 4);
-    p.count = reinterpret_cast<uint32_t *>(work);
+    p.part = reinterpret_cast<float *>(work);
     p.x = a->x; p.ldx = a->ldx; p.x_dtype = a->x_dtype; p.vec = aligned(a->x, a->ldx, a->x_dtype, 16);
     p.ids = a->route_ids; p.weights = a->route_w; p.m = a->m; p.top_k = a->top_k; p.e_start = a->e_start; p.e_len = a->e_len;
     p.out = a->out; p.ldo = a->ldo; p.out_dtype = a->out_dtype; p.act_quant = a->act_quant != 0;
@@ -177,15 +179,18 @@ ws_status_t ws_moe_layer(const ws_moe_layer_args_t *a, void *stream, char *err_t
     LayerParams q = p;
     p.wa = a->w1; p.sa = a->s1; p.wb = a->w3; p.sb = a->s3;
     p.wa_e = a->w1_stride; p.sa_e = a->s1_stride; p.wb_e = a->w3_stride; p.sb_e = a->s3_stride;
-    p.k = a->hidden; p.units = a->inter / 8; p.n = a->hidden / 16;
+    p.k = a->hidden; p.units = a->inter / 8; p.n = a->inter;
     q.wa = q.wb = a->w2; q.sa = q.sb = a->s2; q.wa_e = q.wb_e = a->w2_stride; q.sa_e = q.sb_e = a->s2_stride;
-    q.k = a->inter; q.units = a->hidden / 16; q.n = a->hidden;
+    q.k = a->inter; q.units = a->hidden / 32; q.n = a->hidden;
     const bool pair = a->x_dtype == WS_ACT_F32 && !a->act_quant, full = p.k % kLayerChunk == 0;
     ws_status_t st = pair ? full ? launch_layer<true, true, true, 1>(err, p, stream) : launch_layer<true, true, false, 1>(err, p, stream)
                           : full ? launch_layer<true, false, true, 1>(err, p, stream) : launch_layer<true, false, false, 1>(err, p, stream);
     if (st != WS_OK) return st;
-    if (q.k % kLayerChunk == 0) return a->m <= 4 ? launch_layer<false, true, true, 1>(err, q, stream) : launch_layer<false, true, true, 2>(err, q, stream);
-    return a->m <= 4 ? launch_layer<false, true, false, 1>(err, q, stream) : launch_layer<false, true, false, 2>(err, q, stream);
+    if (q.k % kLayerChunk == 0) st = a->m <= 4 ? launch_layer<false, true, true, 1>(err, q, stream) : launch_layer<false, true, true, 2>(err, q, stream);
+    else st = a->m <= 4 ? launch_layer<false, true, false, 1>(err, q, stream) : launch_layer<false, true, false, 2>(err, q, stream);
+    if (st != WS_OK) return st;
+    q.vec = aligned(a->out, a->ldo, a->out_dtype, 4 * type_bytes(a->out_dtype));
+    return launch(err, layer_sum_kernel, dim3((unsigned)(((int64_t)a->m * (a->hidden / 4) + kLayerSumThreads - 1) / kLayerSumThreads)), kLayerSumThreads, 0, 1, stream, q);
 }
 
 ws_status_t ws_adjust_logits(const ws_adjust_logits_args_t *a, void *stream, char *err_text, size_t err_len) {
