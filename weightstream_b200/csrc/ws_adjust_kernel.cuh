@@ -5,9 +5,15 @@
 //   z = z - f * count - p * (count > 0)                 count: occurrences behind the history's first `prompt` tokens
 //   z = -inf                                            where the row's mask has no bit for v
 //
-// A block takes a slice of a row's vocabulary that fits its registers: it requests its logits first, counts the row's
-// history into a table of its slice in shared memory while they come, and writes every value once.  So a row's history
-// is read by each of its blocks (out of L2), and nothing is exchanged between them.
+// A block takes a slice of a row's vocabulary that fits its registers.  It requests its logits, counts the row's lists into a
+// table of its slice in shared memory while they come (a row's lists are read by each of its blocks, out of L2; nothing is
+// exchanged between blocks), stores the logits under the mask, and then takes the touched values by themselves: every
+// thread notes which of its places are touched, and the block's threads share them out.
+//
+// Other ways, us for one row with 6000 tokens, 64 rows with 4000, 512 bf16 rows with 2000 under masks: touched values where they
+// pass (most vectors of a warp have one, and all lanes wait for it) 6, 35 and 127; noted by who counts first 10, 29 and 86;
+// clusters of a row's slices that count into each other's tables 19, 52 and 169; a plain copy, and a hash table a row beside
+// or behind it 12, 33 and 91.
 #pragma once
 
 #include "ws_values.cuh"
@@ -15,7 +21,11 @@
 namespace ws {
 
 constexpr int kAdjustThreads = 256;
-constexpr uint32_t kAdjustPrompt = 0x80000000u;    // a table's word: occurrences in the answer, this bit for one in the prompt
+constexpr int kAdjustList = 2048;                   // touched places that are noted; beyond, the table is looked through
+// A word of the table: 31 a bias; 30 to 16 occurrences in the prompt; 15 to 0 occurrences behind it.  Rows with longer
+// histories: 30 an occurrence in the prompt, 29 to 0 occurrences behind it.
+constexpr uint32_t kAdjustListed = 0x80000000u, kAdjustPrompt = 0x40000000u;
+constexpr int kAdjustShort = 32767;
 
 struct AdjustParams {
     const void *logits;
@@ -31,7 +41,7 @@ struct AdjustParams {
     const uint32_t *mask;                           // [mask_count, ld_mask] words, bit v % 32 of word v / 32: v is allowed
     const int32_t *mask_rows;                       // [m] or null: row t of the mask
     int64_t n_tokens, n_bias, ld_mask;
-    int32_t m, vocab, mask_count, offset_bytes, bias_offset_bytes, slices;
+    int32_t m, vocab, mask_count, offset_bytes, bias_offset_bytes, slices, in_place;
 };
 
 // Bounds of a row's entries, whatever the offsets hold.
@@ -42,39 +52,102 @@ __device__ __forceinline__ void adjust_range(const void *offsets, int bytes, int
     b = b < a ? a : b > n ? n : b;
 }
 
-struct AdjustRow {
-    float rep, freq, pres;
-    bool masked;
-    const uint32_t *mask;
-};
-
-__device__ __forceinline__ float adjust_value(float z, uint32_t word, const AdjustRow &r) {
-    if (word) {
-        z = z > 0.0f ? __fdiv_rn(z, r.rep) : z * r.rep;
-        const uint32_t n = word & ~kAdjustPrompt;
-        if (n) z = fmaf(-r.freq, (float)n, z) - r.pres;
+// f(entry, value) for the entries [a, b) of a list, by all threads of the block, four loads ahead.  (One copy of f: vectors of
+// entries and a loop unrolled over them made 36 copies of it, whose instructions had to be fetched first: one row with 6000
+// tokens 36 us.)
+template <typename F>
+__device__ __forceinline__ void adjust_list(const int32_t *list, int64_t a, int64_t b, F f) {
+    const int step = blockDim.x;
+    const int n = (int)min(b - a, (int64_t)INT32_MAX - 8 * 1024);       // (a row's own entries)
+    const int32_t *const own = list + a;
+    int32_t ahead[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) ahead[k] = (int)threadIdx.x + k * step < n ? own[threadIdx.x + k * step] : -1;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += step) {
+        const int32_t v = ahead[0];
+        ahead[0] = ahead[1];
+        ahead[1] = ahead[2];
+        ahead[2] = ahead[3];
+        ahead[3] = i + 4 * step < n ? own[i + 4 * step] : -1;
+        f(a + i, v);
     }
-    return z;
+}
+
+// f(place in the list, value) for its n entries, by all threads of the block: 16 bytes a load, two of them at once (four
+// cost 2000 tokens as many instructions as 4000).
+template <typename F>
+__device__ __forceinline__ void adjust_tokens(const int32_t *list, int n, F f) {
+    const int tid = threadIdx.x, head = min(n, (int)(16 - (reinterpret_cast<uintptr_t>(list) & 15)) / 4 & 3), vectors = (n - head) / 4;
+    const int4 *const v = reinterpret_cast<const int4 *>(list + head);
+#pragma unroll 1
+    for (int i = tid; i < vectors; i += 2 * kAdjustThreads) {
+        int4 t[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) t[k] = i + k * kAdjustThreads < vectors ? v[i + k * kAdjustThreads] : make_int4(-1, -1, -1, -1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int at = head + (i + k * kAdjustThreads) * 4;
+            f(at, t[k].x);
+            f(at + 1, t[k].y);
+            f(at + 2, t[k].z);
+            f(at + 3, t[k].w);
+        }
+    }
+    const int ends = n - vectors * 4;               // before the first vector and behind the last
+    if (tid < ends) {
+        const int at = tid < head ? tid : tid + vectors * 4;
+        f(at, list[at]);
+    }
+}
+
+__device__ __forceinline__ const uint32_t *adjust_mask(const AdjustParams &p, int t) {    // null: none
+    const int which = !p.mask ? -1 : p.mask_rows ? p.mask_rows[t] : t;
+    return which >= 0 && which < p.mask_count ? p.mask + which * p.ld_mask : nullptr;
+}
+__device__ __forceinline__ bool adjust_open(const uint32_t *mask, int v) { return !mask || (mask[v >> 5] >> (v & 31) & 1u); }
+constexpr uint32_t kAdjustMinusInf = 0xFF800000u;
+
+// A word of logits under the first bits of a mask.
+template <bool F32>
+__device__ __forceinline__ void adjust_close(uint32_t &w, uint32_t bits) {
+    if constexpr (F32) {
+        w = bits & 1u ? w : kAdjustMinusInf;
+    } else {
+        const uint32_t keep = ((bits & 3u) * 0x8001u & 0x10001u) * 0xFFFFu;        // two bits to two halves
+        w = (w & keep) | (0xFF80FF80u & ~keep);
+    }
 }
 
 // VEC: rows are read and written 16 bytes at a time.  A row's values lie on a grid of vectors that begins at its first
 // aligned address or one vector before; values of the first and last vector that are not the row's are left alone.
-template <bool F32, bool VEC, int U>
-__global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_constant__ AdjustParams p) {
-    constexpr int W = F32 ? 4 : 8;                  // values a vector
+template <bool F32, bool VEC, int U, int BLOCKS>
+__global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __grid_constant__ AdjustParams p) {
+    constexpr int W = F32 ? 4 : 8, kType = F32 ? WS_ACT_F32 : WS_ACT_BF16;      // values a vector
     constexpr int kSlice = kAdjustThreads * U * W;
-    extern __shared__ uint32_t adjust_table[];      // counts, then places of biases (1 + entry), as far as the call has them
-    uint32_t *const count_s = adjust_table, *const bias_s = adjust_table + (p.tokens ? kSlice : 0);
-    const int t = blockIdx.x / p.slices, slice = blockIdx.x % p.slices, tid = threadIdx.x;
+    static_assert(U * W <= 64 && kSlice <= 65536, "a bit for each of a thread's places; a place is 16 bits");
+    extern __shared__ __align__(16) uint32_t adjust_table[];
+    __shared__ uint16_t list_s[kAdjustList];
+    __shared__ int touched_s;
+    const int t = blockIdx.x / p.slices, slice = blockIdx.x - t * p.slices, tid = threadIdx.x, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const char *const x = static_cast<const char *>(p.logits) + (int64_t)t * p.ld * (F32 ? 4 : 2);
     char *const y = static_cast<char *>(p.out) + (int64_t)t * p.ldo * (F32 ? 4 : 2);
     const int skew = VEC ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / (F32 ? 4 : 2)) : 0;  // the grid begins so many values before the row
     const int v0 = slice * kSlice - skew;
-    for (int i = tid * 4; i < (p.tokens ? kSlice : 0) + (p.bias_ids ? kSlice : 0); i += kAdjustThreads * 4)
-        *reinterpret_cast<uint4 *>(adjust_table + i) = make_uint4(0u, 0u, 0u, 0u);
+    const bool lists = p.tokens || p.bias_ids;
+    if (lists) {
+#pragma unroll 1
+        for (int i = tid * 4; i < kSlice; i += kAdjustThreads * 4) *reinterpret_cast<uint4 *>(adjust_table + i) = make_uint4(0u, 0u, 0u, 0u);
+        if (tid == 0) touched_s = 0;
+    }
     wait_predecessor();
-    // ---- the slice's logits
+    // ---- what the row's lists are, then the slice's logits, then the lists
+    int64_t a = 0, b = 0, bias0 = 0, bias1 = 0;
+    if (p.tokens) adjust_range(p.offsets, p.offset_bytes, t, p.n_tokens, a, b);
+    if (p.bias_ids) adjust_range(p.bias_offsets, p.bias_offset_bytes, t, p.n_bias, bias0, bias1);
+    const uint32_t *const mask = adjust_mask(p, t);
+    const bool dense = mask || !p.in_place;         // (else only touched values change)
     uint32_t raw[U][4];
     if constexpr (VEC) {
 #pragma unroll
@@ -83,75 +156,100 @@ __global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_con
             raw[u][0] = raw[u][1] = raw[u][2] = raw[u][3] = 0u;
             asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
                          : "+r"(raw[u][0]), "+r"(raw[u][1]), "+r"(raw[u][2]), "+r"(raw[u][3])
-                         : "l"(x + (int64_t)v * (F32 ? 4 : 2)), "r"((int)(v >= 0 && v <= p.vocab - W)) : "memory");
+                         : "l"(x + (int64_t)v * (F32 ? 4 : 2)), "r"((int)(dense && v >= 0 && v <= p.vocab - W)) : "memory");
         }
     }
-    AdjustRow r;
-    r.rep = p.repetition ? p.repetition[t] : 1.0f;
-    r.freq = p.frequency ? p.frequency[t] : 0.0f;
-    r.pres = p.presence ? p.presence[t] : 0.0f;
-    int which = -1;
-    if (p.mask) which = p.mask_rows ? p.mask_rows[t] : t;
-    r.masked = which >= 0 && which < p.mask_count;
-    r.mask = p.mask + (r.masked ? which * p.ld_mask : 0);
+    const bool listed = bias1 > bias0 || b > a, packed = b - a <= kAdjustShort;     // (the block's conditions)
+    if (listed) {
+        const int low = max(v0, 0);                 // the slice's tokens: low and `width` behind it
+        const uint32_t width = (uint32_t)max(0, min(v0 + kSlice, p.vocab) - low);
+        uint32_t *const word = adjust_table + (low - v0);
+        __syncthreads();
+        if (bias1 > bias0)
+            adjust_list(p.bias_ids, bias0, bias1, [&](int64_t, int32_t v) {
+                if ((uint32_t)(v - low) < width) atomicOr(&word[v - low], kAdjustListed);
+            });
+        if (b > a) {
+            const int behind_at = p.prompt_lens ? p.prompt_lens[t] : 0;
+            const int64_t prompt = a + behind_at;
+            if (packed)
+                adjust_tokens(p.tokens + a, (int)(b - a), [&](int i, int32_t v) {
+                    if ((uint32_t)(v - low) < width) atomicAdd(&word[v - low], i < behind_at ? 0x10000u : 1u);
+                });
+            else
+                adjust_list(p.tokens, a, b, [&](int64_t i, int32_t v) {
+                    if ((uint32_t)(v - low) >= width) return;
+                    if (i < prompt) atomicOr(&word[v - low], kAdjustPrompt);
+                    else atomicAdd(&word[v - low], 1u);
+                });
+        }
+    }
+    // ---- the logits under the mask
+    if (dense) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = (u * kAdjustThreads + tid) * W, v = v0 + at;
+            if (VEC && v >= 0 && v <= p.vocab - W) {
+                if (mask) {                         // (a vector of a row that is not aligned may lie in two words)
+                    const uint32_t bits = __funnelshift_r(mask[v >> 5], mask[(v + W - 1) >> 5], v & 31);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) adjust_close<F32>(raw[u][k], bits >> (F32 ? k : 2 * k));
+                }
+                *reinterpret_cast<uint4 *>(y + (int64_t)v * (F32 ? 4 : 2)) = make_uint4(raw[u][0], raw[u][1], raw[u][2], raw[u][3]);
+            } else {
+#pragma unroll 1
+                for (int k = 0; k < W; ++k) {
+                    // (values of a vector are a block apart where rows are read one by one)
+                    const int w = v0 + (VEC ? at + k : (u * W + k) * kAdjustThreads + tid);
+                    if (w < 0 || w >= p.vocab) continue;
+                    const float z = load1(x, kType, w);
+                    store1(y, kType, w, adjust_open(mask, w) ? z : __uint_as_float(kAdjustMinusInf));
+                }
+            }
+        }
+    }
+    if (!listed) return;
+    // ---- the touched places, a bit each of this thread's
     __syncthreads();
-    // ---- the row's history and biases that fall into the slice
-    if (p.tokens) {
-        int64_t a, b;
-        adjust_range(p.offsets, p.offset_bytes, t, p.n_tokens, a, b);
-        const int64_t prompt = a + (p.prompt_lens ? p.prompt_lens[t] : 0);
-        for (int64_t i = a + tid; i < b; i += kAdjustThreads) {
-            const int32_t v = p.tokens[i];
-            const uint32_t at = (uint32_t)(v - v0);
-            if (v >= 0 && v < p.vocab && at < (uint32_t)kSlice) {
-                if (i < prompt) atomicOr(&count_s[at], kAdjustPrompt);
-                else atomicAdd(&count_s[at], 1u);
-            }
-        }
+    uint64_t mine = 0u;
+#pragma unroll
+    for (int q = 0; q < U * W / 4; ++q) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(adjust_table + (q * kAdjustThreads + tid) * 4);
+        if (w.x | w.y | w.z | w.w) mine |= (uint64_t)((w.x ? 1u : 0u) | (w.y ? 2u : 0u) | (w.z ? 4u : 0u) | (w.w ? 8u : 0u)) << 4 * q;
     }
-    if (p.bias_ids) {
-        int64_t a, b;
-        adjust_range(p.bias_offsets, p.bias_offset_bytes, t, p.n_bias, a, b);
-        for (int64_t i = a + tid; i < b; i += kAdjustThreads) {
-            const int32_t v = p.bias_ids[i];
-            const uint32_t at = (uint32_t)(v - v0);
-            if (v >= 0 && v < p.vocab && at < (uint32_t)kSlice) atomicMax(&bias_s[at], (uint32_t)(i - a) + 1u);
-        }
+    const int count = __popcll(mine);
+    int upto = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
     }
-    int64_t bias0 = 0, bias1;
-    if (p.bias_ids) adjust_range(p.bias_offsets, p.bias_offset_bytes, t, p.n_bias, bias0, bias1);
+    int place = 0;
+    if (lane == 31 && upto) place = atomicAdd(&touched_s, upto);
+    place = __shfl_sync(0xffffffffu, place, 31) + upto - count;
+    for (uint64_t left = mine; left; left &= left - 1, ++place) {
+        const int bit = __ffsll(left) - 1;
+        if (place < kAdjustList) list_s[place] = (uint16_t)(((bit >> 2) * kAdjustThreads + tid) * 4 + (bit & 3));
+    }
     __syncthreads();
-    auto one = [&](float z, int at, int v) {
-        if (p.bias_ids) {
-            const uint32_t e = bias_s[at];
-            if (e) z += p.bias[bias0 + e - 1];
+    // ---- their values.  (In place the mask has been at x already, which gives the same.)
+    const int touched = touched_s, all = touched <= kAdjustList ? touched : kSlice;
+    const float rep = p.repetition && b > a ? p.repetition[t] : 1.0f, freq = p.frequency && b > a ? p.frequency[t] : 0.0f, pres = p.presence && b > a ? p.presence[t] : 0.0f;
+#pragma unroll 1
+    for (int i = tid; i < all; i += kAdjustThreads) {
+        const int at = touched <= kAdjustList ? (int)list_s[i] : i, v = v0 + at;
+        const uint32_t word = adjust_table[at];
+        if (!word || !adjust_open(mask, v)) continue;
+        float z = load1(x, kType, v);
+        if (word & kAdjustListed) {                 // its last entry
+            int64_t e = bias1;
+            while (e > bias0 && p.bias_ids[e - 1] != v) --e;
+            if (e > bias0) z += p.bias[e - 1];
         }
-        if (p.tokens) z = adjust_value(z, count_s[at], r);
-        if (r.masked && !(r.mask[v >> 5] >> (v & 31) & 1u)) z = __uint_as_float(0xFF800000u);
-        return z;
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int at = (u * kAdjustThreads + tid) * W, v = v0 + at;
-        if (VEC && v >= 0 && v <= p.vocab - W) {
-            float z[W];
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                const uint32_t w = raw[u][F32 ? e & 3 : e / 2];
-                z[e] = one(__uint_as_float(F32 ? w : e & 1 ? w & 0xFFFF0000u : w << 16), at + e, v + e);
-            }
-            uint4 o;
-            if constexpr (F32) o = make_uint4(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3]));
-            else o = make_uint4(pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]), pack_bf16x2(z[4], z[5]), pack_bf16x2(z[6], z[7]));
-            *reinterpret_cast<uint4 *>(y + (int64_t)v * (F32 ? 4 : 2)) = o;
-        } else {
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                // (values of a vector are a block apart where rows are read one by one)
-                const int place = VEC ? at + e : (u * W + e) * kAdjustThreads + tid, w = v0 + place;
-                if (w >= 0 && w < p.vocab) store1(y, F32 ? WS_ACT_F32 : WS_ACT_BF16, w, one(load1(x, F32 ? WS_ACT_F32 : WS_ACT_BF16, w), place, w));
-            }
-        }
+        const uint32_t behind = packed ? word & 0xFFFFu : word & (kAdjustPrompt - 1u);
+        if (word & ~kAdjustListed) z = z > 0.0f ? __fdiv_rn(z, rep) : z * rep;
+        if (behind) z = fmaf(-freq, (float)behind, z) - pres;
+        store1(y, kType, v, z);
     }
 }
 

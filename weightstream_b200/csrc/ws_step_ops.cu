@@ -23,25 +23,23 @@ ws_status_t launch_heads(const Err &err, int nu, const HeadsParams &p, void *str
 }
 
 // ---- logits
-template <bool F32, bool VEC, int U>
+template <bool F32, bool VEC, int U, int BLOCKS>
 ws_status_t launch_adjust(const Err &err, AdjustParams &p, void *stream) {
     constexpr int W = F32 ? 4 : 8, slice = kAdjustThreads * U * W;
-    constexpr auto k = adjust_kernel<F32, VEC, U>;
+    if (slice * 4 > 40 * 1024) {                    // (48 KB with the list)
+        const ws_status_t st = allow_smem<adjust_kernel<F32, VEC, U, BLOCKS>>(err, slice * 4);
+        if (st != WS_OK) return st;
+    }
     const int64_t slices = ((int64_t)p.vocab + (VEC ? W - 1 : 0) + slice - 1) / slice;
     if (slices * p.m > INT32_MAX) return err(WS_ERR_CAPACITY, "%d rows of %d logits: too many for one call", p.m, p.vocab);
     p.slices = (int)slices;
-    const int smem = slice * 4 * ((p.tokens ? 1 : 0) + (p.bias_ids ? 1 : 0));
-    if (smem > 47 * 1024) {
-        const ws_status_t st = allow_smem<k>(err, slice * 8);
-        if (st != WS_OK) return st;
-    }
-    return launch(err, k, dim3((unsigned)(slices * p.m)), kAdjustThreads, smem, 1, stream, p);
+    return launch(err, adjust_kernel<F32, VEC, U, BLOCKS>, dim3((unsigned)(slices * p.m)), kAdjustThreads, p.tokens || p.bias_ids ? slice * 4 : 0, 1, stream, p);
 }
 template <bool F32, bool VEC>
 ws_status_t launch_adjust(const Err &err, AdjustParams &p, void *stream) {
     // Few rows are cut into more blocks.
-    if ((int64_t)p.m * p.vocab <= 148 * 8192) return launch_adjust<F32, VEC, F32 ? 2 : 1>(err, p, stream);
-    return launch_adjust<F32, VEC, F32 ? 8 : 4>(err, p, stream);
+    if ((int64_t)p.m * p.vocab <= 148 * 8192) return launch_adjust<F32, VEC, F32 ? 2 : 1, 6>(err, p, stream);
+    return launch_adjust<F32, VEC, F32 ? 8 : 4, F32 ? 4 : 6>(err, p, stream);
 }
 
 // ---- layer
@@ -221,6 +219,8 @@ ws_status_t ws_adjust_logits(const ws_adjust_logits_args_t *a, void *stream, cha
     const int64_t es = type_bytes(a->dtype);
     // a row's values and results lie alike within 16 bytes
     const bool vec = (reinterpret_cast<uintptr_t>(a->logits) - reinterpret_cast<uintptr_t>(a->out)) % 16 == 0 && (a->ld - a->ldo) * es % 16 == 0;
+    p.in_place = a->logits == a->out && a->ld == a->ldo;
+    if (p.in_place && !p.mask && !p.tokens && !p.bias_ids) return WS_OK;
     if (a->dtype == WS_ACT_F32) return vec ? launch_adjust<true, true>(err, p, stream) : launch_adjust<true, false>(err, p, stream);
     return vec ? launch_adjust<false, true>(err, p, stream) : launch_adjust<false, false>(err, p, stream);
 }
