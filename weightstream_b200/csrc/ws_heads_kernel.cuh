@@ -4,7 +4,8 @@
 //   a' = s (a cos - b sin),  b' = s (a sin + b cos)     for the pairs (a, b) of u's rotated part, angle = position * inv_freq
 //
 // The angle is a product of 64 bits, reduced to a turn before its cosine is taken in 32, so that positions of millions
-// have the same error as the first ones.  A token's cosines and sines are computed once a block and serve all its heads.
+// have the same error as the first ones.  A token's cosines and sines are computed once a team of threads and serve all
+// its heads: a lane keeps them, times the weights, for the pairs that it has of every head.
 #pragma once
 
 #include "ws_values.cuh"
@@ -21,14 +22,15 @@ struct HeadsParams {
     int32_t heads[2];
     const void *positions;
     const float *inv_freq;                          // [pairs]
-    int32_t m, d, pairs, start, interleaved, norm, dtype, w_dtype, position_bytes, lanes, groups;
+    int32_t m, d, pairs, start, interleaved, norm, dtype, w_dtype, position_bytes;
+    int32_t lanes, groups, teams;                   // lanes a head; blocks a token, or tokens a block
     float eps, weight_offset, scale;
 };
 
-__device__ __forceinline__ void heads_angles(const HeadsParams &p, int t, float *cos_s, float *sin_s) {
-    if (!p.pairs) return;
+__device__ __forceinline__ void heads_angles(const HeadsParams &p, int t, int tid, int threads, float *cos_s, float *sin_s) {
+    if (!p.pairs || t >= p.m) return;
     const double at = p.position_bytes == 8 ? (double)static_cast<const int64_t *>(p.positions)[t] : (double)static_cast<const int32_t *>(p.positions)[t];
-    for (int i = threadIdx.x; i < p.pairs; i += blockDim.x) {
+    for (int i = tid; i < p.pairs; i += threads) {
         double turns = at * (double)p.inv_freq[i] * 0.15915494309189533577;     // 1 / (2 pi)
         turns -= rint(turns);
         float s, c;
@@ -39,17 +41,20 @@ __device__ __forceinline__ void heads_angles(const HeadsParams &p, int t, float 
 }
 
 // Whole vectors of eight values.  A lane holds NU units of two vectors, those that are rotated into each other where
-// halves are paired, so that a pair never leaves its lane; `lanes` neighbours hold a head.
-template <bool F32, int NU>
-__global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_constant__ HeadsParams p) {
-    __shared__ __align__(16) float cos_s[WS_MAX_PAIRS], sin_s[WS_MAX_PAIRS];
-    const int t = blockIdx.x / p.groups, lane = threadIdx.x & (p.lanes - 1), per = kHeadsThreads / p.lanes;
-    const int all = p.heads[0] + p.heads[1], step = per * p.groups;
+// halves are paired, so that a pair never leaves its lane; `lanes` neighbours hold a head.  A team of threads has a token,
+// or one of `groups` shares of its heads.
+// WHOLE: every lane has all of its vectors.
+template <bool F32, bool INTER, int NU, bool WHOLE>
+__global__ void __launch_bounds__(kHeadsThreads, NU == 1 ? F32 ? 2 : 3 : 1) heads_kernel(const __grid_constant__ HeadsParams p) {
+    __shared__ __align__(16) float cos_s[WS_MAX_PAIRS], sin_s[WS_MAX_PAIRS];      // of all teams: pairs * teams are no more
+    const int threads = kHeadsThreads / p.teams, team = threadIdx.x / threads, tid = threadIdx.x - team * threads;
+    const int t = p.teams > 1 ? blockIdx.x * p.teams + team : blockIdx.x / p.groups, share = p.teams > 1 ? 0 : blockIdx.x % p.groups;
+    const int lane = tid & (p.lanes - 1), per = threads / p.lanes;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // a unit's vectors (first values), -1: none; whether it is rotated
     int at[NU][2];
     bool turn[NU][2];
-    const int rot = 2 * p.pairs, halves = p.interleaved ? 0 : p.pairs / 8;
+    const int rot = 2 * p.pairs, halves = INTER ? 0 : p.pairs / 8;
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
         const int u = n * p.lanes + lane;
@@ -62,81 +67,113 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_const
             } else {
                 v = ((u - halves) * 2 + h) * 8;
                 if (halves && v >= p.start) v += rot;
-                turn[n][h] = p.interleaved && v >= p.start && v < p.start + rot;
+                turn[n][h] = INTER && v >= p.start && v < p.start + rot;
             }
             at[n][h] = v < p.d ? v : -1;
         }
     }
     wait_predecessor();
-    heads_angles(p, t, cos_s, sin_s);
+    heads_angles(p, t, tid, threads, cos_s + team * p.pairs, sin_s + team * p.pairs);
     __syncthreads();
-    for (int head = blockIdx.x % p.groups * per + threadIdx.x / p.lanes; head - (int)(threadIdx.x & 31) / p.lanes < all; head += step) {
-        const bool ok = head < all;
-        const int which = head >= p.heads[0], j = which ? head - p.heads[0] : head;
-        const int64_t from = (int64_t)t * p.ldt[which] + (int64_t)j * p.ldh[which], to = (int64_t)t * p.ldyt[which] + (int64_t)j * p.ldyh[which];
+    const float over_d = 1.0f / (float)p.d;
+    if (t >= p.m) return;                           // (whole warps: a team has 64 threads at least)
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const int heads = p.heads[which], mine = share * per + tid / p.lanes, first = share * per + (tid & ~31) / p.lanes;    // this lane's head, its warp's first
+        if (first >= heads) continue;
+        constexpr int kBytes = F32 ? 4 : 2;
+        const int step = per * p.groups;
+        const int64_t ahead = step * p.ldh[which] * kBytes, ahead_out = step * p.ldyh[which] * kBytes;
+        const char *from = static_cast<const char *>(p.x[which]) + (t * p.ldt[which] + mine * p.ldh[which]) * kBytes;
+        char *to = static_cast<char *>(p.y[which]) + (t * p.ldyt[which] + mine * p.ldyh[which]) * kBytes;
         Eight<F32> raw[NU][2];
+        auto load = [&](bool there) {               // of the head at `from`
 #pragma unroll
-        for (int n = 0; n < NU; ++n)
+            for (int n = 0; n < NU; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) raw[n][h].load(p.x[which], from + (at[n][h] < 0 ? 0 : at[n][h]), ok && at[n][h] >= 0);
-        float r = 1.0f;
-        if (p.norm) {
+                for (int h = 0; h < 2; ++h) {
+                    if (WHOLE) {
+                        if (there) raw[n][h].load_all(from, at[n][h]);
+                    } else {
+                        raw[n][h].load(from, at[n][h] < 0 ? 0 : at[n][h], there && at[n][h] >= 0);
+                    }
+                }
+        };
+        load(mine < heads);
+        // pairs (a, b) become (a fa - b fb, a fc + b fd); without rotation (a fa, b fd)
+        float fa[NU][8], fb[NU][8], fc[NU][8], fd[NU][8];
+#pragma unroll
+        for (int n = 0; n < NU; ++n) {
+            float w[2][8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[h][e] = 1.0f;
+                if (!p.w[which] || (!WHOLE && at[n][h] < 0)) continue;
+                if (p.w_dtype == WS_ACT_F32) {
+                    Eight<true> g;
+                    g.load(p.w[which], at[n][h], true);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[h][e] = p.weight_offset + g.get(e);
+                } else {
+                    Eight<false> g;
+                    g.load(p.w[which], at[n][h], true);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[h][e] = p.weight_offset + g.get(e);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float wa = INTER ? w[e / 4][e % 4 * 2] : w[0][e], wb = INTER ? w[e / 4][e % 4 * 2 + 1] : w[1][e];
+                fa[n][e] = wa;
+                fd[n][e] = wb;
+                fb[n][e] = fc[n][e] = 0.0f;
+                if (!turn[n][INTER ? e / 4 : 0]) continue;
+                const int i = team * p.pairs + (INTER ? (at[n][e / 4] - p.start) / 2 + e % 4 : at[n][0] - p.start + e);
+                const float c = cos_s[i], s = sin_s[i];
+                fa[n][e] = wa * c;
+                fb[n][e] = wb * s;
+                fc[n][e] = wa * s;
+                fd[n][e] = wb * c;
+            }
+        }
+#pragma unroll 1
+        for (int head = mine, lead = first; lead < heads; head += step, lead += step, to += ahead_out) {
+            float v[NU][2][8];
             float sum = 0.0f;
 #pragma unroll
             for (int n = 0; n < NU; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum = fmaf(raw[n][h].get(e), raw[n][h].get(e), sum);
-            for (int o = p.lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            r = rsqrtf(sum / (float)p.d + p.eps);
-        }
-        if (!ok) continue;
-        const void *const w = p.w[which];
-#pragma unroll
-        for (int n = 0; n < NU; ++n) {
-            float v[2][8];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (w && at[n][h] >= 0) {
-                    if (p.w_dtype == WS_ACT_F32) {
-                        Eight<true> g;
-                        g.load(w, at[n][h], true);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[h][e] = raw[n][h].get(e) * r * (p.weight_offset + g.get(e));
-                    } else {
-                        Eight<false> g;
-                        g.load(w, at[n][h], true);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[h][e] = raw[n][h].get(e) * r * (p.weight_offset + g.get(e));
+                    for (int e = 0; e < 8; ++e) {
+                        v[n][h][e] = raw[n][h].get(e);
+                        sum = fmaf(v[n][h][e], v[n][h][e], sum);
                     }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[h][e] = raw[n][h].get(e) * r;
-                }
+            from += ahead;
+            load(head + step < heads);              // the next head's, before this one's sum
+            float r = 1.0f;
+            if (p.norm) {
+                for (int o = p.lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                r = rsqrtf(sum * over_d + p.eps);
             }
-            if (!p.interleaved && turn[n][0]) {
-                const int i = at[n][0] - p.start;
+            if (head >= heads) continue;
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float c = cos_s[i + e], s = sin_s[i + e], a = v[0][e], b = v[1][e];
-                    v[0][e] = a * c - b * s;
-                    v[1][e] = a * s + b * c;
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (at[n][h] < 0) continue;
-                if (p.interleaved && turn[n][h]) {
-                    const int i = (at[n][h] - p.start) / 2;
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        const float c = cos_s[i + e / 2], s = sin_s[i + e / 2], a = v[h][e], b = v[h][e + 1];
-                        v[h][e] = a * c - b * s;
-                        v[h][e + 1] = a * s + b * c;
+                    float &a = v[n][INTER ? e / 4 : 0][INTER ? e % 4 * 2 : e], &b = v[n][INTER ? e / 4 : 1][INTER ? e % 4 * 2 + 1 : e];
+                    const float x = a * r, y = b * r;
+                    a = x * fa[n][e];
+                    b = y * fd[n][e];
+                    if (turn[n][INTER ? e / 4 : 0]) {
+                        a = fmaf(-y, fb[n][e], a);
+                        b = fmaf(x, fc[n][e], b);
                     }
                 }
-                put8(p.y[which], F32 ? WS_ACT_F32 : WS_ACT_BF16, to + at[n][h], v[h]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (WHOLE || at[n][h] >= 0) put8(to, F32 ? WS_ACT_F32 : WS_ACT_BF16, at[n][h], v[n][h]);
             }
         }
     }
@@ -148,7 +185,7 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_any_kernel(const __grid_c
     const int t = blockIdx.x / p.groups, lane = threadIdx.x & 31, per = kHeadsThreads / 32, all = p.heads[0] + p.heads[1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     wait_predecessor();
-    heads_angles(p, t, cos_s, sin_s);
+    heads_angles(p, t, threadIdx.x, kHeadsThreads, cos_s, sin_s);
     __syncthreads();
     const int rot = 2 * p.pairs;
     for (int head = blockIdx.x % p.groups * per + (threadIdx.x >> 5); head < all; head += per * p.groups) {

@@ -15,11 +15,22 @@ namespace {
 bool aligned_to(const void *p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // ---- heads
+template <bool F32, bool INTER>
+ws_status_t launch_heads(const Err &err, int nu, bool whole, const HeadsParams &p, void *stream) {
+    const dim3 grid(p.teams > 1 ? (unsigned)((p.m + p.teams - 1) / p.teams) : (unsigned)p.m * p.groups);
+    if (nu == 1) return launch(err, whole ? heads_kernel<F32, INTER, 1, true> : heads_kernel<F32, INTER, 1, false>, grid, kHeadsThreads, 0, 1, stream, p);
+    return launch(err, nu == 2 ? heads_kernel<F32, INTER, 2, false> : heads_kernel<F32, INTER, 4, false>, grid, kHeadsThreads, 0, 1, stream, p);
+}
 template <bool F32>
-ws_status_t launch_heads(const Err &err, int nu, const HeadsParams &p, void *stream) {
-    const dim3 grid((unsigned)p.m * p.groups);
-    return nu == 1 ? launch(err, heads_kernel<F32, 1>, grid, kHeadsThreads, 0, 1, stream, p) : nu == 2 ? launch(err, heads_kernel<F32, 2>, grid, kHeadsThreads, 0, 1, stream, p)
-                                                                                               : launch(err, heads_kernel<F32, 4>, grid, kHeadsThreads, 0, 1, stream, p);
+ws_status_t launch_heads(const Err &err, int nu, bool whole, const HeadsParams &p, void *stream) {
+    return p.interleaved ? launch_heads<F32, true>(err, nu, whole, p, stream) : launch_heads<F32, false>(err, nu, whole, p, stream);
+}
+
+// ---- routes
+template <bool F32>
+ws_status_t launch_route(const Err &err, int n, dim3 grid, void *stream, const RouteParams &p) {
+    return launch(err, n <= 2 ? route_kernel<2, F32> : n <= 4 ? route_kernel<4, F32> : n <= 8 ? route_kernel<8, F32> : n <= 12 ? route_kernel<12, F32> : n <= 16 ? route_kernel<16, F32> : route_kernel<32, F32>,
+                  grid, kRouteThreads, 0, 1, stream, p);
 }
 
 // ---- logits
@@ -109,14 +120,17 @@ ws_status_t ws_head_norm_rope(const ws_head_norm_rope_args_t *a, void *stream, c
     const int halves = a->interleaved ? 0 : a->pairs / 8, all = halves + (a->d / 8 - 2 * halves + 1) / 2;
     p.lanes = 1;
     while (p.lanes < 32 && p.lanes < all) p.lanes *= 2;
+    const bool whole = all == p.lanes && a->d % 16 == 0;
     const int nu = (all + p.lanes - 1) / p.lanes, per = kHeadsThreads / (vec ? p.lanes : 32);
-    // a token's heads go to several blocks where tokens are few
-    const int rounds = (p.heads[0] + p.heads[1] + per - 1) / per;
-    p.groups = 1;
+    // A token's heads go to several blocks where tokens are few; where they are many, a block takes four, so that a lane has
+    // more heads for what it keeps of a token.
+    const int rounds = (std::max(p.heads[0], p.heads[1]) + per - 1) / per;
+    p.groups = p.teams = 1;
     while (p.groups < rounds && (int64_t)p.m * p.groups < 296) ++p.groups;
+    if (vec && p.m >= 4 * 296 && 4 * p.pairs <= WS_MAX_PAIRS) p.teams = 4;
     if ((int64_t)p.m * p.groups > INT32_MAX) return err(WS_ERR_INVALID, "m=%d out of range", a->m);
     if (!vec) return launch(err, heads_any_kernel, dim3((unsigned)p.m * p.groups), kHeadsThreads, 0, 1, stream, p);
-    return a->dtype == WS_ACT_F32 ? launch_heads<true>(err, nu, p, stream) : launch_heads<false>(err, nu, p, stream);
+    return a->dtype == WS_ACT_F32 ? launch_heads<true>(err, nu, whole, p, stream) : launch_heads<false>(err, nu, whole, p, stream);
 }
 
 ws_status_t ws_moe_route(const ws_moe_route_args_t *a, void *stream, char *err_text, size_t err_len) {
@@ -135,8 +149,7 @@ ws_status_t ws_moe_route(const ws_moe_route_args_t *a, void *stream, char *err_t
     p.m = a->m; p.experts = a->experts; p.top_k = a->top_k; p.score = a->score; p.dtype = a->dtype; p.renormalize = a->renormalize; p.scale = a->scale;
     const dim3 grid((unsigned)(((int64_t)a->m + kRouteThreads / 32 - 1) / (kRouteThreads / 32)));
     const int n = (a->experts + 31) / 32;
-    return launch(err, n <= 2 ? route_kernel<2> : n <= 4 ? route_kernel<4> : n <= 8 ? route_kernel<8> : n <= 12 ? route_kernel<12> : n <= 16 ? route_kernel<16> : route_kernel<32>,
-                  grid, kRouteThreads, 0, 1, stream, p);
+    return a->dtype == WS_ACT_F32 ? launch_route<true>(err, n, grid, stream, p) : launch_route<false>(err, n, grid, stream, p);
 }
 
 int64_t ws_moe_layer_workspace(int32_t m, int32_t top_k, int32_t hidden, int32_t inter) {   // hidden of the routes, their results

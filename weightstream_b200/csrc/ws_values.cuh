@@ -40,6 +40,14 @@ struct Eight {
             asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
                          : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(static_cast<const uint16_t *>(p) + i), "r"((int)ok) : "memory");
     }
+    __device__ __forceinline__ void load_all(const void *p, int64_t i) {  // (without the zeros)
+        if constexpr (F32)
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(static_cast<const float *>(p) + i) : "memory");
+        else
+            asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(static_cast<const uint16_t *>(p) + i) : "memory");
+    }
     __device__ __forceinline__ float get(int e) const {
         return __uint_as_float(F32 ? w[F32 ? e : 0] : e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
     }
