@@ -183,8 +183,30 @@ def test_a_token_repeated_very_often(dev):
 
 
 @pytest.mark.gpu
-def test_long_lists_of_biases(dev):
-    a = batch(13, 3, 700, F32, dev, biases=3000)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_lists_of_biases(dev, dtype):
+    check(batch(13, 3, 700, dtype, dev, biases=3000))
+    check(batch(14, 70, 20003, dtype, dev, biases=400))
+
+
+@pytest.mark.gpu
+def test_more_touched_values_than_are_noted(dev):
+    """A slice of a row where nearly every token has occurred, in batches of few and of many rows."""
+    for m, vocab in ((1, 5000), (80, 17000)):
+        a = batch(15, m, vocab, F32, dev, masks=3)
+        a["tokens"] = torch.arange(vocab - 7, dtype=torch.int32, device=dev).repeat(m)
+        a["offsets"] = torch.arange(m + 1, dtype=torch.int32, device=dev) * (vocab - 7)
+        check(a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [32767, 32768])
+def test_histories_around_the_short_ones(dev, length):
+    a = batch(16, 2, 300, BF16, dev)
+    a["tokens"] = torch.cat([torch.full((length,), 5, dtype=torch.int32, device=dev), torch.randint(0, 300, (length,), dtype=torch.int32, device=dev)])
+    a["offsets"] = torch.tensor([0, length, 2 * length], dtype=torch.int64, device=dev)
+    a["bias_offsets"] = a["bias_offsets"].to(torch.int32)
+    a["prompt_lens"] = torch.tensor([length, length // 2], dtype=torch.int32, device=dev)
     check(a)
 
 

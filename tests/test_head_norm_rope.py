@@ -108,6 +108,18 @@ def test_many_tokens(dev, m, hq, hk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rot,start,hq,hk", [(128, 128, 0, 9, 2), (512, 64, 448, 3, 1), (96, 32, 64, 5, 5), (64, 64, 0, 1, 17)])
+def test_blocks_of_several_tokens(dev, dtype, interleaved, d, rot, start, hq, hk):
+    rng = np.random.default_rng(d + hq)
+    row = made(rng, (1187, (hq + hk) * d), dtype, dev)
+    q, k = row[:, :hq * d].unflatten(1, (hq, d)), row[:, hq * d:].unflatten(1, (hk, d))
+    check(q, k, made(rng, (d,), BF16, dev), made(rng, (d,), BF16, dev), torch.from_numpy(rng.integers(0, 1 << 20, 1187)).to(dev), frequencies(rot // 2, dev),
+          rotary_start=start, interleaved=interleaved, q_out=q, k_out=k)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("positions", [[0, 1, 2 ** 20, 2 ** 24 + 1, 2 ** 31 - 1], [-1, -4097, 10 ** 6 + 1, 2 ** 30 + 3, 77]])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 def test_far_positions(dev, positions, dtype):

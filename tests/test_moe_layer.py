@@ -164,6 +164,15 @@ def test_widest_rows(dev, hidden, inter, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_passes_that_do_not_fit_together(dev, dtype):
+    """Blocks with several passes of many wide rows: shared memory holds one pass' rows at a time."""
+    Layer(2, 64, 7168, 32, 8, 8, dev, dtype, others=0.0).check()
+    Layer(3, 60, 5120, 96, 12, 8, dev, dtype, others=0.1).check(act_quant=True)
+    Layer(4, 64, 32, 4096, 40, 8, dev, dtype, others=0.0).check()
+
+
+@pytest.mark.gpu
 def test_halves_of_one_tensor_and_strided_rows(dev):
     l = Layer(3, 9, 288, 64, 4, 2, dev, fused=True)
     want = l.check()

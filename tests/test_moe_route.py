@@ -138,6 +138,12 @@ def test_masked_and_nan_experts(dev, score, biased):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("score", SCORES)
+def test_many_tokens(dev, score):
+    check(rows_of(8, 3001, 128, F32, dev), 8, score=score, bias=biases(8, 128, dev))
+
+
+@pytest.mark.gpu
 def test_no_rows(dev):
     from weightstream_b200 import ops
     ids, w = ops.moe_route(torch.empty((0, 8), device=dev), 3)

@@ -14,6 +14,10 @@
 // pass (most vectors of a warp have one, and all lanes wait for it) 6, 35 and 127; noted by who counts first 10, 29 and 86;
 // clusters of a row's slices that count into each other's tables 19, 52 and 169; a plain copy, and a hash table a row beside
 // or behind it 12, 33 and 91.
+//
+// Bound: instructions.  One row of 129280 with 6000 tokens 6.5 us, 64 rows with 4000, a mask and biases 27 us (10.3 of HBM),
+// 512 bf16 rows with 2000 and masks 85 us (41; without lists 46, with lists that touch nothing 73): a block's fixed part,
+// the lists that each of a row's sixteen blocks looks through, and the mask's bits.
 #pragma once
 
 #include "ws_values.cuh"
@@ -41,7 +45,7 @@ struct AdjustParams {
     const uint32_t *mask;                           // [mask_count, ld_mask] words, bit v % 32 of word v / 32: v is allowed
     const int32_t *mask_rows;                       // [m] or null: row t of the mask
     int64_t n_tokens, n_bias, ld_mask;
-    int32_t m, vocab, mask_count, offset_bytes, bias_offset_bytes, slices, in_place;
+    int32_t m, vocab, mask_count, offset_bytes, bias_offset_bytes, slices, in_place, bias_table;   // bias_table: a second table, of the biases' places
 };
 
 // Bounds of a row's entries, whatever the offsets hold.
@@ -138,7 +142,7 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
     const bool lists = p.tokens || p.bias_ids;
     if (lists) {
 #pragma unroll 1
-        for (int i = tid * 4; i < kSlice; i += kAdjustThreads * 4) *reinterpret_cast<uint4 *>(adjust_table + i) = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = tid * 4; i < (p.bias_table ? 2 * kSlice : kSlice); i += kAdjustThreads * 4) *reinterpret_cast<uint4 *>(adjust_table + i) = make_uint4(0u, 0u, 0u, 0u);
         if (tid == 0) touched_s = 0;
     }
     wait_predecessor();
@@ -166,8 +170,10 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
         uint32_t *const word = adjust_table + (low - v0);
         __syncthreads();
         if (bias1 > bias0)
-            adjust_list(p.bias_ids, bias0, bias1, [&](int64_t, int32_t v) {
-                if ((uint32_t)(v - low) < width) atomicOr(&word[v - low], kAdjustListed);
+            adjust_list(p.bias_ids, bias0, bias1, [&](int64_t i, int32_t v) {
+                if ((uint32_t)(v - low) >= width) return;
+                atomicOr(&word[v - low], kAdjustListed);
+                if (p.bias_table) atomicMax(&word[v - low + kSlice], (uint32_t)(i - bias0) + 1u);
             });
         if (b > a) {
             const int behind_at = p.prompt_lens ? p.prompt_lens[t] : 0;
@@ -242,8 +248,9 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
         if (!word || !adjust_open(mask, v)) continue;
         float z = load1(x, kType, v);
         if (word & kAdjustListed) {                 // its last entry
-            int64_t e = bias1;
-            while (e > bias0 && p.bias_ids[e - 1] != v) --e;
+            int64_t e = bias0 + adjust_table[at + (p.bias_table ? kSlice : 0)];
+            if (!p.bias_table)
+                for (e = bias1; e > bias0 && p.bias_ids[e - 1] != v;) --e;
             if (e > bias0) z += p.bias[e - 1];
         }
         const uint32_t behind = packed ? word & 0xFFFFu : word & (kAdjustPrompt - 1u);

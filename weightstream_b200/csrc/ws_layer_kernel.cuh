@@ -22,6 +22,16 @@
 // The second kernel's results of a route go to a workspace, and a third, small launch adds up a token's routes in the order
 // of its slots.  (Who brings the last of a token's routes adding them up in the second kernel took 40 to 90 us more with 48
 // to 96 routes: popular experts' blocks ended late.)
+//
+// Bound: HBM, and what stands before the streams.  One token of 7168 x 2048 through six experts 43 us, of which HBM needs 21:
+// routes, plan and activations 9, W1 and W3 17 (5.5 TB/s), the second kernel's beginning 6, W2 9 (4.9 TB/s), the sum 2.  48
+// routes of 30 experts 167 us (107), 96 of 42 236 us (150), fp32 activations rounded to E4M3, 28 routes of 20 experts of 5120
+// x 2304, 104 us (57).  At HBM's rate the issue slots, the conversions of codes and shared memory are each half to three
+// quarters busy: 30 instructions a lane for 16 codes, of which 8 convert, 2 multiply and 4 add.
+//
+// mma.sync and not tcgen05: its block-scaled form takes activations of 8 bits at most, so that a bf16 value held exactly
+// would be two columns and an fp32 value six, and sums over all of K are cut at every step there; the tensor pipe is a
+// quarter busy here.
 #pragma once
 
 #include <type_traits>
@@ -146,8 +156,10 @@ __device__ __forceinline__ int layer_cost(const LayerParams &p, int n) { return 
 // end; the fewer, the less often they join their sums.
 template <bool FIRST>
 __device__ __forceinline__ int layer_group(const LayerParams &p, int64_t all) {
-    const int chunks = (p.k + kLayerChunk - 1) / kLayerChunk, group = chunks >= 16 ? 4 : chunks >= 4 ? 2 : 1;
-    return all < (int64_t)gridDim.x * (kLayerWarps / group) * layer_cost<FIRST>(p, 1) ? 4 : group;
+    const int chunks = (p.k + kLayerChunk - 1) / kLayerChunk, each = (int)(all / gridDim.x) / layer_cost<FIRST>(p, 1);    // units a block
+    // (short rows, many units: a call of 48 routes of 30 experts 167 us with a unit a warp in the second kernel, 170 with two warps)
+    const int group = chunks >= 16 ? 4 : chunks >= 4 && each < 3 * kLayerWarps ? 2 : 1;
+    return each < kLayerWarps / group ? 4 : group;
 }
 
 template <bool FIRST>

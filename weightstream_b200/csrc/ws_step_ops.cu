@@ -37,14 +37,17 @@ ws_status_t launch_route(const Err &err, int n, dim3 grid, void *stream, const R
 template <bool F32, bool VEC, int U, int BLOCKS>
 ws_status_t launch_adjust(const Err &err, AdjustParams &p, void *stream) {
     constexpr int W = F32 ? 4 : 8, slice = kAdjustThreads * U * W;
-    if (slice * 4 > 40 * 1024) {                    // (48 KB with the list)
-        const ws_status_t st = allow_smem<adjust_kernel<F32, VEC, U, BLOCKS>>(err, slice * 4);
+    // The places of biases are looked for in the lists, or where these are long have a table of their own.
+    p.bias_table = p.n_bias / p.m > 128;
+    const int smem = p.tokens || p.bias_ids ? slice * (p.bias_table ? 8 : 4) : 0;
+    if (smem > 40 * 1024) {                         // (48 KB with the list)
+        const ws_status_t st = allow_smem<adjust_kernel<F32, VEC, U, BLOCKS>>(err, slice * 8);
         if (st != WS_OK) return st;
     }
     const int64_t slices = ((int64_t)p.vocab + (VEC ? W - 1 : 0) + slice - 1) / slice;
     if (slices * p.m > INT32_MAX) return err(WS_ERR_CAPACITY, "%d rows of %d logits: too many for one call", p.m, p.vocab);
     p.slices = (int)slices;
-    return launch(err, adjust_kernel<F32, VEC, U, BLOCKS>, dim3((unsigned)(slices * p.m)), kAdjustThreads, p.tokens || p.bias_ids ? slice * 4 : 0, 1, stream, p);
+    return launch(err, adjust_kernel<F32, VEC, U, BLOCKS>, dim3((unsigned)(slices * p.m)), kAdjustThreads, (size_t)smem, 1, stream, p);
 }
 template <bool F32, bool VEC>
 ws_status_t launch_adjust(const Err &err, AdjustParams &p, void *stream) {
