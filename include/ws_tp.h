@@ -363,7 +363,7 @@ typedef struct {
 } ws_moe_route_args_t;
 ws_status_t ws_moe_route(const ws_moe_route_args_t *args, void *stream, char *err, size_t err_len);
 
-/* A whole mixture-of-experts layer of a few tokens over MXFP4 experts, in two kernels:
+/* A whole mixture-of-experts layer of a few tokens over MXFP4 experts, in two kernels and a sum:
  *   g = w1[e] x[t], u = w3[e] x[t];  with limit > 0: g = min(g, limit), u = min(max(u, -limit), limit)
  *   out[t] = sum over t's routes (in the order of their slots) of w2[e] (weight * silu(g) * u)
  * Weights are packed E2M1 (low nibble = even K) with a UE8M0 byte per 32 values of K, as in ws_moe_down_combine_allreduce,

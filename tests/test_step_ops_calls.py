@@ -117,4 +117,50 @@ def test_null_arguments_and_no_rows():
     refused("ws_moe_route", fill(_lib.MoeRouteArgs, experts=8, top_k=1, dtype=1), _lib.WS_OK)
     refused("ws_moe_layer", fill(_lib.MoeLayerArgs, hidden=64, inter=32, top_k=1, e_len=1, x_dtype=1, out_dtype=1), _lib.WS_OK)
     refused("ws_adjust_logits", fill(_lib.AdjustLogitsArgs, vocab=8, dtype=1), _lib.WS_OK)
-    assert L.ws_moe_layer_workspace(0, 6, 64, 64) == 0 and L.ws_moe_layer_workspace(2, 3, 64, 32) > 0
+    assert L.ws_moe_layer_workspace(0, 6, 64, 64) == 0 and L.ws_moe_layer_workspace(2, 3, 64, 32) == 6 * 32 * 4 + 6 * 64 * 4
+
+
+FAR = (1 << 31) + 64        # elements of two bytes: rows that many apart are more than 2^32 bytes apart
+
+
+@pytest.fixture()
+def dev():
+    if not torch.cuda.is_available():
+        pytest.fail("a CUDA device is required for -m gpu tests")
+    return torch.device("cuda:0")
+
+
+def far_apart(t, stride):
+    """The same values, those of the first dimension `stride` elements apart."""
+    room = torch.empty(1 + (t.shape[0] - 1) * stride + sum((n - 1) * k for n, k in zip(t.shape[1:], t.stride()[1:])), dtype=t.dtype, device=t.device)
+    far = room.as_strided(t.shape, (stride, *t.stride()[1:]))
+    far.copy_(t)
+    return far
+
+
+@pytest.mark.gpu
+def test_rows_and_experts_past_32_bits(dev):
+    """Offsets that do not fit in 32 bits, in elements and in bytes: the results are those of compact tensors."""
+    from weightstream_b200 import ops
+    g = torch.Generator(dev).manual_seed(5)
+    normal = lambda *shape: torch.randn(shape, generator=g, device=dev).bfloat16()
+    whole = lambda lo, hi, *shape: torch.randint(lo, hi, shape, generator=g, device=dev, dtype=torch.uint8)
+    x = normal(2, 640)
+    mask = torch.randint(-2 ** 31, 2 ** 31 - 1, (2, 20), generator=g, device=dev, dtype=torch.int32)
+    tokens, offsets = torch.tensor([3, 3, 639, 5], dtype=torch.int32, device=dev), torch.tensor([0, 2, 4], dtype=torch.int32, device=dev)
+    how = dict(tokens=tokens, offsets=offsets, frequency=torch.full((2,), 0.5, device=dev), mask=mask)
+    assert torch.equal(ops.adjust_logits(far_apart(x, FAR), out=far_apart(x, FAR), **how), ops.adjust_logits(x, **how))
+    for got, want in zip(ops.moe_route(far_apart(x, FAR), 8), ops.moe_route(x, 8)):
+        assert torch.equal(got, want)
+    q = normal(2, 3, 128)
+    how = dict(positions=torch.tensor([7, 1000], dtype=torch.int32, device=dev), inv_freq=10000.0 ** (-torch.arange(64, device=dev) / 64))
+    assert torch.equal(ops.head_norm_rope(far_apart(q, FAR), q_out=far_apart(q, FAR), **how)[0], ops.head_norm_rope(q, **how)[0])
+    odd = q[:, :, :126]
+    how["inv_freq"] = how["inv_freq"][:63].contiguous()
+    assert torch.equal(ops.head_norm_rope(far_apart(odd, FAR), q_out=far_apart(odd, FAR), **how)[0], ops.head_norm_rope(odd, **how)[0])
+    x = normal(2, 256)
+    ids, w = torch.tensor([[0, 1], [1, 0]], dtype=torch.int32, device=dev), torch.rand((2, 2), generator=g, device=dev)
+    weights = [f(*shape) for shape, f in zip([(2, 64, 128), (2, 64, 8), (2, 64, 128), (2, 64, 8), (2, 256, 32), (2, 256, 2)], [lambda *n: whole(0, 256, *n), lambda *n: whole(126, 129, *n)] * 3)]
+    want = ops.moe_layer(x, ids, w, *weights)
+    far = [far_apart(t, 2 * FAR) for t in weights]
+    assert torch.equal(ops.moe_layer(far_apart(x, FAR), ids, w, *far, out=far_apart(torch.zeros_like(want), FAR)), want)

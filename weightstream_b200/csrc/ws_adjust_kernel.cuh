@@ -15,8 +15,8 @@
 // clusters of a row's slices that count into each other's tables 19, 52 and 169; a plain copy, and a hash table a row beside
 // or behind it 12, 33 and 91.
 //
-// Bound: instructions.  One row of 129280 with 6000 tokens 6.5 us, 64 rows with 4000, a mask and biases 27 us (10.3 of HBM),
-// 512 bf16 rows with 2000 and masks 85 us (41; without lists 46, with lists that touch nothing 73): a block's fixed part,
+// Bound: instructions.  One row of 129280 with 6000 tokens 6.2 to 7.1 us, 64 rows with 4000, a mask and biases 27 us (10.3 of HBM),
+// 512 bf16 rows with 2000 and masks 85 us (41; one call after the other 84, without lists 43, with lists of -1 69): a block's fixed part,
 // the lists that each of a row's sixteen blocks looks through, and the mask's bits.
 #pragma once
 
@@ -57,8 +57,8 @@ __device__ __forceinline__ void adjust_range(const void *offsets, int bytes, int
 }
 
 // f(entry, value) for the entries [a, b) of a list, by all threads of the block, four loads ahead.  (One copy of f: vectors of
-// entries and a loop unrolled over them made 36 copies of it, whose instructions had to be fetched first: one row with 6000
-// tokens 36 us.)
+// entries and a loop unrolled over them made 36 copies of it: one row with 6000 tokens took 36 us in an
+// early form, with one copy 28.)
 template <typename F>
 __device__ __forceinline__ void adjust_list(const int32_t *list, int64_t a, int64_t b, F f) {
     const int step = blockDim.x;

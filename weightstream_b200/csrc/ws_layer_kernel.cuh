@@ -24,8 +24,8 @@
 // to 96 routes: popular experts' blocks ended late.)
 //
 // Bound: HBM, and what stands before the streams.  One token of 7168 x 2048 through six experts 43 us, of which HBM needs 21:
-// routes, plan and activations 9, W1 and W3 17 (5.5 TB/s), the second kernel's beginning 6, W2 9 (4.9 TB/s), the sum 2.  48
-// routes of 30 experts 167 us (107), 96 of 42 236 us (150), fp32 activations rounded to E4M3, 28 routes of 20 experts of 5120
+// routes, plan and activations 8, W1 and W3 17 (5.6 TB/s), the second kernel's beginning 7, W2 9 (5.1 TB/s), the sum 2.  48
+// routes of 30 experts 165 to 170 us (107), 96 of 42 233 to 238 us (150), fp32 activations rounded to E4M3, 28 routes of 20 experts of 5120
 // x 2304, 104 us (57).  At HBM's rate the issue slots, the conversions of codes and shared memory are each half to three
 // quarters busy: 30 instructions a lane for 16 codes, of which 8 convert, 2 multiply and 4 add.
 //
@@ -157,7 +157,7 @@ __device__ __forceinline__ int layer_cost(const LayerParams &p, int n) { return 
 template <bool FIRST>
 __device__ __forceinline__ int layer_group(const LayerParams &p, int64_t all) {
     const int chunks = (p.k + kLayerChunk - 1) / kLayerChunk, each = (int)(all / gridDim.x) / layer_cost<FIRST>(p, 1);    // units a block
-    // (short rows, many units: a call of 48 routes of 30 experts 167 us with a unit a warp in the second kernel, 170 with two warps)
+    // (short rows, many units: a call of 48 routes of 30 experts 166 us with a unit a warp in the second kernel, 170 with two warps)
     const int group = chunks >= 16 ? 4 : chunks >= 4 && each < 3 * kLayerWarps ? 2 : 1;
     return each < kLayerWarps / group ? 4 : group;
 }

@@ -8,8 +8,8 @@
 // keys are taken again in 64 bits, so that the choice is the definition's and not that of a rounding.
 // Experts whose logit is -inf or NaN are never chosen; places that stay empty hold id -1 and weight 0.
 //
-// Bound: instructions (4096 tokens of 384 experts with a bias, top 8: 20.5 us, 1600 of them a token, of which the choice's
-// nine rounds are 700; HBM would need 1), the launch for few (64 tokens 5.1 us a call).
+// Bound: instructions (4096 tokens of 384 experts with a bias, top 8: 20 to 21 us, 1600 of them
+// a token; HBM would need 1), the launch for few (64 tokens 5.1 us a call).
 #pragma once
 
 #include "ws_values.cuh"

@@ -683,7 +683,7 @@ def moe_layer(x: torch.Tensor, route_ids: torch.Tensor, route_w: torch.Tensor, w
               s3: torch.Tensor, w2: torch.Tensor, s2: torch.Tensor, e_start: int = 0, *, limit: Optional[float] = None,
               act_quant: bool = False, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
               stream=None) -> torch.Tensor:
-    """A whole mixture-of-experts layer of a few tokens, in two kernels::
+    """A whole mixture-of-experts layer of a few tokens, in two kernels and a sum::
 
         g, u   = w1[e] @ x[t], w3[e] @ x[t]              with limit: min(g, limit), u between -limit and limit
         out[t] = sum over t's routes of w2[e] @ (route_w * silu(g) * u)
