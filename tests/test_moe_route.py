@@ -187,3 +187,36 @@ def test_too_many(dev, experts, top_k):
     from weightstream_b200 import ops
     with pytest.raises(ops.WsError, match="CAPACITY"):
         ops.moe_route(torch.zeros((3, experts), device=dev), top_k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [900.0, 1e4, 1e6, 1e9])
+@pytest.mark.parametrize("top_k", [1, 8])
+def test_biases_that_cancel_large_scores(dev, size, top_k):
+    """Keys near zero of scores whose own rounding in 32 bits is larger than what the keys differ by.  Weights: a root of
+    a value above 1 errs by 4 u, the others' arguments are 4 at most: (16 + 2 * 4 + top_k) u."""
+    from weightstream_b200 import ops
+    rng = np.random.default_rng(int(size) + top_k)
+    x = np.where(np.arange(80) < 64, size * (1 + rng.random(80)), -4 + rng.random(80)).astype(np.float32)
+    exact = lambda v: np.sqrt(np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v))))  # noqa: E731
+    step = np.where(np.arange(80) < 64, np.spacing(x), 2e-5)
+    x = (x + rng.integers(-8, 9, (60, 80)) * step).astype(np.float32)
+    bias = (-exact(x.astype(np.float64)).mean(0)).astype(np.float32)
+    ids, w = ops.moe_route(torch.from_numpy(x).to(dev), top_k, score="sqrtsoftplus", bias=torch.from_numpy(bias).to(dev))
+    s = exact(x.astype(np.float64))
+    for t in range(60):
+        want = np.lexsort((np.arange(80), -(s[t] + bias.astype(np.float64))))[:top_k]
+        assert ids[t].tolist() == want.tolist(), t
+        ww = s[t, want] / s[t, want].sum()
+        assert (np.abs(w[t].double().cpu().numpy() - ww) <= (24 + top_k) * U * ww).all(), t
+
+
+@pytest.mark.gpu
+def test_one_large_score_among_small_ones(dev):
+    """The first expert's key is the second largest, whichever way its score's root is rounded to 32 bits."""
+    from weightstream_b200 import ops
+    x = torch.tensor([[1000000.0625, -4.0, -4.0]], device=dev)
+    bias = torch.tensor([-1000.0, -0.13467541, -0.13470542], device=dev)
+    for top_k in (1, 2, 3):
+        ids, _ = ops.moe_route(x, top_k, score="sqrtsoftplus", bias=bias)
+        assert ids[0].tolist() == [1, 0, 2][:top_k]

@@ -5,7 +5,8 @@
 //
 // A warp takes a token, its logits in registers.  Without a bias the order is that of the logits themselves.  With one,
 // keys are compared in 32 bits first; where two neighbours of the order lie as close as their errors, the candidates'
-// keys are taken again in 64 bits, so that the choice is the definition's and not that of a rounding.
+// keys are taken again in 64 bits, so that the choice is the definition's and not that of a rounding.  Errors go by the
+// largest score of the token, chosen or not: a bias may cancel a score of any size and leave its rounding.
 // Experts whose logit is -inf or NaN are never chosen; places that stay empty hold id -1 and weight 0.
 //
 // Bound: instructions (4096 tokens of 384 experts with a bias, top 8: 20 to 21 us, 1600 of them
@@ -18,7 +19,7 @@ namespace ws {
 
 constexpr int kRouteThreads = 128;
 static_assert(WS_ROUTE_MAX_TOP_K == 32 && WS_ROUTE_MAX_EXPERTS <= 32 * 32, "a lane keeps one result, and 32 logits");
-constexpr float kRouteNear = 4e-6f;     // keys whose difference is below this share of theirs: compared in 64 bits
+constexpr float kRouteNear = 4e-6f;     // keys that differ by less than this share of them, of the largest score or of 1: compared in 64 bits
 
 struct RouteParams {
     const void *logits;
@@ -99,6 +100,14 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     const float over = 1.0f / total;
+    // No score is above this: sqrt(ln(1 + e^l)) <= sqrt(max(l, 0) + 1).
+    float reach = 1.0f;
+    if (p.bias && p.score == WS_SCORE_SQRTSOFTPLUS) {
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) big = fmaxf(big, l[i]);
+        reach = sqrtf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))) + 1.0f);
+    }
     uint32_t key[N];
     bool fine = true;                   // no two neighbours of the order are too close
 #pragma unroll
@@ -130,7 +139,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
         const int e = __reduce_min_sync(0xffffffffu, at);
         if (p.bias) {
             const float v = route_unorder(k);
-            if (j && before - v <= kRouteNear * fmaxf(1.0f, fabsf(v))) fine = false;
+            if (j && before - v <= kRouteNear * fmaxf(reach, fabsf(v))) fine = false;
             before = v;
         }
         if (j == p.top_k) break;
@@ -146,7 +155,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
         }
     }
     if (p.bias && !fine) {              // (all lanes alike; rare, so the logits are read again)
-        const float bound = last - kRouteNear * fmaxf(1.0f, fabsf(last));
+        const float bound = last - kRouteNear * fmaxf(reach, fabsf(last));
         auto logit = [&](int i) { return i * 32 + lane < p.experts ? load1(p.logits, p.dtype, row + i * 32 + lane) : -__builtin_huge_valf(); };
         double total64 = 1.0;
         if (soft) {
