@@ -347,7 +347,8 @@ ws_status_t ws_head_norm_rope(const ws_head_norm_rope_args_t *args, void *stream
  *   score = softmax(logits), sigmoid(logits) or sqrt(ln(1 + exp(logits)));  key = score + bias (score without one)
  *   ids = the top_k experts by key, larger first and equal ones by index
  *   weights = scale * score, with renormalize divided by the sum of the chosen scores
- * Experts whose logit is -inf or NaN, or whose key is NaN, are never chosen; places that stay empty hold id -1 and weight 0.
+ * Experts whose logit is -inf or NaN, or whose key is NaN (all of a row's with softmax and a logit of +inf), are never chosen; places
+ * that stay empty hold id -1 and weight 0.
  * The order is that of the definition: near ones are compared in 64 bits.  (Takes the place of the reference's `moe_select`.) */
 enum { WS_SCORE_SOFTMAX = 0, WS_SCORE_SIGMOID = 1, WS_SCORE_SQRTSOFTPLUS = 2 };
 #define WS_ROUTE_MAX_EXPERTS 1024

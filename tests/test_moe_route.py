@@ -220,3 +220,18 @@ def test_one_large_score_among_small_ones(dev):
     for top_k in (1, 2, 3):
         ids, _ = ops.moe_route(x, top_k, score="sqrtsoftplus", bias=bias)
         assert ids[0].tolist() == [1, 0, 2][:top_k]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_softmax_that_is_no_number_chooses_none(dev, biased, renormalize, dtype):
+    """With a logit of +inf every score of the row is NaN."""
+    from weightstream_b200 import ops
+    x = rows_of(9, 4, 40, dtype, dev)
+    x[1, 7] = x[3, 0] = x[3, 39] = math.inf
+    how = dict(score="softmax", bias=biases(9, 40, dev) if biased else None, renormalize=renormalize)
+    ids, w = ops.moe_route(x, 6, **how)
+    assert (ids[[1, 3]] == -1).all() and (w[[1, 3]] == 0).all()
+    check(x[[0, 2]], 6, **how)

@@ -120,6 +120,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     int mine = -1;                      // lane j: the j-th expert
     float before = __builtin_huge_valf(), last = 0.0f;
     const int rounds = p.top_k + (p.bias ? 1 : 0);      // one more: how close the first that is left out comes
+    // A softmax over a logit of +inf is NaN for all; with a bias the keys are, without one they are the logits.
+    const uint32_t none = soft && !p.bias ? route_order(__builtin_huge_valf()) : 0u;
     uint32_t best = 0u;                 // of this lane's keys that are left
     uint32_t left[N];
 #pragma unroll
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 #pragma unroll 1
     for (int j = 0; j < rounds; ++j) {
         const uint32_t k = __reduce_max_sync(0xffffffffu, best);
-        if (!k) break;
+        if (!k || k == none) break;
         int at = 0x7fffffff;            // its place, where this lane has it
         if (best == k) {
 #pragma unroll

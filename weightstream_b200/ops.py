@@ -609,7 +609,8 @@ def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias:
     ``"softmax"``, ``"sigmoid"`` or ``"sqrtsoftplus"`` of the logits.  A weight is ``scale * score``, with ``renormalize`` over the
     sum of the chosen scores.  The choice is that of exact scores: near ones are compared in 64 bits.
 
-    Experts whose logit is -inf or NaN, or whose key is NaN, are never chosen; places that stay empty hold id -1 and weight 0.
+    Experts whose logit is -inf or NaN, or whose key is NaN (all of a row's with softmax and a logit of +inf), are never chosen;
+    places that stay empty hold id -1 and weight 0.
     """
     r = (_native or _load()).moe_route(logits, top_k, _SCORES.get(score, -1), bias, renormalize, scale, _handle(stream, logits))
     if r is not None:
