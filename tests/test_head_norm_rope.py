@@ -223,3 +223,14 @@ def test_host_tensors_are_refused():
     from weightstream_b200 import ops
     with pytest.raises(ValueError, match="CUDA"):
         ops.head_norm_rope(**arguments())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start", [2 ** 31, 2 ** 32, -2 ** 32, 2 ** 32 + 8, 2 ** 62, 2 ** 70, -2 ** 70])
+def test_starts_beyond_32_bits_are_refused(dev, start):
+    from weightstream_b200 import ops
+    a = {k: v.to(dev) for k, v in arguments().items()}
+    with pytest.raises(ValueError, match="not within"):
+        ops.head_norm_rope(**{**a, "inv_freq": torch.ones(4, device=dev)}, rotary_start=start)
+    q, _ = ops.head_norm_rope(torch.ones((3, 2, 16), device=dev), rotary_start=start)      # (without positions there is no part)
+    assert (q - 1).abs().max() < 1e-6

@@ -295,6 +295,14 @@ bool rows(const at::Tensor *t, const at::Tensor &like, int64_t m, int64_t n, int
 bool vec(const at::Tensor *t, const at::Tensor &like, int64_t n) {
     return t && t->dim() == 1 && t->size(0) == n && t->is_contiguous() && t->device() == like.device();
 }
+// A whole number of [0, INT32_MAX]; false for others, which the Python layer refuses or ignores.
+bool word(PyObject *o, int32_t *out) {
+    int beyond = 0;
+    const long v = PyLong_AsLongAndOverflow(o, &beyond);
+    if (beyond || v < 0 || v > INT32_MAX) return false;     // (-1 with an error set, where it is none)
+    *out = (int32_t)v;
+    return true;
+}
 // A result type as Python names it; None stands for `otherwise`.
 bool result_dtype(PyObject *o, at::ScalarType otherwise, at::ScalarType *out, int32_t *code) {
     if (o != Py_None && !THPDtype_Check(o)) return false;
@@ -542,15 +550,16 @@ PyObject *py_head_norm_rope(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     }
     a.position_bytes = 8;
     if ((v[2] == Py_None) != (v[3] == Py_None)) Py_RETURN_NONE;
-    a.start = (int32_t)PyLong_AsLong(v[9]);
     if (v[2] != Py_None) {
+        if (!word(v[9], &a.start)) {
+            if (PyErr_Occurred()) return nullptr;
+            Py_RETURN_NONE;
+        }
         const at::Tensor *pos = tensor(v[2]), *inv = tensor(v[3]);
         if (!vec(pos, *q, m) || (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong)) Py_RETURN_NONE;
         if (!inv || inv->dim() != 1 || inv->size(0) < 1 || inv->size(0) > WS_MAX_PAIRS || !vec(inv, *q, inv->size(0)) || inv->scalar_type() != at::kFloat) Py_RETURN_NONE;
         a.positions = pos->data_ptr(); a.position_bytes = (int32_t)pos->element_size();
         a.inv_freq = inv->data_ptr<float>(); a.pairs = (int32_t)inv->size(0);
-    } else {
-        a.start = 0;
     }
     a.norm = PyObject_IsTrue(v[6]); a.interleaved = PyObject_IsTrue(v[10]);
     a.eps = (float)PyFloat_AsDouble(v[7]); a.weight_offset = (float)PyFloat_AsDouble(v[8]); a.scale = (float)PyFloat_AsDouble(v[11]);
