@@ -164,3 +164,18 @@ def test_rows_and_experts_past_32_bits(dev):
     want = ops.moe_layer(x, ids, w, *weights)
     far = [far_apart(t, 2 * FAR) for t in weights]
     assert torch.equal(ops.moe_layer(far_apart(x, FAR), ids, w, *far, out=far_apart(torch.zeros_like(want), FAR)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [2 ** 31, 2 ** 32 + 1, 2 ** 63, -2 ** 70])
+def test_whole_numbers_beyond_a_word_are_value_errors(dev, value):
+    """Of device tensors too, which the native front end takes first."""
+    from weightstream_b200 import ops
+    f, args = calls()["moe_layer"]
+    args = {k: v.to(dev) for k, v in args.items()}
+    with pytest.raises(ValueError, match="e_start"):
+        f(**args, e_start=value)
+    with pytest.raises(ValueError, match="top_k"):
+        ops.moe_route(args["x"], value)
+    with pytest.raises(ValueError, match="top"):
+        ops.token_logprobs(args["x"], torch.zeros(3, dtype=torch.int32, device=dev), top=value)

@@ -303,6 +303,11 @@ bool word(PyObject *o, int32_t *out) {
     *out = (int32_t)v;
     return true;
 }
+// What a function returns of an argument that it does not take: the error that is set, or None.
+PyObject *explained() {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+}
 // A result type as Python names it; None stands for `otherwise`.
 bool result_dtype(PyObject *o, at::ScalarType otherwise, at::ScalarType *out, int32_t *code) {
     if (o != Py_None && !THPDtype_Check(o)) return false;
@@ -394,15 +399,15 @@ PyObject *py_token_logprobs(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (nargs != 4) { PyErr_SetString(PyExc_TypeError, "token_logprobs takes 4 arguments"); return nullptr; }
     const at::Tensor *x = tensor(v[0]), *tok = tensor(v[1]);
-    const long top = PyLong_AsLong(v[2]);
-    if (PyErr_Occurred()) return nullptr;
-    if (!x || !tok || x->dim() != 2 || top < 0 || top > WS_MAX_TOP) Py_RETURN_NONE;
     ws_token_logprobs_args_t a{};
+    if (!word(v[2], &a.top)) return explained();
+    const int32_t top = a.top;
+    if (!x || !tok || x->dim() != 2 || top > WS_MAX_TOP) Py_RETURN_NONE;
     const int64_t m = x->size(0), vocab = x->size(1);
     if (m > INT32_MAX || vocab > INT32_MAX || !rows(x, *x, m, vocab, &a.ld) || !act_dtype(*x, &a.dtype) || !vec(tok, *x, m)) Py_RETURN_NONE;
     if (tok->scalar_type() != at::kInt && tok->scalar_type() != at::kLong) Py_RETURN_NONE;
     a.logits = x->data_ptr(); a.tokens = tok->data_ptr(); a.token_bytes = (int32_t)tok->element_size();
-    a.m = (int32_t)m; a.vocab = (int32_t)vocab; a.top = (int32_t)top;
+    a.m = (int32_t)m; a.vocab = (int32_t)vocab;
     CallOn on(*x, v[3]);
     if (PyErr_Occurred()) return nullptr;
     at::Tensor out[5];
@@ -551,10 +556,7 @@ PyObject *py_head_norm_rope(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     a.position_bytes = 8;
     if ((v[2] == Py_None) != (v[3] == Py_None)) Py_RETURN_NONE;
     if (v[2] != Py_None) {
-        if (!word(v[9], &a.start)) {
-            if (PyErr_Occurred()) return nullptr;
-            Py_RETURN_NONE;
-        }
+        if (!word(v[9], &a.start)) return explained();
         const at::Tensor *pos = tensor(v[2]), *inv = tensor(v[3]);
         if (!vec(pos, *q, m) || (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong)) Py_RETURN_NONE;
         if (!inv || inv->dim() != 1 || inv->size(0) < 1 || inv->size(0) > WS_MAX_PAIRS || !vec(inv, *q, inv->size(0)) || inv->scalar_type() != at::kFloat) Py_RETURN_NONE;
@@ -587,13 +589,13 @@ PyObject *py_moe_route(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (nargs != 7) { PyErr_SetString(PyExc_TypeError, "moe_route takes 7 arguments"); return nullptr; }
     const at::Tensor *x = tensor(v[0]);
-    const long top = PyLong_AsLong(v[1]), score = PyLong_AsLong(v[2]);
-    if (PyErr_Occurred()) return nullptr;
-    if (!x || x->dim() != 2) Py_RETURN_NONE;
     ws_moe_route_args_t a{};
+    if (!word(v[1], &a.top_k) || !word(v[2], &a.score)) return explained();    // (an unknown score is -1)
+    const int32_t top = a.top_k;
+    if (!x || x->dim() != 2) Py_RETURN_NONE;
     const int64_t m = x->size(0), n = x->size(1);
     if (m > INT32_MAX || n > INT32_MAX || !rows(x, *x, m, n, &a.ld) || !act_dtype(*x, &a.dtype) || top < 1 || top > n || top > WS_ROUTE_MAX_TOP_K) Py_RETURN_NONE;
-    a.logits = x->data_ptr(); a.m = (int32_t)m; a.experts = (int32_t)n; a.top_k = (int32_t)top; a.score = (int32_t)score;
+    a.logits = x->data_ptr(); a.m = (int32_t)m; a.experts = (int32_t)n;
     if (v[3] != Py_None) {
         const at::Tensor *b = tensor(v[3]);
         if (!vec(b, *x, n) || b->scalar_type() != at::kFloat) Py_RETURN_NONE;
@@ -641,14 +643,14 @@ PyObject *py_moe_layer(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
         !experts(tensor(v[5]), *x, n, f, h / 2, &a.w3, &a.w3_stride) || !experts(tensor(v[6]), *x, n, f, h / 32, &a.s3, &a.s3_stride) ||
         !experts(tensor(v[7]), *x, n, h, f / 2, &a.w2, &a.w2_stride) || !experts(tensor(v[8]), *x, n, h, f / 32, &a.s2, &a.s2_stride))
         Py_RETURN_NONE;
-    const long start = PyLong_AsLong(v[9]);
+    if (!word(v[9], &a.e_start)) return explained();
     a.limit = (float)PyFloat_AsDouble(v[10]);
     a.act_quant = PyObject_IsTrue(v[11]);
     if (PyErr_Occurred()) return nullptr;
     at::ScalarType type = at::kFloat;
-    if (start < 0 || start > INT32_MAX || !(a.limit >= 0.0f) || (v[12] == Py_None && !result_dtype(v[13], at::kFloat, &type, &a.out_dtype))) Py_RETURN_NONE;
+    if (!(a.limit >= 0.0f) || (v[12] == Py_None && !result_dtype(v[13], at::kFloat, &type, &a.out_dtype))) Py_RETURN_NONE;
     a.x = x->data_ptr(); a.route_ids = ids->data_ptr<int32_t>(); a.route_w = w->data_ptr<float>();
-    a.m = (int32_t)m; a.hidden = (int32_t)h; a.inter = (int32_t)f; a.top_k = (int32_t)k; a.e_start = (int32_t)start; a.e_len = (int32_t)n;
+    a.m = (int32_t)m; a.hidden = (int32_t)h; a.inter = (int32_t)f; a.top_k = (int32_t)k; a.e_len = (int32_t)n;
     CallOn on(*x, v[14]);
     if (PyErr_Occurred()) return nullptr;
     at::Tensor made, work;
