@@ -339,3 +339,20 @@ def test_host_tensors_are_refused():
     from weightstream_b200 import ops
     with pytest.raises(ValueError, match="CUDA"):
         ops.moe_layer(**arguments())
+
+
+@pytest.mark.parametrize("limit", [1e-46, 1e-60, 5e-324])
+def test_limits_that_are_nothing_in_32_bits_are_refused(limit):
+    from weightstream_b200 import ops
+    with pytest.raises(ValueError, match="limit"):
+        ops.moe_layer(**arguments(), limit=limit)
+
+
+@pytest.mark.gpu
+def test_the_smallest_limits(dev):
+    from weightstream_b200 import ops
+    l = Layer(20, 4, 64, 32, 2, 2, dev, others=0.0)
+    l.check(limit=2.0 ** -100)
+    for limit in (1e-46, 5e-324):
+        with pytest.raises(ValueError, match="limit"):
+            l.call(limit=limit)

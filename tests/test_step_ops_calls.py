@@ -179,3 +179,9 @@ def test_whole_numbers_beyond_a_word_are_value_errors(dev, value):
         ops.moe_route(args["x"], value)
     with pytest.raises(ValueError, match="top"):
         ops.token_logprobs(args["x"], torch.zeros(3, dtype=torch.int32, device=dev), top=value)
+
+
+def test_layer_entry_refuses_a_limit_that_is_no_number():
+    base = dict(x=P, ldx=64, route_ids=P, route_w=P, w1=P, s1=P, w3=P, s3=P, w2=P, s2=P, w1_stride=1024, s1_stride=64, w3_stride=1024, s3_stride=64, w2_stride=1024, s2_stride=64,
+                out=P, ldo=64, workspace=P, workspace_bytes=1 << 20, m=3, hidden=64, inter=32, top_k=2, e_len=4, x_dtype=1, out_dtype=1, limit=float("nan"))
+    refused("ws_moe_layer", fill(_lib.MoeLayerArgs, **base), text="limit")

@@ -168,6 +168,7 @@ ws_status_t ws_moe_layer(const ws_moe_layer_args_t *a, void *stream, char *err_t
         return err(WS_ERR_INVALID, "m=%d top_k=%d hidden=%d inter=%d: widths are multiples of 32", a->m, a->top_k, a->hidden, a->inter);
     if (a->e_len < 1 || a->e_start < 0) return err(WS_ERR_INVALID, "bad local expert range");
     if (!is_type(a->x_dtype) || !is_type(a->out_dtype)) return err(WS_ERR_INVALID, "unknown type of a tensor");
+    if (a->limit != a->limit) return err(WS_ERR_INVALID, "limit is no number");
     if (a->top_k > kLayerMaxTopK || (int64_t)a->m * a->top_k > kLayerMaxRoutes) return err(WS_ERR_CAPACITY, "m*top_k = %d*%d exceeds %d routes per call", a->m, a->top_k, kLayerMaxRoutes);
     if (a->e_len > kLayerMaxExperts || a->hidden > kLayerMaxWidth || a->inter > kLayerMaxWidth)
         return err(WS_ERR_CAPACITY, "%d experts of %d x %d: at most %d of %d", a->e_len, a->hidden, a->inter, kLayerMaxExperts, kLayerMaxWidth);

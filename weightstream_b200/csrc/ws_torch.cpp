@@ -644,11 +644,12 @@ PyObject *py_moe_layer(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
         !experts(tensor(v[7]), *x, n, h, f / 2, &a.w2, &a.w2_stride) || !experts(tensor(v[8]), *x, n, h, f / 32, &a.s2, &a.s2_stride))
         Py_RETURN_NONE;
     if (!word(v[9], &a.e_start)) return explained();
-    a.limit = (float)PyFloat_AsDouble(v[10]);
+    const double limit = PyFloat_AsDouble(v[10]);
+    a.limit = (float)limit;
     a.act_quant = PyObject_IsTrue(v[11]);
     if (PyErr_Occurred()) return nullptr;
     at::ScalarType type = at::kFloat;
-    if (!(a.limit >= 0.0f) || (v[12] == Py_None && !result_dtype(v[13], at::kFloat, &type, &a.out_dtype))) Py_RETURN_NONE;
+    if (!(a.limit >= 0.0f) || (limit != 0.0 && a.limit == 0.0f) || (v[12] == Py_None && !result_dtype(v[13], at::kFloat, &type, &a.out_dtype))) Py_RETURN_NONE;
     a.x = x->data_ptr(); a.route_ids = ids->data_ptr<int32_t>(); a.route_w = w->data_ptr<float>();
     a.m = (int32_t)m; a.hidden = (int32_t)h; a.inter = (int32_t)f; a.top_k = (int32_t)k; a.e_len = (int32_t)n;
     CallOn on(*x, v[14]);

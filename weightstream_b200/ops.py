@@ -667,8 +667,8 @@ def _moe_layer_args(x, route_ids, route_w, w1, s1, w3, s3, w2, s2, e_start, limi
         for what, t, stride in (("w", w, strides[0]), ("s", s, strides[1])):
             setattr(a, what + name, t.data_ptr())
             setattr(a, what + name + "_stride", stride)
-    if limit is not None and not limit > 0.0:
-        raise ValueError(f"limit must be positive, got {limit}")
+    if limit is not None and not C.c_float(limit).value > 0.0:
+        raise ValueError(f"limit must be positive in 32 bits, got {limit}")
     a.limit, a.act_quant = limit or 0.0, bool(act_quant)
     dtype = out.dtype if out is not None else out_dtype
     if dtype not in _TYPES:
