@@ -268,3 +268,62 @@ def test_host_tensors_are_refused():
     from weightstream_b200 import ops
     with pytest.raises(ValueError, match="CUDA"):
         ops.adjust_logits(**arguments())
+
+
+def lopsided(seed, m, vocab, length, dtype, dev, *, row=1, others=0, pad=0, **how):
+    """A batch in which one row lists `length` biases and the others few or none."""
+    rng = np.random.default_rng(seed)
+    a = batch(seed, m, vocab, dtype, dev, biases=0, pad=pad, **how)
+    n = np.full(m, others)
+    n[row] = length
+    ids = rng.integers(-1, vocab + 1, int(n.sum()))
+    put = lambda v, t: torch.from_numpy(np.asarray(v)).to(t).to(dev)  # noqa: E731
+    a.update(bias_ids=put(ids, torch.int32), bias=put(rng.standard_normal(ids.size) * 5, F32), bias_offsets=put(np.concatenate([[0], np.cumsum(n)]), torch.int32))
+    return a
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,vocab,length,others", [(2, 700, 200, 0), (9, 2500, 1000, 3), (40, 20003, 4000, 7), (100, 20003, 9000, 2), (300, 4111, 30000, 0), (500, 8192, 20000, 20),
+                                                   (7, 129, 700, 1)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_one_long_list_of_biases(dev, dtype, m, vocab, length, others, pad):
+    a = lopsided(m + length, m, vocab, length, dtype, dev, others=others, pad=pad, row=m - 1)
+    got = check(a)
+    b = {**a, "logits": a["logits"].clone()}
+    assert torch.equal(check(b, out=b["logits"]), got)
+    check(lopsided(m, m, vocab, length, dtype, dev, others=others, row=0, history=0, masks=0))
+
+
+@pytest.mark.gpu
+def test_the_last_entry_counts_in_a_long_list(dev):
+    for length in (129, 5000):
+        a = lopsided(17, 64, 3000, length, F32, dev, history=0, masks=0)
+        a["bias_ids"][:] = torch.arange(length, dtype=torch.int32, device=dev) % 3      # every entry but the last three is overtaken
+        check(a)
+
+
+@pytest.mark.gpu
+def test_one_long_list_among_many_rows_takes_no_longer_than_it_is(dev):
+    """One of 512 rows lists 50000 tokens, or all rows list 97 each.  A block that goes through the list a constant number of
+    times takes some hundred rounds of its threads for it; one that looks for each of its listed values in the whole list takes as
+    many times that as it has values for a thread."""
+    from weightstream_b200 import ops
+    a = lopsided(18, 512, 50000, 50000, BF16, dev, history=0, masks=0)
+    a["bias_ids"] = torch.randperm(50000, device=dev).to(torch.int32)
+    b = {**a, "bias_offsets": torch.arange(513, dtype=torch.int32, device=dev) * 97}
+
+    def elapsed(how):
+        times = []
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            ops.adjust_logits(**how)
+            begin.record()
+            for _ in range(5):
+                ops.adjust_logits(**how)
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times)
+
+    assert elapsed(a) < 8 * elapsed(b), (elapsed(a), elapsed(b))

@@ -30,6 +30,10 @@ constexpr int kAdjustList = 2048;                   // touched places that are n
 // histories: 30 an occurrence in the prompt, 29 to 0 occurrences behind it.
 constexpr uint32_t kAdjustListed = 0x80000000u, kAdjustPrompt = 0x40000000u;
 constexpr int kAdjustShort = 32767;
+// A row's list of biases is looked through for each of its listed values up to this length; longer ones have their places in a
+// table.  Lists of 32, 64 and 128 in all rows, us, looked through / in a second table: 64 fp32 rows 15.2 / 15.2, 19.3 / 15.6
+// and 28 / 15.6, 512 bf16 rows with 2000 tokens each 91 / 118, 114 / 120 and 166 / 122.
+constexpr int kAdjustFew = 64;
 
 struct AdjustParams {
     const void *logits;
@@ -123,6 +127,90 @@ __device__ __forceinline__ void adjust_close(uint32_t &w, uint32_t bits) {
     }
 }
 
+// A row of a block: its lists, its mask, where its slice begins.
+struct AdjustRow {
+    const AdjustParams &p;
+    int t, v0;                                      // v0: the token of the slice's first place
+    int64_t a, b, bias0, bias1;
+
+    __device__ __forceinline__ AdjustRow(const AdjustParams &p, int t, int v0) : p(p), t(t), v0(v0), a(0), b(0), bias0(0), bias1(0) {
+        if (p.tokens) adjust_range(p.offsets, p.offset_bytes, t, p.n_tokens, a, b);
+        if (p.bias_ids) adjust_range(p.bias_offsets, p.bias_offset_bytes, t, p.n_bias, bias0, bias1);
+    }
+    __device__ __forceinline__ bool packed() const { return b - a <= kAdjustShort; }    // (the block's conditions)
+    // Counts the lists' tokens of `span` places from `from` on into the table, and with `last` the places of biases from that
+    // word of it on.
+    __device__ __forceinline__ void count(uint32_t *table, int from, int span, int last) const {
+        const int low = max(v0 + from, 0);          // those tokens: low and `width` behind it
+        const uint32_t width = (uint32_t)max(0, min(v0 + from + span, p.vocab) - low);
+        uint32_t *const word = table + (low - v0 - from);
+        if (bias1 > bias0)
+            adjust_list(p.bias_ids, bias0, bias1, [&](int64_t i, int32_t v) {
+                if ((uint32_t)(v - low) >= width) return;
+                atomicOr(&word[v - low], kAdjustListed);
+                if (last) atomicMax(&word[v - low + last], (uint32_t)(i - bias0) + 1u);
+            });
+        if (b > a) {
+            const int behind_at = p.prompt_lens ? p.prompt_lens[t] : 0;
+            const int64_t prompt = a + behind_at;
+            if (packed())
+                adjust_tokens(p.tokens + a, (int)(b - a), [&](int i, int32_t v) {
+                    if ((uint32_t)(v - low) < width) atomicAdd(&word[v - low], i < behind_at ? 0x10000u : 1u);
+                });
+            else
+                adjust_list(p.tokens, a, b, [&](int64_t i, int32_t v) {
+                    if ((uint32_t)(v - low) >= width) return;
+                    if (i < prompt) atomicOr(&word[v - low], kAdjustPrompt);
+                    else atomicAdd(&word[v - low], 1u);
+                });
+        }
+    }
+    // What becomes of the value of token v, whose word of the table is `word`; `listed`: its bias' place and one more, 0 where
+    // that is still to be looked for.
+    __device__ __forceinline__ void change(const char *x, char *y, int type, int v, uint32_t word, uint32_t listed, float rep, float freq, float pres) const {
+        float z = load1(x, type, v);
+        if (word & kAdjustListed) {                 // its last entry
+            int64_t e = bias0 + listed;
+            if (!listed)
+                for (e = bias1; e > bias0 && p.bias_ids[e - 1] != v;) --e;
+            if (e > bias0) z += p.bias[e - 1];
+        }
+        const uint32_t behind = packed() ? word & 0xFFFFu : word & (kAdjustPrompt - 1u);
+        if (word & ~kAdjustListed) z = z > 0.0f ? __fdiv_rn(z, rep) : z * rep;
+        if (behind) z = fmaf(-freq, (float)behind, z) - pres;
+        store1(y, type, v, z);
+    }
+    __device__ __forceinline__ float of(const float *values, float otherwise) const { return values && b > a ? values[t] : otherwise; }
+};
+
+// The touched values of a slice whose row has a long list of biases in a batch of short ones, after its logits have been
+// stored: in halves, so that the table's second half has room for the places of the first one's biases.  Every place of the table is
+// looked at.  (A function of its own: as a branch of the kernel it cost all other rows 2 to 6 %.)
+template <bool F32, int SLICE>
+__device__ __noinline__ void adjust_halves(const AdjustParams &p, uint32_t *table, int t, int v0) {
+    const AdjustRow r(p, t, v0);
+    const uint32_t *const mask = adjust_mask(p, t);
+    const char *const x = static_cast<const char *>(p.logits) + (int64_t)t * p.ld * (F32 ? 4 : 2);
+    char *const y = static_cast<char *>(p.out) + (int64_t)t * p.ldo * (F32 ? 4 : 2);
+    const float rep = r.of(p.repetition, 1.0f), freq = r.of(p.frequency, 0.0f), pres = r.of(p.presence, 0.0f);
+#pragma unroll 1
+    for (int from = 0; from < SLICE; from += SLICE / 2) {
+        if (from) {
+            __syncthreads();                        // the first half's values have been taken
+#pragma unroll 1
+            for (int i = threadIdx.x; i < SLICE; i += kAdjustThreads) table[i] = 0u;
+        }
+        __syncthreads();
+        r.count(table, from, SLICE / 2, SLICE / 2);
+        __syncthreads();
+#pragma unroll 1
+        for (int at = threadIdx.x; at < SLICE / 2; at += kAdjustThreads) {
+            const uint32_t word = table[at];
+            if (word && adjust_open(mask, v0 + from + at)) r.change(x, y, F32 ? WS_ACT_F32 : WS_ACT_BF16, v0 + from + at, word, table[at + SLICE / 2], rep, freq, pres);
+        }
+    }
+}
+
 // VEC: rows are read and written 16 bytes at a time.  A row's values lie on a grid of vectors that begins at its first
 // aligned address or one vector before; values of the first and last vector that are not the row's are left alone.
 template <bool F32, bool VEC, int U, int BLOCKS>
@@ -147,9 +235,7 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
     }
     wait_predecessor();
     // ---- what the row's lists are, then the slice's logits, then the lists
-    int64_t a = 0, b = 0, bias0 = 0, bias1 = 0;
-    if (p.tokens) adjust_range(p.offsets, p.offset_bytes, t, p.n_tokens, a, b);
-    if (p.bias_ids) adjust_range(p.bias_offsets, p.bias_offset_bytes, t, p.n_bias, bias0, bias1);
+    const AdjustRow r(p, t, v0);
     const uint32_t *const mask = adjust_mask(p, t);
     const bool dense = mask || !p.in_place;         // (else only touched values change)
     uint32_t raw[U][4];
@@ -163,32 +249,10 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
                          : "l"(x + (int64_t)v * (F32 ? 4 : 2)), "r"((int)(dense && v >= 0 && v <= p.vocab - W)) : "memory");
         }
     }
-    const bool listed = bias1 > bias0 || b > a, packed = b - a <= kAdjustShort;     // (the block's conditions)
-    if (listed) {
-        const int low = max(v0, 0);                 // the slice's tokens: low and `width` behind it
-        const uint32_t width = (uint32_t)max(0, min(v0 + kSlice, p.vocab) - low);
-        uint32_t *const word = adjust_table + (low - v0);
+    const bool listed = r.bias1 > r.bias0 || r.b > r.a, halves = !p.bias_table && r.bias1 - r.bias0 > kAdjustFew;   // (the block's conditions)
+    if (listed && !halves) {
         __syncthreads();
-        if (bias1 > bias0)
-            adjust_list(p.bias_ids, bias0, bias1, [&](int64_t i, int32_t v) {
-                if ((uint32_t)(v - low) >= width) return;
-                atomicOr(&word[v - low], kAdjustListed);
-                if (p.bias_table) atomicMax(&word[v - low + kSlice], (uint32_t)(i - bias0) + 1u);
-            });
-        if (b > a) {
-            const int behind_at = p.prompt_lens ? p.prompt_lens[t] : 0;
-            const int64_t prompt = a + behind_at;
-            if (packed)
-                adjust_tokens(p.tokens + a, (int)(b - a), [&](int i, int32_t v) {
-                    if ((uint32_t)(v - low) < width) atomicAdd(&word[v - low], i < behind_at ? 0x10000u : 1u);
-                });
-            else
-                adjust_list(p.tokens, a, b, [&](int64_t i, int32_t v) {
-                    if ((uint32_t)(v - low) >= width) return;
-                    if (i < prompt) atomicOr(&word[v - low], kAdjustPrompt);
-                    else atomicAdd(&word[v - low], 1u);
-                });
-        }
+        r.count(adjust_table, 0, kSlice, p.bias_table ? kSlice : 0);
     }
     // ---- the logits under the mask
     if (dense) {
@@ -215,6 +279,7 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
         }
     }
     if (!listed) return;
+    if (halves) return adjust_halves<F32, kSlice>(p, adjust_table, t, v0);
     // ---- the touched places, a bit each of this thread's
     __syncthreads();
     uint64_t mine = 0u;
@@ -240,23 +305,13 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
     __syncthreads();
     // ---- their values.  (In place the mask has been at x already, which gives the same.)
     const int touched = touched_s, all = touched <= kAdjustList ? touched : kSlice;
-    const float rep = p.repetition && b > a ? p.repetition[t] : 1.0f, freq = p.frequency && b > a ? p.frequency[t] : 0.0f, pres = p.presence && b > a ? p.presence[t] : 0.0f;
+    const float rep = r.of(p.repetition, 1.0f), freq = r.of(p.frequency, 0.0f), pres = r.of(p.presence, 0.0f);
 #pragma unroll 1
     for (int i = tid; i < all; i += kAdjustThreads) {
         const int at = touched <= kAdjustList ? (int)list_s[i] : i, v = v0 + at;
         const uint32_t word = adjust_table[at];
         if (!word || !adjust_open(mask, v)) continue;
-        float z = load1(x, kType, v);
-        if (word & kAdjustListed) {                 // its last entry
-            int64_t e = bias0 + adjust_table[at + (p.bias_table ? kSlice : 0)];
-            if (!p.bias_table)
-                for (e = bias1; e > bias0 && p.bias_ids[e - 1] != v;) --e;
-            if (e > bias0) z += p.bias[e - 1];
-        }
-        const uint32_t behind = packed ? word & 0xFFFFu : word & (kAdjustPrompt - 1u);
-        if (word & ~kAdjustListed) z = z > 0.0f ? __fdiv_rn(z, rep) : z * rep;
-        if (behind) z = fmaf(-freq, (float)behind, z) - pres;
-        store1(y, kType, v, z);
+        r.change(x, y, kType, v, word, p.bias_table ? adjust_table[at + kSlice] : 0u, rep, freq, pres);
     }
 }
 

@@ -37,8 +37,9 @@ ws_status_t launch_route(const Err &err, int n, dim3 grid, void *stream, const R
 template <bool F32, bool VEC, int U, int BLOCKS>
 ws_status_t launch_adjust(const Err &err, AdjustParams &p, void *stream) {
     constexpr int W = F32 ? 4 : 8, slice = kAdjustThreads * U * W;
-    // The places of biases are looked for in the lists, or where these are long have a table of their own.
-    p.bias_table = p.n_bias / p.m > 128;
+    // The places of biases are looked for in the lists, or where these are long have a table of their own.  (A long list in a
+    // batch of short ones makes room for one in its blocks.)
+    p.bias_table = p.n_bias / p.m > kAdjustFew;
     const int smem = p.tokens || p.bias_ids ? slice * (p.bias_table ? 8 : 4) : 0;
     if (smem > 40 * 1024) {                         // (48 KB with the list)
         const ws_status_t st = allow_smem<adjust_kernel<F32, VEC, U, BLOCKS>>(err, slice * 8);
