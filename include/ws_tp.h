@@ -326,7 +326,7 @@ ws_status_t ws_lora_expand(const ws_lora_args_t *args, void *stream, char *err, 
  *   u = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight)      over a head's d values (norm = 0: u = x * weight)
  *   a' = scale (a cos - b sin), b' = scale (a sin + b cos)         angle = position * inv_freq[i], for the pairs
  *   (a, b) = (u[start + i], u[start + pairs + i]), or with interleaved (u[start + 2 i], u[start + 2 i + 1]);
- * the other values of u stay.  The angle is a product of 64 bits.  pairs = 0: no rotation (positions and inv_freq unused).
+ * the other values of u stay.  The angle is exact up to positions of 2^53.  pairs = 0: no rotation (positions and inv_freq unused).
  * q_out and k_out may be q and k themselves.  (Takes the place of the reference's `rmsnorm` and `rope` launches in front of its
  * attention.) */
 #define WS_MAX_PAIRS 1024

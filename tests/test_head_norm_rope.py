@@ -234,3 +234,29 @@ def test_starts_beyond_32_bits_are_refused(dev, start):
         ops.head_norm_rope(**{**a, "inv_freq": torch.ones(4, device=dev)}, rotary_start=start)
     q, _ = ops.head_norm_rope(torch.ones((3, 2, 16), device=dev), rotary_start=start)      # (without positions there is no part)
     assert (q - 1).abs().max() < 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,far", [(torch.int32, 2 ** 31), (torch.int64, 2 ** 31), (torch.int64, 2 ** 40), (torch.int64, 2 ** 53)])
+@pytest.mark.parametrize("d", [16, 14])
+def test_angles_of_far_positions(dev, dtype, far, d):
+    """Cosines and sines by themselves: heads of (1, 0) without a norm.  An argument of half a turn at most is rounded to 32 bits
+    (pi 2^-25, less than 2 u), cosine and sine err by 2 u, the products and the sum with zeros add a rounding each: 6 u.  The angle
+    itself is the oracle's to 2^-60: a rational number reduced by a pi of 75 digits."""
+    from fractions import Fraction
+
+    from weightstream_b200 import ops
+    rng = np.random.default_rng(far.bit_length() + d)
+    f, m = d // 2, 200
+    two_pi = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628")
+    positions = rng.integers(far - far // 4, far, m) * rng.choice([-1, 1], m)
+    inv = np.concatenate([[1.0, 0.5], 1.0 - rng.random(f - 2) * 0.9]).astype(np.float32)
+    q = torch.zeros((m, 1, d), device=dev)
+    q[:, :, :f] = 1.0
+    got, _ = ops.head_norm_rope(q, positions=torch.from_numpy(positions).to(dtype).to(dev), inv_freq=torch.from_numpy(inv).to(dev), norm=False)
+    got = got.double().cpu().numpy()[:, 0]
+    for t in range(m):
+        for i in range(f):
+            turn = int(positions[t]) * Fraction(float(inv[i])) / two_pi
+            angle = float((turn - round(turn)) * two_pi)
+            assert abs(got[t, i] - np.cos(angle)) <= 6 * U and abs(got[t, f + i] - np.sin(angle)) <= 6 * U, (positions[t], inv[i])

@@ -3,8 +3,8 @@
 //   u = x * rsqrt(mean(x^2) + eps) * (o + w)            over the d values of a head
 //   a' = s (a cos - b sin),  b' = s (a sin + b cos)     for the pairs (a, b) of u's rotated part, angle = position * inv_freq
 //
-// The angle is a product of 64 bits, reduced to a turn before its cosine is taken in 32, so that positions of millions
-// have the same error as the first ones.  A token's cosines and sines are computed once a team of threads and serve all
+// The angle is the whole product of position and frequency, in two numbers of 64 bits, reduced to a turn before its cosine is
+// taken in 32, so that positions up to 2^53 have the same error as the first ones.  A token's cosines and sines are computed once a team of threads and serve all
 // its heads: a lane keeps them, times the weights, for the pairs that it has of every head.
 //
 // Bound: HBM for many tokens (8192 tokens of 64 and 8 heads of 128 bf16 values 63 us, 4.8 TB/s; 12 instructions a value before
@@ -35,7 +35,10 @@ __device__ __forceinline__ void heads_angles(const HeadsParams &p, int t, int ti
     if (!p.pairs || t >= p.m) return;
     const double at = p.position_bytes == 8 ? (double)static_cast<const int64_t *>(p.positions)[t] : (double)static_cast<const int32_t *>(p.positions)[t];
     for (int i = tid; i < p.pairs; i += threads) {
-        double turns = at * (double)p.inv_freq[i] * 0.15915494309189533577;     // 1 / (2 pi)
+        // at * f = whole + rest exactly, and 1 / (2 pi) in two numbers: what is lost is below 2^-52 of a turn.
+        constexpr double kTurn = 0.15915494309189535, kTurnRest = -9.839338337591243e-18;
+        const double f = (double)p.inv_freq[i], whole = at * f, rest = fma(at, f, -whole);
+        double turns = fma(whole, kTurn, -rint(whole * kTurn)) + fma(whole, kTurnRest, rest * kTurn);
         turns -= rint(turns);
         float s, c;
         sincospif((float)(2.0 * turns), &s, &c);

@@ -555,8 +555,8 @@ def head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positio
 
     for the ``len(inv_freq)`` pairs of the part that begins at ``rotary_start``: value i and the one ``len(inv_freq)`` behind it,
     or with ``interleaved`` neighbours.  Values outside the part keep ``u``.  Without weights they count as one and
-    ``weight_offset`` is not added; ``norm=False`` leaves the norm out, no ``positions`` the rotation.  The angle is a product of
-    64 bits, so positions (int32 or int64) may be millions; everything else between the loads and the one rounding is held in 32.
+    ``weight_offset`` is not added; ``norm=False`` leaves the norm out, no ``positions`` the rotation.  The angle is exact for
+    positions (int32 or int64) up to 2^53; everything else between the loads and the one rounding is held in 32 bits.
 
     Returns ``(q', k')`` of the inputs' type, contiguous or in ``q_out`` and ``k_out``, which may be ``q`` and ``k`` themselves.
     """
