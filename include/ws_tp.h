@@ -323,7 +323,7 @@ ws_status_t ws_lora_shrink(const ws_lora_args_t *args, void *stream, char *err, 
 ws_status_t ws_lora_expand(const ws_lora_args_t *args, void *stream, char *err, size_t err_len);
 
 /* Norms of queries and keys, head by head, and the rotation of positions:
- *   u = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight)      over a head's d values (norm = 0: u = x * weight)
+ *   u = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight)      over a head's d values (norm = 0: x * (weight_offset + weight))
  *   a' = scale (a cos - b sin), b' = scale (a sin + b cos)         angle = position * inv_freq[i], for the pairs
  *   (a, b) = (u[start + i], u[start + pairs + i]), or with interleaved (u[start + 2 i], u[start + 2 i + 1]);
  * the other values of u stay.  The angle is exact up to positions of 2^53.  pairs = 0: no rotation (positions and inv_freq unused).
@@ -369,9 +369,13 @@ ws_status_t ws_moe_route(const ws_moe_route_args_t *args, void *stream, char *er
  *   out[t] = sum over t's routes (in the order of their slots) of w2[e] (weight * silu(g) * u)
  * Weights are packed E2M1 (low nibble = even K) with a UE8M0 byte per 32 values of K, as in ws_moe_down_combine_allreduce,
  * every expert's rows one after the other; experts lie w1_stride .. s2_stride bytes apart, so W1 and W3 may be halves of one
- * tensor.  Scale byte 0 counts as 0, 255 gives infinities or NaN.  Routes to experts outside [e_start, e_start + e_len), such as
+ * tensor.  Scale byte 0 counts as 0, 255 gives infinities or NaN, as bytes above 222 (2^95) may: sums are held in fp32 in units of a
+ * row's largest activation.  Routes to experts outside [e_start, e_start + e_len), such as
  * -1, are other ranks': out then is this rank's part of the sum (ws_allreduce_f32).
- * Activations are not rounded (act_quant 0), or x and the weighted hidden are rounded as the fused steps do (1).
+ * act_quant 0: bf16 activations are held as they are, fp32 ones and the weighted hidden in 22 bits or more, both down to 2^-17 of their
+ * row's largest (bf16: 2^-29) and below that to 2^-40 of it.  1: x and the weighted hidden are rounded as the fused steps do.
+ * Routes and weights may be what the kernel in front of the call on its stream writes; as long as the call runs nothing may
+ * change them (the second kernel reads them before the first has ended).
  * hidden and inter are multiples of 32; weights, scales and strides are multiples of 16 bytes.
  * At most 512 routes (m * top_k), 512 local experts, top_k 8 and widths of 24576 (WS_ERR_CAPACITY beyond).  The workspace
  * (ws_moe_layer_workspace bytes, 16-byte aligned) is written first, so calls on one stream may share it. */
@@ -401,7 +405,8 @@ ws_status_t ws_moe_layer(const ws_moe_layer_args_t *args, void *stream, char *er
  *   z = -inf                                       where the row's mask has no bit for the token
  * Row t's history is tokens[offsets[t] .. offsets[t + 1]), its biases likewise; offsets outside [0, n_tokens] are taken to its
  * ends, and tokens outside [0, vocab) ignored.  Bit v % 32 of word v / 32 of a mask allows token v; row t uses mask row
- * mask_rows[t] (NULL: t), and none if that is outside [0, mask_count).  out may be logits itself. */
+ * mask_rows[t] (NULL: t).  A row whose mask row is outside [0, mask_count), such as -1, has no mask: all its tokens are allowed.  out may
+ * be logits itself. */
 typedef struct {
     const void *logits;       /* [m, vocab], row stride ld (elements)               */
     int64_t ld;

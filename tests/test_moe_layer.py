@@ -356,3 +356,36 @@ def test_the_smallest_limits(dev):
     for limit in (1e-46, 5e-324):
         with pytest.raises(ValueError, match="limit"):
             l.call(limit=limit)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_weights_and_routes_written_just_before_the_call(dev, captured):
+    """What another kernel wrote in front of the call counts, for the second kernel too, which reads its weights early."""
+    a, b = (Layer(seed, 5, 512, 256, 6, 3, dev, others=0.0) for seed in (21, 22))
+    want = [a.check(), b.check()]
+    own = Layer(23, 5, 512, 256, 6, 3, dev)
+    outs = [torch.empty_like(want[0]) for _ in range(40)]
+
+    def run():
+        for i, out in enumerate(outs):
+            l = (a, b)[i % 2]
+            for to, at in zip([own.x, own.w, *own.weights, own.ids], [l.x, l.w, *l.weights, l.ids]):
+                to.copy_(at)
+            own.call(out=out)
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        graph.replay()
+    else:
+        run()
+    assert all(torch.equal(out, want[i % 2]) for i, out in enumerate(outs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,top_k,dtype,how", [(2, 4, 3, BF16, {}), (12, 3, 2, BF16, {}), (6, 3, 2, F32, {}), (5, 3, 2, F32, dict(act_quant=True, limit=10.0, out_dtype=BF16))])
+def test_a_served_size(dev, m, n, top_k, dtype, how):
+    """Many units of long rows: warps share K in the first kernel, units of several passes in every block."""
+    Layer(m + n, m, 7168, 2048, n, top_k, dev, dtype, others=0.1).check(**how)

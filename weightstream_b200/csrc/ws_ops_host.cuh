@@ -44,7 +44,8 @@ ws_status_t allow_smem(const Err &err, int bytes) {
     return e == cudaSuccess ? WS_OK : err(WS_ERR_CUDA, "%d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
 }
 
-// The kernels begin with griddepcontrol.wait, so their launch may overlap the end of the kernel before them.
+// The kernels wait for the one before them (griddepcontrol.wait) before they read what it may have written, so their launch
+// may overlap its end.  (One of a call's own kernels may read earlier what the call's first one has waited for.)
 template <typename P>
 ws_status_t launch(const Err &err, void (*kernel)(P), dim3 grid, unsigned threads, size_t smem, unsigned cluster, void *stream, const P &params) {
     cudaLaunchConfig_t cfg{};

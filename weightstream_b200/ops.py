@@ -447,7 +447,8 @@ def adjust_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None
     [m] (1, 0 and 0 without them).  Its biases are ``bias[j]`` (fp32) of ``bias_ids[j]`` (int32) for ``j`` from
     ``bias_offsets[t]`` to ``bias_offsets[t + 1]``; of a token that is listed twice the last entry counts.  Tokens outside
     [0, vocab), such as -1 for padding, are ignored.  ``mask`` is int32 [masks, words >= ceil(vocab / 32)], bit ``v % 32`` of word
-    ``v // 32`` allows token ``v``; row ``t`` uses mask row ``mask_rows[t]`` (int32 [m], -1: no mask), or ``t`` without it.
+    ``v // 32`` allows token ``v``; row ``t`` uses mask row ``mask_rows[t]`` (int32 [m]), or ``t`` without it.  A row whose mask row is
+    outside [0, masks), such as -1, has no mask: all its tokens are allowed, so an index of a mask that is gone turns a grammar off.
 
     Returns ``out``, of the logits' type, which may be ``logits`` itself.  A row that no token is left of is -inf throughout;
     NaN stays NaN.
@@ -695,9 +696,12 @@ def moe_layer(x: torch.Tensor, route_ids: torch.Tensor, route_w: torch.Tensor, w
     ``route_ids`` int32 and ``route_w`` fp32 [m, top_k] are those of :func:`moe_route`; this rank holds the experts from ``e_start``
     on, and routes to others, such as -1, count nothing: the result is then this rank's part, for ``Endpoint.allreduce_``.
 
-    Activations are not rounded on the way; ``act_quant`` rounds x and the weighted hidden to E4M3 with a power of two for 32
-    values, as the fused steps and the reference do.  Sums are fp32, a token's routes are added in the order of its slots.  At most
-    512 routes (m * top_k) of top_k 8, 512 experts and widths of 24576; more raise ``WsError``.  Returns ``out`` [m, hidden], fp32 or ``out_dtype``.
+    bf16 activations are held as they are, fp32 ones and the weighted hidden in 22 bits or more, down to 2^-17 of their row's
+    largest value (bf16: 2^-29) and below that to 2^-40 of it; ``act_quant`` rounds x and the weighted hidden to E4M3 with a power of
+    two for 32 values, as the fused steps and the reference do.  Sums are fp32, in units of a row's largest activation, so scale bytes
+    above 222 (2^95) may give infinities; a token's routes are added in the order of its slots.  At most 512 routes (m * top_k) of
+    top_k 8, 512 experts and widths of 24576; more raise ``WsError``.  Routes and weights may be written by what stands in front of the
+    call on its stream.  Returns ``out`` [m, hidden], fp32 or ``out_dtype``.
     """
     r = (_native or _load()).moe_layer(x, route_ids, route_w, w1, s1, w3, s3, w2, s2, e_start, 0.0 if limit is None else limit or -1.0, act_quant,
                                      out, out_dtype, _handle(stream, x))
