@@ -327,3 +327,37 @@ def test_one_long_list_among_many_rows_takes_no_longer_than_it_is(dev):
         return min(times)
 
     assert elapsed(a) < 8 * elapsed(b), (elapsed(a), elapsed(b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,vocab,length,others", [(3, 129, 192, 0), (3, 129, 193, 0), (20, 700, 1000, 3), (4, 33000, 250, 0), (40, 20003, 2000, 7), (200, 20003, 9000, 2),
+                                                   (600, 4111, 30000, 0), (25, 129280, 1500, 1)])
+@pytest.mark.parametrize("pad", [0, 5])
+def test_one_long_list_in_a_batch_of_short_ones(dev, dtype, m, vocab, length, others, pad):
+    """No more than 64 biases a row on average, so a long list's places share the table of the counts."""
+    for row, how in ((m - 1, {}), (0, dict(history=0)), (1, dict(masks=0))):
+        a = lopsided(m + length, m, vocab, length, dtype, dev, others=others, pad=pad, row=row, **how)
+        assert a["bias"].shape[0] // m <= 64
+        got = check(a)
+        b = {**a, "logits": a["logits"].clone()}
+        assert torch.equal(check(b, out=b["logits"]), got)
+
+
+@pytest.mark.gpu
+def test_the_last_entry_counts_in_a_long_list_among_short_ones(dev):
+    for m, length in ((40, 193), (128, 5000)):
+        a = lopsided(17, m, 3000, length, F32, dev, history=0, masks=0)
+        a["bias_ids"][:] = torch.arange(length, dtype=torch.int32, device=dev) % 3
+        check(a)
+
+
+@pytest.mark.gpu
+def test_long_histories_beside_a_long_list(dev):
+    """A history beyond 32767 tokens is counted in wider fields, in both halves."""
+    a = lopsided(19, 30, 20003, 1500, BF16, dev, row=2, history=30)
+    n = 40000
+    a["tokens"] = torch.cat([a["tokens"][:0], torch.randint(0, 20003, (n,), dtype=torch.int32, device=dev), torch.full((n,), 11, dtype=torch.int32, device=dev)])
+    a["offsets"] = torch.tensor([0, 0, 0] + [2 * n] * 28, dtype=torch.int32, device=dev)
+    a["prompt_lens"][2] = n // 2
+    check(a)

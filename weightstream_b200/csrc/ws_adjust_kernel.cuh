@@ -15,8 +15,8 @@
 // clusters of a row's slices that count into each other's tables 19, 52 and 169; a plain copy, and a hash table a row beside
 // or behind it 12, 33 and 91.
 //
-// Bound: instructions.  One row of 129280 with 6000 tokens 6.2 to 7.1 us, 64 rows with 4000, a mask and biases 27 us (10.3 of HBM),
-// 512 bf16 rows with 2000 and masks 85 us (41; one call after the other 84, without lists 43, with lists of -1 69): a block's fixed part,
+// Bound: instructions.  One row of 129280 with 6000 tokens 6.2 to 7.1 us, 64 rows with 4000, a mask and biases 26 to 27 us (10.3 of HBM),
+// 512 bf16 rows with 2000 and masks 83 to 85 us (41; one call after the other 83 to 84, without lists 43, with lists of -1 69): a block's fixed part,
 // the lists that each of a row's sixteen blocks looks through, and the mask's bits.
 #pragma once
 
@@ -34,6 +34,10 @@ constexpr int kAdjustShort = 32767;
 // table.  Lists of 32, 64 and 128 in all rows, us, looked through / in a second table: 64 fp32 rows 15.2 / 15.2, 19.3 / 15.6
 // and 28 / 15.6, 512 bf16 rows with 2000 tokens each 91 / 118, 114 / 120 and 166 / 122.
 constexpr int kAdjustFew = 64;
+// The same for a row's own list in a batch of shorter ones, which costs more: it is gone through twice, with the row's tokens.  Every
+// fourth row with a list of 128, 192 or 250, looked through / in halves: 64 fp32 rows 18.2 / 13.7, 22.5 / 14.3 and 26.5 / 14.6 us,
+// 512 bf16 rows with 2000 tokens each 102 / 116, 121 / 118 and 142 / 119.
+constexpr int kAdjustLong = 192;
 
 struct AdjustParams {
     const void *logits;
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kAdjustThreads, BLOCKS) adjust_kernel(const __
                          : "l"(x + (int64_t)v * (F32 ? 4 : 2)), "r"((int)(dense && v >= 0 && v <= p.vocab - W)) : "memory");
         }
     }
-    const bool listed = r.bias1 > r.bias0 || r.b > r.a, halves = !p.bias_table && r.bias1 - r.bias0 > kAdjustFew;   // (the block's conditions)
+    const bool listed = r.bias1 > r.bias0 || r.b > r.a, halves = !p.bias_table && r.bias1 - r.bias0 > kAdjustLong;   // (the block's conditions)
     if (listed && !halves) {
         __syncthreads();
         r.count(adjust_table, 0, kSlice, p.bias_table ? kSlice : 0);
