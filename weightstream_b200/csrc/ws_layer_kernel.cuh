@@ -148,12 +148,16 @@ struct LayerPlan {
 };
 
 // What a unit of a pass of n routes costs, in fortieths: an SM's part of HBM while the columns' loads and products are hidden
-// by it (24 experts of 7168 x 2048, all with n routes, n = 1, 4, 8: first kernel 66, 68, 73 us; second 35, 36, 53).
+// by it (24 experts of 7168 x 2048, all with n routes, n = 1, 4, 8: first kernel 66, 68, 73 us; second 35, 36, 53).  With one cost
+// for all: 96 routes of 48 experts of 7168 x 2048 211 us instead of 197, 256 routes of 32 of 1024 x 512 39 instead of 33, others within 6 %.
 template <bool FIRST>
 __device__ __forceinline__ int layer_cost(const LayerParams &p, int n) { return FIRST ? 40 + n / 2 : n <= 4 ? 40 : 57; }
 
 // Warps that share a unit by K, for units of this cost together: the more, the less the warps wait for the last one at the
-// end; the fewer, the less often they join their sums.
+// end; the fewer, the less often they join their sums.  One warp a unit everywhere, us: 12 routes of 24 experts of 7168 x 2048 66 instead
+// of 63, 128 routes of 64 of 7168 x 256 71 instead of 67; but 128 routes of 32 of 4096 x 1536 88 instead of 100, 32 routes of 64 of 1024 x
+// 512 21 instead of 24, so the rule is not the best one for all widths.  Four everywhere: slower throughout, 140 instead of 89 with 512
+// routes of 128 of 2048 x 768.
 template <bool FIRST>
 __device__ __forceinline__ int layer_group(const LayerParams &p, int64_t all) {
     const int chunks = (p.k + kLayerChunk - 1) / kLayerChunk, each = (int)(all / gridDim.x) / layer_cost<FIRST>(p, 1);    // units a block

@@ -9,7 +9,7 @@
 // largest score of the token, chosen or not: a bias may cancel a score of any size and leave its rounding.
 // Experts whose logit is -inf or NaN are never chosen; places that stay empty hold id -1 and weight 0.
 //
-// Bound: instructions (4096 tokens of 384 experts with a bias, top 8: 20 to 21 us, 1600 of them
+// Bound: instructions (4096 tokens of 384 experts with a bias, top 8: 19 to 21 us, 1600 of them
 // a token; HBM would need 1), the launch for few (64 tokens 5.1 us a call).
 #pragma once
 
