@@ -30,8 +30,8 @@ constexpr int kAdjustList = 2048;                   // touched places that are n
 // histories: 30 an occurrence in the prompt, 29 to 0 occurrences behind it.
 constexpr uint32_t kAdjustListed = 0x80000000u, kAdjustPrompt = 0x40000000u;
 constexpr int kAdjustShort = 32767;
-// A row's list of biases is looked through for each of its listed values up to this length; longer ones have their places in a
-// table.  Lists of 32, 64 and 128 in all rows, us, looked through / in a second table: 64 fp32 rows 15.2 / 15.2, 19.3 / 15.6
+// Lists of biases are looked through for each of a row's listed values up to this length, on average over the batch; longer ones
+// have their places in a table.  Lists of 32, 64 and 128 in all rows, us, looked through / in a second table: 64 fp32 rows 15.2 / 15.2, 19.3 / 15.6
 // and 28 / 15.6, 512 bf16 rows with 2000 tokens each 91 / 118, 114 / 120 and 166 / 122.
 constexpr int kAdjustFew = 64;
 // The same for a row's own list in a batch of shorter ones, which costs more: it is gone through twice, with the row's tokens.  Every
