@@ -25,8 +25,8 @@
 //
 // Bound: HBM, and what stands before the streams.  One token of 7168 x 2048 through six experts 43 us, of which HBM needs 21:
 // routes, plan and activations 8, W1 and W3 17 (5.6 TB/s), the second kernel's beginning 7, W2 9 (5.1 TB/s), the sum 2.  48
-// routes of 30 experts 165 to 170 us (107), 96 of 42 233 to 238 us (150), fp32 activations rounded to E4M3, 28 routes of 20 experts of 5120
-// x 2304, 104 us (57).  At HBM's rate the issue slots, the conversions of codes and shared memory are each half to three
+// routes of 30 experts 165 to 173 us (107), 96 of 42 233 to 241 us (150), fp32 activations rounded to E4M3, 28 routes of 20 experts of 5120
+// x 2304, 103 to 106 us (57).  At HBM's rate the issue slots, the conversions of codes and shared memory are each half to three
 // quarters busy: 30 instructions a lane for 16 codes, of which 8 convert, 2 multiply and 4 add.
 //
 // mma.sync and not tcgen05: its block-scaled form takes activations of 8 bits at most, so that a bf16 value held exactly
